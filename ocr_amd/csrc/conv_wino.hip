@@ -43,24 +43,13 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 
-// Packed f32 arithmetic as inline assembly: one instruction for two floats at the price of one.  Written as vector
-// expressions the compiler selects the same instructions but splits them into scalar ones again wherever MFMAs are
-// near, which doubles the vector-ALU time between the MFMAs.
+// Arithmetic on two floats, one scalar instruction each: the packed float32 instructions that would do both at once have
+// given wrong results on MI355X now and then, and the library is built without them.
 __device__ __forceinline__ floatx2 pk_fma(floatx2 a, floatx2 b, floatx2 c) {
-    floatx2 d;
-    asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
+    return floatx2{__builtin_fmaf(a.x, b.x, c.x), __builtin_fmaf(a.y, b.y, c.y)};
 }
-__device__ __forceinline__ floatx2 pk_add(floatx2 a, floatx2 b) {
-    floatx2 d;
-    asm("v_pk_add_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-    return d;
-}
-__device__ __forceinline__ floatx2 pk_sub(floatx2 a, floatx2 b) {
-    floatx2 d;
-    asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(d) : "v"(a), "v"(b));
-    return d;
-}     // arithmetic on these compiles to packed f32 instructions
+__device__ __forceinline__ floatx2 pk_add(floatx2 a, floatx2 b) { return a + b; }
+__device__ __forceinline__ floatx2 pk_sub(floatx2 a, floatx2 b) { return a - b; }
 
 constexpr int kCK = 8;            // input channels per chunk
 constexpr int kRS = 12;           // floats per raw pixel in LDS (8 + pad: conflict-free 16-byte reads)
