@@ -358,6 +358,82 @@ int ocrhip_ctc_beam_search(ocrhip_handle h, const float* d_logits, int B, int T,
                            const int* d_row0, int blank, int num_beams, int* d_tokens, float* d_scores,
                            ocrhip_stream stream);
 
+/* ------------------------------------------------------------- 8-bit products, distillation --
+ * Operators for a recogniser whose dense layers multiply 8-bit floating point blocks, and for the distance of such a
+ * (student's) logits from the float32 recogniser's (teacher's).  No counterpart in the reference.  All of them check
+ * their arguments before anything else, allocate nothing, keep nothing of the handle's between calls (two calls on two
+ * streams, or in two captured graphs, share no memory) and leave the current device as it was.
+ *
+ * Block-scaled 8-bit matrix of R rows and C columns: row r at d_q + r * ld_q, OCP e4m3 bytes (8 bits, no infinities),
+ * the columns from C up to the next multiple of 128 zero; the scale of the block (row block i, column block j) is the
+ * byte d_scale[j * ld_scale + i] = exponent + 127, column blocks being 128 columns and row blocks `block_rows` rows (1 or
+ * 128): the element (r, c) stands for q[r][c] * 2^(d_scale[(c / 128) * ld_scale + r / block_rows] - 127).
+ *   ld_q: multiple of 128, >= C;  ld_scale: multiple of 16, >= the number of row blocks;  both pointers 16-byte aligned.
+ *
+ * ocrhip_quantize_fp8: x (rows, cols), or its transpose, as such a matrix.  The exponent of a block is the least e with
+ * amax <= 448 * 2^e, amax over the finite values of the block (0 for a block without any but zeros; at least -127);
+ * values are rounded to nearest, ties to even; infinities and NaN become NaN.
+ *   d_x    : device float32 or bfloat16 (x_dtype), row r at d_x + r * ld_x elements
+ *   d_q    : (R, ld_q) bytes with R = transpose ? cols : rows; every row is written up to its columns rounded up to 128
+ *   d_scale: (ceil(C / 128), ld_scale) bytes, the first ceil(R / block_rows) of a row are written
+ * rows == 0 or cols == 0: nothing is written. */
+int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x,
+                        int block_rows, int transpose, uint8_t* d_q, int64_t ld_q, uint8_t* d_scale, int64_t ld_scale,
+                        ocrhip_stream stream);
+
+/* ocrhip_gemm_fp8: C (M, N) = A (M, K) . B (N, K)^T + bias, C float32 or bfloat16.  A has a scale per row and 128 values
+ * of k (block_rows 1), B per row or per 128 rows (b_block_rows 1 or 128).  A NaN in a row of A or B makes that row or
+ * column of C NaN.  The sums of one call always run in the same order; they are float32, but for one step of a bfloat16
+ * result: the 8-bit matrix instruction drops what lies 2^-13 below the largest product among up to 16 neighbours in k.
+ * For a float32 result operand values (bytes times scale) below 2^-126 in magnitude count as 0 and from 2^128 on as
+ * infinite.
+ *   d_bias: device float32 (N) or NULL;  d_c: row m at d_c + m * ld_c elements, ld_c >= N;  M >= 0, N >= 0, K >= 1
+ *   d_ws  : device scratch of ocrhip_gemm_fp8_workspace(M, N, K) bytes, 16-byte aligned (NULL when that is 0); what it
+ *           holds before and after the call does not matter, calls that overlap need one each */
+size_t ocrhip_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K);
+int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uint8_t* d_a_scale, int64_t ld_a_scale,
+                    const uint8_t* d_b, int64_t ld_b, const uint8_t* d_b_scale, int64_t ld_b_scale, int b_block_rows,
+                    int64_t M, int64_t N, int64_t K, const float* d_bias, void* d_c, int c_dtype, int64_t ld_c, void* d_ws,
+                    size_t ws_bytes, ocrhip_stream stream);
+
+/* ocrhip_linear_fp8: the same with A given as float32 or bfloat16 values, which the call quantises by rows (block_rows 1)
+ * exactly as ocrhip_quantize_fp8 does: a Dense layer on 8-bit weights, from single time steps on.
+ *   d_x : device (M, K), row m at d_x + m * ld_x elements;  d_ws: ocrhip_linear_fp8_workspace(M, N, K) bytes */
+size_t ocrhip_linear_fp8_workspace(int64_t M, int64_t N, int64_t K);
+int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_x, const uint8_t* d_b, int64_t ld_b,
+                      const uint8_t* d_b_scale, int64_t ld_b_scale, int b_block_rows, int64_t M, int64_t N, int64_t K,
+                      const float* d_bias, void* d_c, int c_dtype, int64_t ld_c, void* d_ws, size_t ws_bytes,
+                      ocrhip_stream stream);
+
+/* ocrhip_top_logits: the K largest logits of every row, in descending order (the lower class first among equals; a NaN
+ * ranks above every number, as in a descending sort), and the row's log normaliser at a temperature.
+ *   d_logits: device float32 or bfloat16 (dtype), row r at d_logits + r * ld elements, V classes, 1 <= V <= 262144
+ *   d_values: device (rows, K) float32;  d_index: device (rows, K) int32;  1 <= K <= 64, K <= V
+ *   d_lse   : device (rows) float32 = log sum_v exp(logit_v / temperature), or NULL;  temperature > 0, finite */
+int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t rows, int V, int64_t ld, int K,
+                      float temperature, float* d_values, int* d_index, float* d_lse, ocrhip_stream stream);
+
+/* ocrhip_distill_loss: distillation loss of a student's logits s against the K entries (class, logit) of a teacher per
+ * row, and its gradient in the same pass.  With q = softmax(s / temperature):
+ *   d_top_lse == NULL: p = softmax of the entries' logits / temperature;
+ *       loss = weight * temperature^2 * sum_k p_k log(p_k / q_k),  grad_v = weight * temperature * (q_v - p_v)
+ *   d_top_lse (the teacher's log normaliser at this temperature, as ocrhip_top_logits returns it): p_k = exp(logit_k /
+ *       temperature - lse), everything outside the entries is one more class with p_rest = max(0, 1 - sum p_k) and q_rest
+ *       = the sum of q there (none when the entries name all V classes);  loss as above plus p_rest log(p_rest / q_rest),
+ *       grad_v = weight * temperature * q_v * (1 - p_rest / q_rest) outside the entries
+ * An entry whose class lies outside [0, V) is none, one whose logit is -infinity has p_k = 0; several entries of one
+ * class add up.  Without d_top_lse a row whose entries carry no probability (none, or all -infinity) has loss 0 and
+ * gradient 0.  A row with weight 0 has both 0 and is not read.  A class with p > 0 and q = 0 makes the loss +infinity.
+ * A NaN or +infinity among the logits or the entries' values makes the row's loss and gradient NaN.
+ *   d_logits    : device float32 or bfloat16 (dtype), row r at d_logits + r * ld elements, 1 <= V <= 262144
+ *   d_top_values: device (rows, K) float32, d_top_index: device (rows, K) int32, in any order;  1 <= K <= 64
+ *   d_row_weight: device (rows) float32 or NULL (1);  d_loss: device (rows) float32 or NULL
+ *   d_grad      : of d_logits' type, row r at d_grad + r * ld_grad elements, or NULL; must not overlap d_logits */
+int ocrhip_distill_loss(ocrhip_handle h, const void* d_logits, int dtype, int64_t rows, int V, int64_t ld,
+                        const float* d_top_values, const int* d_top_index, int K, const float* d_top_lse,
+                        float temperature, const float* d_row_weight, float* d_loss, void* d_grad, int64_t ld_grad,
+                        ocrhip_stream stream);
+
 /* ------------------------------------------------------------------------------ stage timers --
  * Per-kernel device timing with HIP events recorded on the caller's stream around every launch the
  * library makes.  Replaces the hierarchical @timer / Timer instrumentation that wraps every stage of

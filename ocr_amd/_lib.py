@@ -12,8 +12,8 @@ OCRHIP_OK, OCRHIP_EINVAL, OCRHIP_ECAP, OCRHIP_EHIP, OCRHIP_ESTATE = 0, -1, -2, -
 F32, BF16, U8 = 0, 1, 2
 MERGE_UNION, MERGE_AVERAGE, MERGE_WEIGHTED = 0, 1, 2
 
-c_int, c_float, c_void_p, c_char_p, c_int64 = (ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p,
-                                                ctypes.c_int64)
+c_int, c_float, c_void_p, c_char_p, c_int64, c_size_t = (ctypes.c_int, ctypes.c_float, ctypes.c_void_p,
+                                                          ctypes.c_char_p, ctypes.c_int64, ctypes.c_size_t)
 
 
 class TensorDesc(ctypes.Structure):
@@ -62,6 +62,18 @@ SIGNATURES = {
                                   c_void_p]),
     'ocrhip_ctc_beam_search': (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p,
                                        c_void_p, c_void_p]),
+    'ocrhip_quantize_fp8': (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_int64,
+                                    c_void_p, c_int64, c_void_p]),
+    'ocrhip_gemm_fp8_workspace': (c_size_t, [c_int64, c_int64, c_int64]),
+    'ocrhip_gemm_fp8': (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                                c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
+    'ocrhip_linear_fp8_workspace': (c_size_t, [c_int64, c_int64, c_int64]),
+    'ocrhip_linear_fp8': (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64,
+                                  c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
+    'ocrhip_top_logits': (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_int, c_float, c_void_p, c_void_p,
+                                  c_void_p, c_void_p]),
+    'ocrhip_distill_loss': (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p,
+                                    c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     'ocrhip_profile_enable': (c_int, [c_void_p, c_int]),
     'ocrhip_profile_collect': (c_int, [c_void_p, ctypes.POINTER(KernelStat), c_int, ctypes.POINTER(c_int)]),
 }

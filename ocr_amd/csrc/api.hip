@@ -1217,6 +1217,163 @@ int ocrhip_ctc_beam_search(ocrhip_handle h, const float* d_logits, int B, int T,
     return launch_ctc_beam(h, d_logits, B, T, V, d_lengths, d_row0, blank, num_beams, d_tokens, d_scores, (hipStream_t)stream);
 }
 
+// ------------------------------------------------------------------------------------------ 8-bit products, distillation
+
+// These entry points put the handle's device in place for the call only.
+namespace {
+struct DeviceScope {
+    int before = -1;
+    DeviceScope() { if (hipGetDevice(&before) != hipSuccess) before = -1; }
+    ~DeviceScope() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// one past the last byte of `rows` rows of `row_bytes` bytes, `ld_bytes` apart
+bool overlap(const void* a, int64_t a_rows, int64_t a_ld, int64_t a_row, const void* b, int64_t b_rows, int64_t b_ld, int64_t b_row) {
+    if (!a || !b || a_rows == 0 || b_rows == 0) return false;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    return a0 < b0 + (uintptr_t)((b_rows - 1) * b_ld + b_row) && b0 < a0 + (uintptr_t)((a_rows - 1) * a_ld + a_row);
+}
+
+constexpr int64_t kMaxExtent = 1ll << 40;       // keeps every byte offset far inside int64
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t esize(int dtype) { return dtype == OCRHIP_F32 ? 4 : 2; }
+
+int check_values(const char* who, const char* what, const void* p, int dtype, int64_t rows, int64_t cols, int64_t ld) {
+    OCR_REQUIRE(dtype == OCRHIP_F32 || dtype == OCRHIP_BF16, "%s: %s must be F32 or BF16 (dtype %d)", who, what, dtype);
+    OCR_REQUIRE(rows >= 0 && cols >= 0 && rows < (1ll << 31) && cols < (1ll << 31), "%s: %s has %lld rows and %lld columns", who, what, (long long)rows, (long long)cols);
+    OCR_REQUIRE(ld >= cols && ld < kMaxExtent && (rows == 0 || ld == 0 || rows <= kMaxExtent / ld), "%s: rows of %s are %lld elements apart (%lld rows of %lld)", who, what, (long long)ld, (long long)rows, (long long)cols);
+    OCR_REQUIRE(rows == 0 || cols == 0 || p, "%s: %s is null", who, what);
+    OCR_REQUIRE(aligned(p, (uintptr_t)esize(dtype)), "%s: %s is not aligned to its elements", who, what);
+    return OCRHIP_OK;
+}
+
+int check_blocks(const char* who, const char* what, const uint8_t* q, int64_t ld, const uint8_t* scale, int64_t ld_scale, int block_rows, int64_t rows, int64_t cols) {
+    OCR_REQUIRE(block_rows == 1 || block_rows == 128, "%s: %s has a scale per %d rows (1 or 128)", who, what, block_rows);
+    OCR_REQUIRE(rows >= 0 && cols >= 0 && rows < (1ll << 31) && cols < (1ll << 31), "%s: %s has %lld rows and %lld columns", who, what, (long long)rows, (long long)cols);
+    OCR_REQUIRE(ld % 128 == 0 && ld >= cols && ld < kMaxExtent && (rows == 0 || ld == 0 || rows <= kMaxExtent / ld), "%s: row stride %lld of %s must be a multiple of 128 and at least its %lld columns", who, (long long)ld, what, (long long)cols);
+    OCR_REQUIRE(ld_scale % 16 == 0 && ld_scale >= (rows + block_rows - 1) / block_rows && ld_scale < (1ll << 32),
+                "%s: scale row stride %lld of %s must be a multiple of 16 and at least its number of row blocks", who, (long long)ld_scale, what);
+    OCR_REQUIRE(rows == 0 || cols == 0 || (q && scale), "%s: %s is null", who, what);
+    OCR_REQUIRE(aligned(q, 16) && aligned(scale, 16), "%s: %s must be 16-byte aligned", who, what);
+    return OCRHIP_OK;
+}
+
+int check_product(const char* who, int64_t M, int64_t N, int64_t K, const float* bias, void* c, int c_dtype, int64_t ld_c, const void* ws, size_t ws_bytes, size_t need) {
+    OCR_REQUIRE(K >= 1, "%s: K must be at least 1 (got %lld)", who, (long long)K);
+    OCR_TRY(check_values(who, "the output", c, c_dtype, M, N, ld_c));
+    OCR_REQUIRE(aligned(bias, 4), "%s: the bias is not aligned to its elements", who);
+    OCR_REQUIRE(need == 0 || M == 0 || N == 0 || (ws && aligned(ws, 16)), "%s: needs a 16-byte aligned workspace of %zu bytes", who, need);
+    if (M && N && ws_bytes < need) {
+        set_error("%s: the workspace has %zu bytes, %zu are needed", who, ws_bytes, need);
+        return OCRHIP_ECAP;
+    }
+    return OCRHIP_OK;
+}
+
+int check_rows(const char* who, const void* x, int dtype, int64_t rows, int V, int64_t ld, int K, float temperature) {
+    OCR_REQUIRE(V >= 1 && V <= 262144, "%s: %d classes (1 .. 262144)", who, V);
+    OCR_REQUIRE(K >= 1 && K <= 64, "%s: %d entries per row (1 .. 64)", who, K);
+    OCR_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(1.0f / temperature), "%s: temperature must be positive and finite (got %g)", who, (double)temperature);
+    return check_values(who, "logits", x, dtype, rows, V, ld);
+}
+}  // namespace
+
+#define OCR_OPERATOR(h)          \
+    DeviceScope device_scope;    \
+    OCR_HANDLE(h)
+
+int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, int block_rows, int transpose,
+                        uint8_t* d_q, int64_t ld_q, uint8_t* d_scale, int64_t ld_scale, ocrhip_stream stream) {
+    OCR_TRY(check_values("quantize_fp8", "x", d_x, x_dtype, rows, cols, ld_x));
+    OCR_REQUIRE(transpose == 0 || transpose == 1, "quantize_fp8: transpose is 0 or 1");
+    const int64_t R = transpose ? cols : rows, C = transpose ? rows : cols;
+    OCR_TRY(check_blocks("quantize_fp8", "the output", d_q, ld_q, d_scale, ld_scale, block_rows, R, C));
+    const int64_t cb = (C + 127) / 128, x_row = cols * esize(x_dtype), x_ld = ld_x * esize(x_dtype);
+    OCR_REQUIRE(!overlap(d_x, rows, x_ld, x_row, d_q, R, ld_q, ld_q) && !overlap(d_x, rows, x_ld, x_row, d_scale, cb, ld_scale, ld_scale) &&
+                    !overlap(d_q, R, ld_q, ld_q, d_scale, cb, ld_scale, ld_scale),
+                "quantize_fp8: x, the bytes and the scales must not overlap");
+    OCR_OPERATOR(h);
+    return launch_quantize_fp8(d_x, x_dtype, rows, cols, ld_x, block_rows, transpose != 0, d_q, ld_q, d_scale, ld_scale, (hipStream_t)stream);
+}
+
+size_t ocrhip_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) { return M > 0 && N > 0 && K > 0 ? gemm_fp8_workspace(M, N, K) : 0; }
+
+int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uint8_t* d_a_scale, int64_t ld_a_scale, const uint8_t* d_b,
+                    int64_t ld_b, const uint8_t* d_b_scale, int64_t ld_b_scale, int b_block_rows, int64_t M, int64_t N, int64_t K,
+                    const float* d_bias, void* d_c, int c_dtype, int64_t ld_c, void* d_ws, size_t ws_bytes, ocrhip_stream stream) {
+    OCR_TRY(check_product("gemm_fp8", M, N, K, d_bias, d_c, c_dtype, ld_c, d_ws, ws_bytes, ocrhip_gemm_fp8_workspace(M, N, K)));
+    OCR_TRY(check_blocks("gemm_fp8", "a", d_a, ld_a, d_a_scale, ld_a_scale, 1, M, K));
+    OCR_TRY(check_blocks("gemm_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K));
+    const int64_t c_ld = ld_c * esize(c_dtype), c_row = N * esize(c_dtype), kb = (K + 127) / 128;
+    OCR_REQUIRE(!overlap(d_c, M, c_ld, c_row, d_a, M, ld_a, K) && !overlap(d_c, M, c_ld, c_row, d_b, N, ld_b, K) &&
+                    !overlap(d_c, M, c_ld, c_row, d_a_scale, kb, ld_a_scale, M) && !overlap(d_c, M, c_ld, c_row, d_b_scale, kb, ld_b_scale, (N + b_block_rows - 1) / b_block_rows) &&
+                    !overlap(d_c, M, c_ld, c_row, d_bias, d_bias ? 1 : 0, 0, N * 4) &&
+                    !overlap(d_c, M, c_ld, c_row, d_ws, ws_bytes ? 1 : 0, 0, (int64_t)ws_bytes),
+                "gemm_fp8: the output overlaps an input or the workspace");
+    OCR_OPERATOR(h);
+    return launch_gemm_fp8(Fp8Operand{d_a, d_a_scale, ld_a, ld_a_scale}, Fp8Operand{d_b, d_b_scale, ld_b, ld_b_scale}, b_block_rows, M, N, K, d_bias,
+                           d_c, c_dtype, ld_c, d_ws, (hipStream_t)stream);
+}
+
+// workspace of linear_fp8: the quantised rows, their scales, then the product's own
+size_t ocrhip_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return (size_t)(M * round_up(K, 128) + (K + 127) / 128 * round_up(M, 16)) + gemm_fp8_workspace(M, N, K);
+}
+
+int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_x, const uint8_t* d_b, int64_t ld_b, const uint8_t* d_b_scale,
+                      int64_t ld_b_scale, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* d_bias, void* d_c, int c_dtype,
+                      int64_t ld_c, void* d_ws, size_t ws_bytes, ocrhip_stream stream) {
+    OCR_TRY(check_values("linear_fp8", "x", d_x, x_dtype, M, K, ld_x));
+    OCR_TRY(check_product("linear_fp8", M, N, K, d_bias, d_c, c_dtype, ld_c, d_ws, ws_bytes, ocrhip_linear_fp8_workspace(M, N, K)));
+    OCR_TRY(check_blocks("linear_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K));
+    const int64_t c_ld = ld_c * esize(c_dtype), c_row = N * esize(c_dtype), x_ld = ld_x * esize(x_dtype), x_row = K * esize(x_dtype), kb = (K + 127) / 128;
+    OCR_REQUIRE(!overlap(d_c, M, c_ld, c_row, d_x, M, x_ld, x_row) && !overlap(d_c, M, c_ld, c_row, d_b, N, ld_b, K) &&
+                    !overlap(d_c, M, c_ld, c_row, d_b_scale, kb, ld_b_scale, (N + b_block_rows - 1) / b_block_rows) && !overlap(d_c, M, c_ld, c_row, d_bias, d_bias ? 1 : 0, 0, N * 4) &&
+                    !overlap(d_c, M, c_ld, c_row, d_ws, ws_bytes ? 1 : 0, 0, (int64_t)ws_bytes) &&
+                    !overlap(d_x, M, x_ld, x_row, d_ws, ws_bytes ? 1 : 0, 0, (int64_t)ws_bytes),
+                "linear_fp8: the output or the workspace overlaps an input");
+    OCR_OPERATOR(h);
+    if (M == 0 || N == 0) return OCRHIP_OK;
+    uint8_t* q = reinterpret_cast<uint8_t*>(d_ws);
+    const int64_t ld_q = round_up(K, 128), ld_s = round_up(M, 16);
+    uint8_t* sc = q + M * ld_q;
+    OCR_TRY(launch_quantize_fp8(d_x, x_dtype, M, K, ld_x, 1, false, q, ld_q, sc, ld_s, (hipStream_t)stream));
+    return launch_gemm_fp8(Fp8Operand{q, sc, ld_q, ld_s}, Fp8Operand{d_b, d_b_scale, ld_b, ld_b_scale}, b_block_rows, M, N, K, d_bias, d_c, c_dtype,
+                           ld_c, sc + kb * ld_s, (hipStream_t)stream);
+}
+
+int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t rows, int V, int64_t ld, int K, float temperature, float* d_values,
+                      int* d_index, float* d_lse, ocrhip_stream stream) {
+    OCR_TRY(check_rows("top_logits", d_logits, dtype, rows, V, ld, K, temperature));
+    OCR_REQUIRE(K <= V, "top_logits: %d of %d classes", K, V);
+    OCR_REQUIRE(rows == 0 || (d_values && d_index), "top_logits: null output");
+    OCR_REQUIRE(aligned(d_values, 4) && aligned(d_index, 4) && aligned(d_lse, 4), "top_logits: an output is not aligned to its elements");
+    OCR_OPERATOR(h);
+    return launch_top_logits(d_logits, dtype, rows, V, ld, K, temperature, d_values, d_index, d_lse, (hipStream_t)stream);
+}
+
+int ocrhip_distill_loss(ocrhip_handle h, const void* d_logits, int dtype, int64_t rows, int V, int64_t ld, const float* d_top_values,
+                        const int* d_top_index, int K, const float* d_top_lse, float temperature, const float* d_row_weight, float* d_loss,
+                        void* d_grad, int64_t ld_grad, ocrhip_stream stream) {
+    OCR_TRY(check_rows("distill_loss", d_logits, dtype, rows, V, ld, K, temperature));
+    OCR_REQUIRE(rows == 0 || d_loss || d_grad, "distill_loss: ask for the loss and/or the gradient");
+    OCR_REQUIRE(rows == 0 || (d_top_values && d_top_index), "distill_loss: the teacher's entries are null");
+    OCR_REQUIRE(aligned(d_top_values, 4) && aligned(d_top_index, 4) && aligned(d_top_lse, 4) && aligned(d_row_weight, 4) && aligned(d_loss, 4),
+                "distill_loss: a buffer is not aligned to its elements");
+    if (d_grad) {
+        OCR_TRY(check_values("distill_loss", "the gradient", d_grad, dtype, rows, V, ld_grad));
+        const int64_t e = esize(dtype);
+        OCR_REQUIRE(!overlap(d_grad, rows, ld_grad * e, V * e, d_logits, rows, ld * e, V * e), "distill_loss: the gradient overlaps the logits");
+    }
+    OCR_OPERATOR(h);
+    return launch_distill_loss(d_logits, dtype, rows, V, ld, d_top_values, d_top_index, K, d_top_lse, temperature, d_row_weight, d_loss, d_grad, ld_grad,
+                               (hipStream_t)stream);
+}
+
 int ocrhip_set_option(ocrhip_handle h, const char* name, int value) {
     OCR_HANDLE(h);
     OCR_REQUIRE(name, "set_option: null name");

@@ -40,6 +40,8 @@ SOURCES = {
     'conv_bf16.hip': [],
     'conv_bf16t.hip': [],
     'bf16_misc.hip': [],
+    'fp8.hip': [],
+    'distill.hip': [],
     'rnn.hip': [],
     'rnn_persistent.hip': [],
     'pool.hip': [],

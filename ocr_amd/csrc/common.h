@@ -359,4 +359,23 @@ int launch_ctc_greedy_partial(const float* pmax, const int* pidx, int n_blocks, 
 int launch_ctc_beam(ocrhip_ctx* h, const float* logits, int B, int T, int V, const int* lengths, const int* row0, int blank,
                     int num_beams, int* tokens, float* scores, hipStream_t s);
 
+// fp8.hip: e4m3 operands with a power-of-two scale per block (see ocrhip_quantize_fp8 for the layout)
+struct Fp8Operand {
+    const uint8_t* q;
+    const uint8_t* scale;
+    int64_t ld, ld_scale;
+};
+int launch_quantize_fp8(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, int block_rows, bool transpose,
+                        uint8_t* q, int64_t ld_q, uint8_t* scale, int64_t ld_scale, hipStream_t s);
+//   b_block_rows: rows of b that share a scale (1 or 128; a always has 1).  ws: gemm_fp8_workspace bytes.
+size_t gemm_fp8_workspace(int64_t M, int64_t N, int64_t K);
+int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* bias,
+                    void* c, int c_dtype, int64_t ld_c, void* ws, hipStream_t s);
+
+// distill.hip
+int launch_top_logits(const void* x, int dtype, int64_t rows, int V, int64_t ld, int K, float temperature, float* values, int* index, float* lse,
+                      hipStream_t s);
+int launch_distill_loss(const void* x, int dtype, int64_t rows, int V, int64_t ld, const float* top_values, const int* top_index, int K, const float* top_lse,
+                        float temperature, const float* weight, float* loss, void* grad, int64_t ld_grad, hipStream_t s);
+
 }  // namespace ocrhip
