@@ -1236,6 +1236,7 @@ bool overlap(const void* a, int64_t a_rows, int64_t a_ld, int64_t a_row, const v
     return a0 < b0 + (uintptr_t)((b_rows - 1) * b_ld + b_row) && b0 < a0 + (uintptr_t)((a_rows - 1) * a_ld + a_row);
 }
 
+constexpr int64_t kMaxDepth = 1ll << 22;         // K of a product, and the row strides of its operands: 256 rows stay within 31 bits
 constexpr int64_t kMaxExtent = 1ll << 40;       // keeps every byte offset far inside int64
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -1250,19 +1251,21 @@ int check_values(const char* who, const char* what, const void* p, int dtype, in
     return OCRHIP_OK;
 }
 
-int check_blocks(const char* who, const char* what, const uint8_t* q, int64_t ld, const uint8_t* scale, int64_t ld_scale, int block_rows, int64_t rows, int64_t cols) {
+int check_blocks(const char* who, const char* what, const uint8_t* q, int64_t ld, const uint8_t* scale, int64_t ld_scale, int block_rows, int64_t rows, int64_t cols,
+                 bool operand) {
     OCR_REQUIRE(block_rows == 1 || block_rows == 128, "%s: %s has a scale per %d rows (1 or 128)", who, what, block_rows);
     OCR_REQUIRE(rows >= 0 && cols >= 0 && rows < (1ll << 31) && cols < (1ll << 31), "%s: %s has %lld rows and %lld columns", who, what, (long long)rows, (long long)cols);
     OCR_REQUIRE(ld % 128 == 0 && ld >= cols && ld < kMaxExtent && (rows == 0 || ld == 0 || rows <= kMaxExtent / ld), "%s: row stride %lld of %s must be a multiple of 128 and at least its %lld columns", who, (long long)ld, what, (long long)cols);
     OCR_REQUIRE(ld_scale % 16 == 0 && ld_scale >= (rows + block_rows - 1) / block_rows && ld_scale < (1ll << 32),
                 "%s: scale row stride %lld of %s must be a multiple of 16 and at least its number of row blocks", who, (long long)ld_scale, what);
     OCR_REQUIRE(rows == 0 || cols == 0 || (q && scale), "%s: %s is null", who, what);
+    OCR_REQUIRE(!operand || ld <= kMaxDepth, "%s: row stride %lld of %s exceeds %lld", who, (long long)ld, what, (long long)kMaxDepth);
     OCR_REQUIRE(aligned(q, 16) && aligned(scale, 16), "%s: %s must be 16-byte aligned", who, what);
     return OCRHIP_OK;
 }
 
 int check_product(const char* who, int64_t M, int64_t N, int64_t K, const float* bias, void* c, int c_dtype, int64_t ld_c, const void* ws, size_t ws_bytes, size_t need) {
-    OCR_REQUIRE(K >= 1, "%s: K must be at least 1 (got %lld)", who, (long long)K);
+    OCR_REQUIRE(K >= 1 && K <= kMaxDepth, "%s: K must be 1 .. %lld (got %lld)", who, (long long)kMaxDepth, (long long)K);
     OCR_TRY(check_values(who, "the output", c, c_dtype, M, N, ld_c));
     OCR_REQUIRE(aligned(bias, 4), "%s: the bias is not aligned to its elements", who);
     OCR_REQUIRE(need == 0 || M == 0 || N == 0 || (ws && aligned(ws, 16)), "%s: needs a 16-byte aligned workspace of %zu bytes", who, need);
@@ -1290,7 +1293,7 @@ int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t r
     OCR_TRY(check_values("quantize_fp8", "x", d_x, x_dtype, rows, cols, ld_x));
     OCR_REQUIRE(transpose == 0 || transpose == 1, "quantize_fp8: transpose is 0 or 1");
     const int64_t R = transpose ? cols : rows, C = transpose ? rows : cols;
-    OCR_TRY(check_blocks("quantize_fp8", "the output", d_q, ld_q, d_scale, ld_scale, block_rows, R, C));
+    OCR_TRY(check_blocks("quantize_fp8", "the output", d_q, ld_q, d_scale, ld_scale, block_rows, R, C, false));
     const int64_t cb = (C + 127) / 128, x_row = cols * esize(x_dtype), x_ld = ld_x * esize(x_dtype);
     OCR_REQUIRE(!overlap(d_x, rows, x_ld, x_row, d_q, R, ld_q, ld_q) && !overlap(d_x, rows, x_ld, x_row, d_scale, cb, ld_scale, ld_scale) &&
                     !overlap(d_q, R, ld_q, ld_q, d_scale, cb, ld_scale, ld_scale),
@@ -1305,8 +1308,8 @@ int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uin
                     int64_t ld_b, const uint8_t* d_b_scale, int64_t ld_b_scale, int b_block_rows, int64_t M, int64_t N, int64_t K,
                     const float* d_bias, void* d_c, int c_dtype, int64_t ld_c, void* d_ws, size_t ws_bytes, ocrhip_stream stream) {
     OCR_TRY(check_product("gemm_fp8", M, N, K, d_bias, d_c, c_dtype, ld_c, d_ws, ws_bytes, ocrhip_gemm_fp8_workspace(M, N, K)));
-    OCR_TRY(check_blocks("gemm_fp8", "a", d_a, ld_a, d_a_scale, ld_a_scale, 1, M, K));
-    OCR_TRY(check_blocks("gemm_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K));
+    OCR_TRY(check_blocks("gemm_fp8", "a", d_a, ld_a, d_a_scale, ld_a_scale, 1, M, K, true));
+    OCR_TRY(check_blocks("gemm_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K, true));
     const int64_t c_ld = ld_c * esize(c_dtype), c_row = N * esize(c_dtype), kb = (K + 127) / 128;
     OCR_REQUIRE(!overlap(d_c, M, c_ld, c_row, d_a, M, ld_a, K) && !overlap(d_c, M, c_ld, c_row, d_b, N, ld_b, K) &&
                     !overlap(d_c, M, c_ld, c_row, d_a_scale, kb, ld_a_scale, M) && !overlap(d_c, M, c_ld, c_row, d_b_scale, kb, ld_b_scale, (N + b_block_rows - 1) / b_block_rows) &&
@@ -1320,7 +1323,7 @@ int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uin
 
 // workspace of linear_fp8: the quantised rows, their scales, then the product's own
 size_t ocrhip_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || linear_fp8_fits_rows(M)) return 0;
     return (size_t)(M * round_up(K, 128) + (K + 127) / 128 * round_up(M, 16)) + gemm_fp8_workspace(M, N, K);
 }
 
@@ -1329,7 +1332,7 @@ int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_
                       int64_t ld_c, void* d_ws, size_t ws_bytes, ocrhip_stream stream) {
     OCR_TRY(check_values("linear_fp8", "x", d_x, x_dtype, M, K, ld_x));
     OCR_TRY(check_product("linear_fp8", M, N, K, d_bias, d_c, c_dtype, ld_c, d_ws, ws_bytes, ocrhip_linear_fp8_workspace(M, N, K)));
-    OCR_TRY(check_blocks("linear_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K));
+    OCR_TRY(check_blocks("linear_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K, true));
     const int64_t c_ld = ld_c * esize(c_dtype), c_row = N * esize(c_dtype), x_ld = ld_x * esize(x_dtype), x_row = K * esize(x_dtype), kb = (K + 127) / 128;
     OCR_REQUIRE(!overlap(d_c, M, c_ld, c_row, d_x, M, x_ld, x_row) && !overlap(d_c, M, c_ld, c_row, d_b, N, ld_b, K) &&
                     !overlap(d_c, M, c_ld, c_row, d_b_scale, kb, ld_b_scale, (N + b_block_rows - 1) / b_block_rows) && !overlap(d_c, M, c_ld, c_row, d_bias, d_bias ? 1 : 0, 0, N * 4) &&
@@ -1338,6 +1341,8 @@ int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_
                 "linear_fp8: the output or the workspace overlaps an input");
     OCR_OPERATOR(h);
     if (M == 0 || N == 0) return OCRHIP_OK;
+    if (linear_fp8_fits_rows(M))
+        return launch_linear_fp8_rows(d_x, x_dtype, ld_x, Fp8Operand{d_b, d_b_scale, ld_b, ld_b_scale}, b_block_rows, M, N, K, d_bias, d_c, c_dtype, ld_c, (hipStream_t)stream);
     uint8_t* q = reinterpret_cast<uint8_t*>(d_ws);
     const int64_t ld_q = round_up(K, 128), ld_s = round_up(M, 16);
     uint8_t* sc = q + M * ld_q;

@@ -18,7 +18,9 @@
 //     That is 1e-4 of the result at most for ordinary data, a fortieth of the rounding to bfloat16 that follows.
 //   float32 result: the bytes times their scale are converted to bfloat16 on the way from LDS (exact: 4 significant bits)
 //     and multiplied by v_mfma_f32_16x16x32_bf16, which keeps float32 throughout, at half the rate.
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "common.h"
 
@@ -30,6 +32,7 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kBlk = 128;            // values of k that share a scale
@@ -106,6 +109,7 @@ struct GemmArgs {
     int64_t lda, ldas, ldb, ldbs, ldc;
     int64_t M;
     int N, K;
+    bool vec;            // rows of C (in linear_fp8's kernel: of A) start on the width of a vector access
 };
 
 // scale byte -> the float whose exponent field it is (what the conversion below reads)
@@ -118,61 +122,414 @@ __device__ __forceinline__ bf16x8 to_bf16(int lo, int hi, float scale) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// wave: 16 rows x 64 columns, operands straight from memory in the layout the instruction reads (lane: row l % 16, the 32
-// bytes of k group l / 16; the group's order inside the 128 values does not matter, as A and B have the same)
-template <int BROWS, bool OUT_F32>
-__global__ __launch_bounds__(256) void gemm_simple_kernel(GemmArgs g) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t m0 = (int64_t)blockIdx.x * 64 + wave * 16;
-    const int n0 = blockIdx.y * 64;
-    const int r = lane & 15, kg = lane >> 4;
-    const int64_t m = m0 + r;
-    floatx4 acc[4] = {};
-    const int nkb = (g.K + kBlk - 1) / kBlk;
-    for (int kb = 0; kb < nkb; ++kb) {
-        intx8 a = {};
-        int sa = kBias;
-        if (m < g.M) {
-            a = *reinterpret_cast<const intx8*>(g.a + m * g.lda + (int64_t)kb * kBlk + kg * 32);
-            sa = g.as[kb * g.ldas + m];
-        }
-        const float fa = scale_float(sa);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int n = n0 + t * 16 + r;
-            intx8 b = {};
-            int sb = kBias;
-            if (n < g.N) {
-                b = *reinterpret_cast<const intx8*>(g.b + (int64_t)n * g.ldb + (int64_t)kb * kBlk + kg * 32);
-                sb = g.bs[kb * g.ldbs + n / BROWS];
-            }
-            if constexpr (OUT_F32) {
-                const float fb = scale_float(sb);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a[2 * i], a[2 * i + 1], fa), to_bf16(b[2 * i], b[2 * i + 1], fb), acc[t], 0, 0, 0);
-            } else {
-                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], 0, 0, 0, sa, 0, sb);
-            }
-        }
+template <bool OUT_F32>
+__device__ __forceinline__ void store_c(void* c, int64_t at, float v) {
+    if (OUT_F32)
+        reinterpret_cast<float*>(c)[at] = v;
+    else
+        reinterpret_cast<__bf16*>(c)[at] = (__bf16)v;
+}
+// 4 neighbouring columns of a row, of which `left` exist; wide: rows start on the vector's alignment
+template <bool OUT_F32>
+__device__ __forceinline__ void store_c4(void* c, int64_t at, floatx4 v, int left, bool wide) {
+    if (wide && left >= 4) {
+        if (OUT_F32)
+            *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(c) + at) = v;
+        else
+            *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(c) + at) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        return;
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int n = n0 + t * 16 + r;
-        if (n >= g.N) continue;
-        const float bias = g.bias ? g.bias[n] : 0.0f;
+    for (int e = 0; e < 4; ++e)
+        if (e < left) store_c<OUT_F32>(c, at + e, v[e]);
+}
+
+// NV values x[k0 ..] of a row of K (zeros beyond); vec: rows start on 16 bytes
+template <int NV>
+__device__ __forceinline__ void load_run(const float* x, int k0, int K, bool vec, float* v) {
+    if (vec && k0 + NV <= K) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t mo = m0 + kg * 4 + e;
-            if (mo >= g.M) continue;
-            const float v = acc[t][e] + bias;
-            if (OUT_F32)
-                reinterpret_cast<float*>(g.c)[mo * g.ldc + n] = v;
-            else
-                reinterpret_cast<__bf16*>(g.c)[mo * g.ldc + n] = (__bf16)v;
+        for (int e = 0; e < NV; e += 4) {
+            const floatx4 t = *reinterpret_cast<const floatx4*>(x + k0 + e);
+            v[e] = t[0]; v[e + 1] = t[1]; v[e + 2] = t[2]; v[e + 3] = t[3];
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < NV; ++e) v[e] = k0 + e < K ? x[k0 + e] : 0.0f;
+}
+template <int NV>
+__device__ __forceinline__ void load_run(const uint16_t* x, int k0, int K, bool vec, float* v) {
+    if (vec && k0 + NV <= K) {
+#pragma unroll
+        for (int e = 0; e < NV; e += 8) {
+            const intx4 t = *reinterpret_cast<const intx4*>(x + k0 + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[e + 2 * i] = __int_as_float(t[i] << 16);
+                v[e + 2 * i + 1] = __int_as_float(t[i] & (int)0xFFFF0000);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < NV; ++e) v[e] = k0 + e < K ? load_f32(x + k0 + e) : 0.0f;
+}
+
+// ---- few rows of A (M <= 64): bound by reading B once
+//
+// A wave owns 16 columns of C (rows of B) for all of M and every waves_k-th block of k; it reads B straight into the
+// registers the matrix instruction takes it from (16 whole 128-byte lines per block), so nothing is staged and the loads
+// of several blocks are in flight at once.  The waves_k partial sums meet in LDS, added in the order of the waves.
+// XT: type of A.  void: quantised operands.  float / uint16_t: values that the wave quantises itself - a lane holds 32
+// values of a row, the block's maximum is two lane exchanges away, and the bytes land in the registers the matrix
+// instruction reads - which saves linear_fp8 a launch; up to 32 rows, beyond that every wave's own quantisation costs more
+// than a launch of its own that does it once.
+template <class XT, int IM, bool OUT_F32, int BROWS>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k) {
+    extern __shared__ float red[];               // [wave][IM][4][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wn = wave / waves_k, wk = wave % waves_k, waves_n = (blockDim.x >> 6) / waves_k;
+    const int r = lane & 15, kg = lane >> 4;
+    const int n0 = (blockIdx.x * waves_n + wn) * 16;
+    const int n = n0 + r;
+    const int nkb = (g.K + kBlk - 1) / kBlk;
+    const bool n_ok = n < g.N;
+    const uint8_t* bp = g.b + (int64_t)(n_ok ? n : 0) * g.ldb + kg * 32;
+    floatx4 acc[IM] = {};
+    for (int kb = wk; kb < nkb; kb += waves_k) {
+        intx8 b = *reinterpret_cast<const intx8*>(bp + (int64_t)kb * kBlk);
+        const int sb = g.bs[kb * g.ldbs + (n_ok ? n : 0) / BROWS];
+        intx8 a[IM];
+        int sa[IM];
+#pragma unroll
+        for (int i = 0; i < IM; ++i) {
+            const int m = min(i * 16 + r, (int)g.M - 1);
+            if constexpr (__is_same(XT, void)) {
+                a[i] = *reinterpret_cast<const intx8*>(g.a + m * g.lda + (int64_t)kb * kBlk + kg * 32);
+                sa[i] = g.as[kb * g.ldas + m];
+            } else {
+                const XT* xp = reinterpret_cast<const XT*>(g.a) + m * g.lda;
+                const int k0 = kb * kBlk + kg * 32;
+                float v[32], amax = 0.0f;
+                load_run<32>(xp, k0, g.K, g.vec, v);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) amax = fmaxf(amax, finite_magnitude(v[e]));
+                amax = fmaxf(amax, __shfl_xor(amax, 16));
+                amax = fmaxf(amax, __shfl_xor(amax, 32));
+                sa[i] = (int)scale_byte(amax);
+                const float inv = inverse_scale((unsigned)sa[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    a[i][e] = (int)pack4_e4m3(no_infinity(v[4 * e] * inv), no_infinity(v[4 * e + 1] * inv), no_infinity(v[4 * e + 2] * inv), no_infinity(v[4 * e + 3] * inv));
+            }
+        }
+        if constexpr (OUT_F32) {
+            const float fb = scale_float(sb);
+            bf16x8 bv[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) bv[t] = to_bf16(b[2 * t], b[2 * t + 1], fb);
+#pragma unroll
+            for (int i = 0; i < IM; ++i) {
+                const float fa = scale_float(sa[i]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[t], to_bf16(a[i][2 * t], a[i][2 * t + 1], fa), acc[i], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < IM; ++i) acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a[i], acc[i], 0, 0, 0, sb, 0, sa[i]);
+        }
+    }
+    // B is the row operand: lane r holds C[i * 16 + r][n0 + 4 kg + e]
+    if (waves_k > 1) {
+#pragma unroll
+        for (int i = 0; i < IM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[((wave * IM + i) * 4 + e) * 64 + lane] = acc[i][e];
+        __syncthreads();
+        if (wk != 0) return;
+        for (int w = 1; w < waves_k; ++w)
+#pragma unroll
+            for (int i = 0; i < IM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][e] += red[(((wave + w) * IM + i) * 4 + e) * 64 + lane];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int no = n0 + kg * 4 + e;
+        if (no >= g.N) continue;
+        const float bias = g.bias ? g.bias[no] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < IM; ++i) {
+            const int64_t m = i * 16 + r;
+            if (m < g.M) store_c<OUT_F32>(g.c, m * g.ldc + no, acc[i][e] + bias);
         }
     }
 }
+
+// ---- tiles
+//
+// A workgroup computes BM x BN of C.  Per block of 128 values of k its rows of A and B (whole 128-byte lines) and A's scale
+// bytes go straight from memory to LDS; the next block's copies are in flight while this one is multiplied (two buffers,
+// one barrier per block).  A row is 8 pieces of 16 bytes; piece c of row r lies at place c ^ (r / 2 % 8), so that the 16
+// lanes of a read phase (16 rows, the same piece) hit 16 different groups of banks; the copy writes lane after lane, so
+// the permutation is applied to the address it reads from.  Rows beyond M or N are offsets beyond the descriptor: zeros.
+// B is the matrix instruction's row operand, A its column operand: a lane then holds 4 neighbouring columns of one row.
+struct TileArgs {
+    GemmArgs g;
+    int tiles_m, tiles_n, splits, kb_split;       // kb_split: blocks of k per split
+    float* part;                                  // splits > 1: [split][M][N] partial sums
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// (no template parameter may reach the arguments of an LDS-destination load: the host pass would drop the kernel's stub)
+__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* dst, int voff, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)dst, 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t rsrc, unsigned char* dst, int voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)dst, 4, voff, 0, 0, 0);
+}
+
+template <int BM, int BN>
+constexpr int tile_stage_bytes() { return (BM + BN) * kBlk + 512; }      // operands, then 256 scale bytes of A and of B
+
+template <int BM, int BN, int WGM, int WGN, bool OUT_F32, int BROWS>
+__global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
+    constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, IM = TM / 16, IN = TN / 16;
+    constexpr int NA = BM / 8, NI = (BM + BN) / 8, PER = NI / WAVES;     // copies of 8 rows: A's, all, per wave
+    constexpr int STAGE = tile_stage_bytes<BM, BN>();
+    static_assert(NI % WAVES == 0 && BM <= 256 && BN <= 256 && (BROWS == 1 || TN <= 128), "tile");
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const GemmArgs& g = a.g;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    const int r = lane & 15, kg = lane >> 4;
+
+    // workgroups go to the 8 dies in turn: every die gets a contiguous range of the work, in bands of 8 tile rows, so that
+    // the tiles it computes at one time share their rows of A and B in its L2
+    const unsigned total = gridDim.x, xcd = blockIdx.x & 7u;
+    unsigned work = xcd * (total >> 3) + min(xcd, total & 7u) + (blockIdx.x >> 3);
+    const unsigned per_split = (unsigned)a.tiles_m * a.tiles_n;
+    const int split = (int)(work / per_split);
+    work %= per_split;
+    const unsigned band = work / (8u * a.tiles_n), rows_in_band = min(8u, a.tiles_m - band * 8);
+    const unsigned in_band = work - band * 8u * a.tiles_n;
+    const int64_t m0 = (int64_t)(band * 8 + in_band % rows_in_band) * BM;
+    const int n0 = (int)(in_band / rows_in_band) * BN;
+
+    const int nkb = (g.K + kBlk - 1) / kBlk;
+    const int kb0 = split * a.kb_split, kb1 = min(nkb, kb0 + a.kb_split);
+
+    const int rows_a = (int)min((int64_t)BM, g.M - m0), rows_b = min(BN, g.N - n0);
+    const int k_bytes = (kb1 - kb0) * kBlk;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(g.a + m0 * g.lda + (int64_t)kb0 * kBlk), 0, (unsigned)((rows_a - 1) * (int)g.lda + k_bytes), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)(g.b + n0 * g.ldb + (int64_t)kb0 * kBlk), 0, (unsigned)((rows_b - 1) * (int)g.ldb + k_bytes), 0x00020000);
+    int src[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = wave * PER + i;
+        const int row = (c < NA ? c : c - NA) * 8 + (lane >> 3);
+        const int piece = (lane & 7) ^ (row >> 1 & 7);
+        const bool ok = row < (c < NA ? rows_a : rows_b);
+        src[i] = ok ? row * (int)(c < NA ? g.lda : g.ldb) + piece * 16 : (int)0x80000000;
+    }
+    auto issue = [&](int kb) {
+        unsigned char* base = lds + (kb & 1) * STAGE;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = wave * PER + i;
+            copy16(c < NA ? ra : rb, base + c * 1024, src[i], (kb - kb0) * kBlk);
+        }
+        if (wave == 0) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.as + (int64_t)kb * g.ldas + m0), 0, (unsigned)min((int64_t)BM, g.ldas - m0), 0x00020000);
+            copy4(rs, base + (BM + BN) * kBlk, lane * 4);
+        }
+        if (BROWS == 1 && wave == WAVES - 1) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.bs + (int64_t)kb * g.ldbs + n0), 0, (unsigned)min((int64_t)BN, g.ldbs - n0), 0x00020000);
+            copy4(rs, base + (BM + BN) * kBlk + 256, lane * 4);
+        }
+    };
+    // the wave's columns lie within one block of 128: its scale is a scalar load, one block ahead
+    const int64_t sb_col = min(n0 + wn * TN, g.N - 1) / kBlk;
+    int sb_next = BROWS == 1 ? 0 : g.bs[(int64_t)kb0 * g.ldbs + sb_col];
+
+    floatx4 acc[IM][IN];
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    issue(kb0);
+    const int a_row = wm * TM + r, b_row = wn * TN + r;
+    for (int kb = kb0; kb < kb1; ++kb) {
+        // my copies have landed and my reads of the other buffer are done; behind the barrier everybody's
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (kb + 1 < kb1) issue(kb + 1);
+        const unsigned char* base = lds + (kb & 1) * STAGE;
+        const unsigned char* pa = base + a_row * kBlk;
+        const unsigned char* pb = base + (BM + b_row) * kBlk;
+        const unsigned char* psa = base + (BM + BN) * kBlk + a_row;
+        const unsigned char* psb = base + (BM + BN) * kBlk + 256 + b_row;
+        const int sw = r >> 1;                          // rows 16 apart have the same permutation
+        int sb = sb_next;
+        if (BROWS != 1 && kb + 1 < kb1) sb_next = g.bs[(int64_t)(kb + 1) * g.ldbs + sb_col];
+        if constexpr (OUT_F32) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {               // 16 of the lane's 32 bytes: two instructions of 32 values of k
+                const int at = ((2 * kg + h) ^ sw) * 16;
+                bf16x8 bv[IN][2];
+#pragma unroll
+                for (int j = 0; j < IN; ++j) {
+                    const intx4 q = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at);
+                    const float f = scale_float(BROWS == 1 ? (int)psb[j * 16] : sb);
+                    bv[j][0] = to_bf16(q[0], q[1], f);
+                    bv[j][1] = to_bf16(q[2], q[3], f);
+                }
+#pragma unroll
+                for (int i = 0; i < IM; ++i) {
+                    const intx4 q = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at);
+                    const float f = scale_float((int)psa[i * 16]);
+                    const bf16x8 a0 = to_bf16(q[0], q[1], f), a1 = to_bf16(q[2], q[3], f);
+#pragma unroll
+                    for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j][0], a0, acc[i][j], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j][1], a1, acc[i][j], 0, 0, 0);
+                }
+            }
+        } else {
+            const int at0 = ((2 * kg) ^ sw) * 16, at1 = ((2 * kg + 1) ^ sw) * 16;
+            intx8 bv[IN];
+            int sbv[IN];
+#pragma unroll
+            for (int j = 0; j < IN; ++j) {
+                const intx4 lo = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at0), hi = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at1);
+                bv[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                sbv[j] = BROWS == 1 ? (int)psb[j * 16] : sb;
+            }
+#pragma unroll
+            for (int i = 0; i < IM; ++i) {
+                const intx4 lo = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at0), hi = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at1);
+                const intx8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                const int sa = psa[i * 16];
+#pragma unroll
+                for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv[j], av, acc[i][j], 0, 0, 0, sbv[j], 0, sa);
+            }
+        }
+    }
+    // lane (r, kg) holds C[m0 + wm TM + 16 i + r][n0 + wn TN + 16 j + 4 kg .. + 3]
+    const bool partial = a.splits > 1;
+    float* part = partial ? a.part + (int64_t)split * g.M * g.N : nullptr;
+    const bool wide = partial ? (g.N & 3) == 0 : g.vec;
+#pragma unroll
+    for (int j = 0; j < IN; ++j) {
+        const int n = n0 + wn * TN + j * 16 + kg * 4;
+        floatx4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (g.bias && !partial)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[e] = n + e < g.N ? g.bias[n + e] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < IM; ++i) {
+            const int64_t m = m0 + wm * TM + i * 16 + r;
+            if (m >= g.M) continue;
+            const floatx4 v = acc[i][j] + bias;
+            if (partial)
+                store_c4<true>(part, m * g.N + n, v, g.N - n, wide);
+            else
+                store_c4<OUT_F32>(g.c, m * g.ldc + n, v, g.N - n, wide);
+        }
+    }
+}
+
+// the partial sums of the splits, in their order, and the bias
+template <bool OUT_F32>
+__global__ __launch_bounds__(256) void gemm_join_kernel(const float* __restrict__ part, int splits, int64_t M, int N, const float* __restrict__ bias, void* c, int64_t ldc) {
+    const int64_t count = M * N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        float v = part[i];
+        for (int z = 1; z < splits; ++z) v += part[z * count + i];
+        const int64_t m = i / N;
+        const int n = (int)(i - m * N);
+        store_c<OUT_F32>(c, m * ldc + n, v + (bias ? bias[n] : 0.0f));
+    }
+}
+
+std::mutex g_tile_mutex;
+
+template <int BM, int BN, int WGM, int WGN, bool OUT_F32, int BROWS>
+int launch_tile(const TileArgs& a, hipStream_t s) {
+    constexpr int bytes = 2 * tile_stage_bytes<BM, BN>();
+    auto kernel = &gemm_tile_kernel<BM, BN, WGM, WGN, OUT_F32, BROWS>;
+    static bool opted[64] = {};
+    int dev = 0;
+    OCR_HIP_CHECK(hipGetDevice(&dev));
+    {
+        std::lock_guard<std::mutex> lock(g_tile_mutex);
+        if (!opted[dev & 63]) {
+            OCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            opted[dev & 63] = true;
+        }
+    }
+    hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WGM, WGN, OUT_F32, BROWS>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(WGM * WGN * 64), bytes, s, a);
+    OCR_HIP_CHECK(hipGetLastError());
+    return OCRHIP_OK;
+}
+
+struct TilePlan {
+    int bm, bn, splits, kb_split;
+    int64_t tiles_m, tiles_n;
+};
+
+// Which tiles a product of M > kMaxRows rows takes, and into how many pieces of k it is split.
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
+    TilePlan p;
+    const int64_t nkb = (K + kBlk - 1) / kBlk;
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+    const bool large = !out_f32 && big >= 192;
+    p.bm = p.bn = large ? 256 : 128;
+    p.tiles_m = (M + p.bm - 1) / p.bm;
+    p.tiles_n = (N + p.bn - 1) / p.bn;
+    const int64_t tiles = p.tiles_m * p.tiles_n;
+    int64_t splits = 1;
+    if (tiles < 256 && nkb >= 8) splits = std::min<int64_t>(std::min<int64_t>(nkb / 4, (512 + tiles - 1) / tiles), 16);
+    p.kb_split = (int)((nkb + splits - 1) / splits);
+    p.splits = (int)((nkb + p.kb_split - 1) / p.kb_split);
+    return p;
+}
+
+template <class XT, bool OUT_F32, int BROWS>
+int launch_rows(const GemmArgs& g, hipStream_t s) {
+    const int nkb = (g.K + kBlk - 1) / kBlk;
+    int waves_k = 1;
+    while (waves_k < 8 && waves_k * 2 <= nkb) waves_k *= 2;
+    const int waves_n = std::max(1, 4 / waves_k);
+    const int waves = waves_k * waves_n, im = (int)((g.M + 15) / 16);
+    const dim3 grid((unsigned)((g.N + 16 * waves_n - 1) / (16 * waves_n))), block(waves * 64);
+    const size_t lds = waves_k > 1 ? (size_t)waves * im * 4 * 64 * sizeof(float) : 0;
+    switch (im) {
+        case 1: hipLaunchKernelGGL((gemm_rows_kernel<XT, 1, OUT_F32, BROWS>), grid, block, lds, s, g, waves_k); break;
+        case 2: hipLaunchKernelGGL((gemm_rows_kernel<XT, 2, OUT_F32, BROWS>), grid, block, lds, s, g, waves_k); break;
+        case 3:
+            if constexpr (__is_same(XT, void)) hipLaunchKernelGGL((gemm_rows_kernel<XT, 3, OUT_F32, BROWS>), grid, block, lds, s, g, waves_k);
+            break;
+        default:
+            if constexpr (__is_same(XT, void)) hipLaunchKernelGGL((gemm_rows_kernel<XT, 4, OUT_F32, BROWS>), grid, block, lds, s, g, waves_k);
+            break;
+    }
+    OCR_HIP_CHECK(hipGetLastError());
+    return OCRHIP_OK;
+}
+
+template <class XT>
+int launch_rows_any(const GemmArgs& g, bool f32, int b_block_rows, hipStream_t s) {
+    if (b_block_rows == 1) return f32 ? launch_rows<XT, true, 1>(g, s) : launch_rows<XT, false, 1>(g, s);
+    return f32 ? launch_rows<XT, true, kBlk>(g, s) : launch_rows<XT, false, kBlk>(g, s);
+}
+
+constexpr int kMaxRows = 64;          // gemm_rows_kernel: rows of A
+constexpr int kMaxOwnRows = 32;       // the same, quantising them itself
 
 }  // namespace
 
@@ -193,27 +550,56 @@ int launch_quantize_fp8(const void* x, int x_dtype, int64_t rows, int64_t cols, 
 }
 
 size_t gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    (void)M; (void)N; (void)K;
-    return 0;
+    if (M <= kMaxRows) return 0;
+    const int a = plan_tiles(M, N, K, true).splits, b = plan_tiles(M, N, K, false).splits, splits = std::max(a, b);
+    return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
 }
 
 int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* bias,
                     void* c, int c_dtype, int64_t ld_c, void* ws, hipStream_t s) {
-    (void)ws;
     if (M == 0 || N == 0) return OCRHIP_OK;
-    GemmArgs g{a.q, a.scale, b.q, b.scale, bias, c, a.ld, a.ld_scale, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K};
     const bool f32 = c_dtype == OCRHIP_F32;
-    ProfScope prof("gemm_fp8", 2.0 * (double)M * N * K, (double)(M + N) * K + (f32 ? 4.0 : 2.0) * (double)M * N, s);
-    const dim3 grid((unsigned)((M + 63) / 64), (unsigned)((N + 63) / 64));
-    if (b_block_rows == 1) {
-        if (f32) hipLaunchKernelGGL((gemm_simple_kernel<1, true>), grid, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((gemm_simple_kernel<1, false>), grid, dim3(256), 0, s, g);
-    } else {
-        if (f32) hipLaunchKernelGGL((gemm_simple_kernel<kBlk, true>), grid, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((gemm_simple_kernel<kBlk, false>), grid, dim3(256), 0, s, g);
+    const bool vec = ld_c % 4 == 0 && reinterpret_cast<uintptr_t>(c) % (f32 ? 16 : 8) == 0;
+    GemmArgs g{a.q, a.scale, b.q, b.scale, bias, c, a.ld, a.ld_scale, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K, vec};
+    const double flops = 2.0 * (double)M * N * K, bytes = (double)(M + N) * K + (f32 ? 4.0 : 2.0) * (double)M * N;
+    if (M <= kMaxRows) {
+        ProfScope prof(f32 ? "gemm_fp8<rows,f32>" : "gemm_fp8<rows,bf16>", flops, bytes, s);
+        return launch_rows_any<void>(g, f32, b_block_rows, s);
     }
-    OCR_HIP_CHECK(hipGetLastError());
+    const TilePlan p = plan_tiles(M, N, K, f32);
+    OCR_REQUIRE(p.tiles_m * p.tiles_n * p.splits < (1ll << 31), "gemm_fp8: too many tiles");
+    TileArgs t{g, (int)p.tiles_m, (int)p.tiles_n, p.splits, p.kb_split, reinterpret_cast<float*>(ws)};
+    {
+        ProfScope prof(p.bm == 256 ? "gemm_fp8<256,bf16>" : f32 ? "gemm_fp8<128,f32>" : "gemm_fp8<128,bf16>", flops, bytes, s);
+        if (p.bm == 256)
+            OCR_TRY(b_block_rows == 1 ? (launch_tile<256, 256, 2, 4, false, 1>(t, s)) : (launch_tile<256, 256, 2, 4, false, kBlk>(t, s)));
+        else if (f32)
+            OCR_TRY(b_block_rows == 1 ? (launch_tile<128, 128, 2, 2, true, 1>(t, s)) : (launch_tile<128, 128, 2, 2, true, kBlk>(t, s)));
+        else
+            OCR_TRY(b_block_rows == 1 ? (launch_tile<128, 128, 2, 2, false, 1>(t, s)) : (launch_tile<128, 128, 2, 2, false, kBlk>(t, s)));
+    }
+    if (p.splits > 1) {
+        ProfScope prof("gemm_fp8<join>", (double)p.splits * M * N, ((f32 ? 4.0 : 2.0) + 4.0 * p.splits) * (double)M * N, s);
+        const dim3 grid((unsigned)std::min<int64_t>((M * N + 255) / 256, 4096));
+        if (f32)
+            hipLaunchKernelGGL(gemm_join_kernel<true>, grid, dim3(256), 0, s, t.part, p.splits, M, (int)N, bias, c, ld_c);
+        else
+            hipLaunchKernelGGL(gemm_join_kernel<false>, grid, dim3(256), 0, s, t.part, p.splits, M, (int)N, bias, c, ld_c);
+        OCR_HIP_CHECK(hipGetLastError());
+    }
     return OCRHIP_OK;
+}
+
+bool linear_fp8_fits_rows(int64_t M) { return M <= kMaxOwnRows; }
+
+int launch_linear_fp8_rows(const void* x, int x_dtype, int64_t ld_x, const Fp8Operand& b, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* bias,
+                           void* c, int c_dtype, int64_t ld_c, hipStream_t s) {
+    if (M == 0 || N == 0) return OCRHIP_OK;
+    const bool f32 = c_dtype == OCRHIP_F32, xf32 = x_dtype == OCRHIP_F32;
+    const bool vec = ld_x % (xf32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    GemmArgs g{reinterpret_cast<const uint8_t*>(x), nullptr, b.q, b.scale, bias, c, ld_x, 0, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K, vec};
+    ProfScope prof("linear_fp8<rows>", 2.0 * (double)M * N * K, (xf32 ? 4.0 : 2.0) * (double)M * K + (double)N * K + (f32 ? 4.0 : 2.0) * (double)M * N, s);
+    return xf32 ? launch_rows_any<float>(g, f32, b_block_rows, s) : launch_rows_any<uint16_t>(g, f32, b_block_rows, s);
 }
 
 }  // namespace ocrhip

@@ -106,6 +106,8 @@ def test_good_arguments_reach_the_handle(name):
     ('quantize_fp8', dict(q=P + 64), 'overlap'),
     ('quantize_fp8', dict(scale=64 * P + 128), 'overlap'),
     ('gemm_fp8', dict(K=0), 'K must be'),
+    ('gemm_fp8', dict(K=(1 << 22) + 1, ld_a=(1 << 22) + 128, ld_b=(1 << 22) + 128), 'K must be'),
+    ('gemm_fp8', dict(ld_b=1 << 23), 'exceeds'),
     ('gemm_fp8', dict(M=-1), 'rows'),
     ('gemm_fp8', dict(c_dtype=2), 'F32 or BF16'),
     ('gemm_fp8', dict(c=None), 'output is null'),
@@ -125,8 +127,8 @@ def test_good_arguments_reach_the_handle(name):
     ('gemm_fp8', dict(c=32 * P), 'overlaps'),
     ('linear_fp8', dict(x_dtype=1, x=P + 1), 'aligned'),
     ('linear_fp8', dict(ld_x=100), 'elements apart'),
-    ('linear_fp8', dict(ws=None), 'workspace'),
-    ('linear_fp8', dict(ws=48 * P + 4), 'workspace'),
+    ('linear_fp8', dict(M=500, ws=None), 'workspace'),
+    ('linear_fp8', dict(M=500, ws=48 * P + 4), 'workspace'),
     ('linear_fp8', dict(c=P), 'overlaps'),
     ('linear_fp8', dict(ws=P), 'overlaps'),
     ('linear_fp8', dict(ws=40 * P), 'overlaps'),
@@ -161,9 +163,9 @@ def test_refusals_of_the_c_entries(name, over, part):
 
 def test_a_workspace_that_is_too_small_is_a_capacity_error():
     from ocr_amd import _lib
-    need = _lib.load().ocrhip_linear_fp8_workspace(10, 7, 200)
-    assert need >= 10 * 256 + 2 * 16
-    rc, msg = _call('linear_fp8', ws_bytes=need - 1)
+    need = _lib.load().ocrhip_linear_fp8_workspace(500, 7, 200)
+    assert need >= 500 * 256 + 2 * 512
+    rc, msg = _call('linear_fp8', M=500, ws_bytes=need - 1)
     assert rc == -2 and str(need) in msg
 
 
