@@ -35,6 +35,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+std::mutex g_lds_mutex;              // guards the once-per-device LDS opt-in of the kernels that need more than 64 KB
+
 constexpr int kBlk = 128;            // values of k that share a scale
 constexpr int kBias = 127;           // stored byte = exponent + 127 (255 is no exponent: the instruction takes it as NaN)
 
@@ -72,33 +74,200 @@ __device__ __forceinline__ unsigned pack4_e4m3(float a, float b, float c, float 
 // an infinity would saturate to the largest value in the conversion: make it a NaN first
 __device__ __forceinline__ float no_infinity(float v) { return fabsf(v) == INFINITY ? __uint_as_float(0x7FC00000u) : v; }
 
+// Vectors at the alignment of their elements: rows of odd length start anywhere, and global memory takes 16-byte accesses
+// at any element.
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef int intx4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// NV (a multiple of 8) values x[k0 ..] of a row of K, zeros beyond
+template <int NV>
+__device__ __forceinline__ void load_run(const float* x, int64_t k0, int64_t K, float* v) {
+    if (k0 + NV <= K) {
+#pragma unroll
+        for (int e = 0; e < NV; e += 4) {
+            const floatx4 t = *reinterpret_cast<const floatx4_any*>(x + k0 + e);
+            v[e] = t[0]; v[e + 1] = t[1]; v[e + 2] = t[2]; v[e + 3] = t[3];
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < NV; ++e) v[e] = k0 + e < K ? x[k0 + e] : 0.0f;
+}
+template <int NV>
+__device__ __forceinline__ void load_run(const uint16_t* x, int64_t k0, int64_t K, float* v) {
+    if (k0 + NV <= K) {
+#pragma unroll
+        for (int e = 0; e < NV; e += 8) {
+            const intx4 t = *reinterpret_cast<const intx4_any*>(x + k0 + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[e + 2 * i] = __int_as_float(t[i] << 16);
+                v[e + 2 * i + 1] = __int_as_float(t[i] & (int)0xFFFF0000);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < NV; ++e) v[e] = k0 + e < K ? load_f32(x + k0 + e) : 0.0f;
+}
+
+// ---- quantise
+//
+// Bound by reading x and writing the bytes once.  16 lanes hold a block of a row, 8 values each (one or two 16-byte loads,
+// 8 bytes to store); the maximum crosses them by four exchanges.
+constexpr int kRowsWg = 16;           // rows a workgroup of 256 threads works on at a time
+constexpr int kBlocksWg = 4;          // column blocks it walks: their loads are in flight together
+
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+__device__ __forceinline__ uint64_t pack8_e4m3(const float* v, float inv) {
+    float t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = no_infinity(v[e] * inv);
+    return (uint64_t)pack4_e4m3(t[0], t[1], t[2], t[3]) | (uint64_t)pack4_e4m3(t[4], t[5], t[6], t[7]) << 32;
+}
+
+// one scale per row and 128 columns: 16 rows x 4 column blocks
 template <class T>
-__global__ __launch_bounds__(256) void quantize_simple_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, int block_rows,
-                                                              int transpose, uint8_t* __restrict__ q, int64_t ld_q,
-                                                              uint8_t* __restrict__ scale, int64_t ld_s) {
-    __shared__ float part[4];
-    const int64_t rb = blockIdx.x, cb = blockIdx.y;
-    const int tid = threadIdx.x;
-    const int64_t r0 = rb * block_rows, c0 = cb * kBlk;
-    const int nr = (int)min((int64_t)block_rows, rows - r0);
-    auto value = [&](int r, int c) -> float {
-        if (c0 + c >= cols) return 0.0f;
-        return load_f32(transpose ? x + (c0 + c) * ld_x + r0 + r : x + (r0 + r) * ld_x + c0 + c);
-    };
-    float amax = 0.0f;
-    for (int i = tid; i < nr * kBlk; i += 256) amax = fmaxf(amax, finite_magnitude(value(i / kBlk, i % kBlk)));
-    for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    if ((tid & 63) == 0) part[tid >> 6] = amax;
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, uint8_t* __restrict__ q,
+                                                            int64_t ld_q, uint8_t* __restrict__ scale, int64_t ld_s, unsigned chunks) {
+    const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;
+    const int64_t row = (int64_t)(blockIdx.x / chunks) * kRowsWg + sub, kb0 = (int64_t)(blockIdx.x % chunks) * kBlocksWg;
+    const int nkb = (int)min((int64_t)kBlocksWg, (cols + kBlk - 1) / kBlk - kb0);
+    const bool there = row < rows;
+    const T* p = x + (there ? row : 0) * ld_x;
+    float v[kBlocksWg][8];
+#pragma unroll
+    for (int i = 0; i < kBlocksWg; ++i)
+        if (i < nkb) load_run<8>(p, (kb0 + i) * kBlk + part * 8, cols, v[i]);
+#pragma unroll
+    for (int i = 0; i < kBlocksWg; ++i) {
+        if (i >= nkb) break;
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_magnitude(v[i][e]));
+        const unsigned byte = scale_byte(max16(amax));
+        if (!there) continue;
+        *reinterpret_cast<uint64_t*>(q + row * ld_q + (kb0 + i) * kBlk + part * 8) = pack8_e4m3(v[i], inverse_scale(byte));
+        if (part == 0) scale[(kb0 + i) * ld_s + row] = (uint8_t)byte;
+    }
+}
+
+// one scale per 128 rows x 128 columns: a workgroup holds the block in registers
+template <class T>
+__global__ __launch_bounds__(256) void quantize_block_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, uint8_t* __restrict__ q,
+                                                             int64_t ld_q, uint8_t* __restrict__ scale, int64_t ld_s, unsigned col_blocks) {
+    __shared__ float wave_max[4];
+    const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;
+    const int64_t rb = blockIdx.x / col_blocks, cb = blockIdx.x % col_blocks;
+    float v[kBlk / kRowsWg][8], amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kBlk / kRowsWg; ++i) {
+        const int64_t row = rb * kBlk + i * kRowsWg + sub;
+        if (row < rows) load_run<8>(x + row * ld_x, cb * kBlk + part * 8, cols, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kBlk / kRowsWg; ++i) {
+        if (rb * kBlk + i * kRowsWg + sub >= rows) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_magnitude(v[i][e]));
+    }
+    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = amax;
     __syncthreads();
-    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const unsigned byte = scale_byte(amax);
+    const unsigned byte = scale_byte(fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3])));
     const float inv = inverse_scale(byte);
-    if (tid == 0) scale[cb * ld_s + rb] = (uint8_t)byte;
-    for (int i = tid; i < nr * (kBlk / 4); i += 256) {
-        const int r = i / (kBlk / 4), c = i % (kBlk / 4) * 4;
-        float v[4];
-        for (int e = 0; e < 4; ++e) v[e] = no_infinity(value(r, c + e) * inv);
-        *reinterpret_cast<unsigned*>(q + (r0 + r) * ld_q + c0 + c) = pack4_e4m3(v[0], v[1], v[2], v[3]);
+    if (threadIdx.x == 0) scale[cb * ld_s + rb] = (uint8_t)byte;
+#pragma unroll
+    for (int i = 0; i < kBlk / kRowsWg; ++i) {
+        const int64_t row = rb * kBlk + i * kRowsWg + sub;
+        if (row >= rows) break;
+        *reinterpret_cast<uint64_t*>(q + row * ld_q + cb * kBlk + part * 8) = pack8_e4m3(v[i], inv);
+    }
+}
+
+// The transpose of x: a workgroup reads 128 rows x WC columns (whole vectors along the rows), passes them through LDS (rows
+// an odd number of floats apart: the column-wise reads of a wave spread over the banks) and writes 128 bytes of WC rows of
+// the result.  Four threads share a column, 32 values each.  WC 64: a scale per column; WC 128: one scale for the block.
+template <class T, int WC>
+__global__ __launch_bounds__(256) void quantize_transpose_kernel(const T* __restrict__ x, int64_t ld_x, int64_t x_rows, int64_t x_cols, uint8_t* __restrict__ q,
+                                                                 int64_t ld_q, uint8_t* __restrict__ scale, int64_t ld_s, unsigned col_tiles) {
+    constexpr int LD = WC + 1, PASS = 256 / (WC / 8);          // rows per pass of the workgroup
+    extern __shared__ float tile[];
+    __shared__ float wave_max[4];
+    __shared__ uint8_t bytes[WC];
+    const int tid = threadIdx.x;
+    // neighbouring tiles of a row of x (which share the lines at their borders) on one die
+    const unsigned total = gridDim.x, xcd = blockIdx.x & 7u;
+    const unsigned work = xcd * (total >> 3) + min(xcd, total & 7u) + (blockIdx.x >> 3);
+    const int64_t r0 = (int64_t)(work / col_tiles) * kBlk, c0 = (int64_t)(work % col_tiles) * WC;
+    {
+        const int c = tid % (WC / 8) * 8, sub = tid / (WC / 8);
+        float v[kBlk / PASS][8];
+#pragma unroll
+        for (int i = 0; i < kBlk / PASS; ++i) {
+            const int64_t row = r0 + i * PASS + sub;
+            if (row < x_rows)
+                load_run<8>(x + row * ld_x, c0 + c, x_cols, v[i]);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kBlk / PASS; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tile[(i * PASS + sub) * LD + c + e] = v[i][e];
+    }
+    __syncthreads();
+    const int seg = tid & 3;
+    constexpr int COLS = WC / 64;                              // columns per thread
+    float amax[COLS];
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) {
+        const int c = (tid >> 2) + k * 64;
+        amax[k] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) amax[k] = fmaxf(amax[k], finite_magnitude(tile[(seg * 32 + e) * LD + c]));
+        amax[k] = fmaxf(amax[k], __shfl_xor(amax[k], 1));
+        amax[k] = fmaxf(amax[k], __shfl_xor(amax[k], 2));
+    }
+    if (WC == 128) {
+        float m = fmaxf(amax[0], amax[COLS - 1]);
+        for (int o = 4; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if ((tid & 63) == 0) wave_max[tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+#pragma unroll
+        for (int k = 0; k < COLS; ++k) amax[k] = m;
+        if (tid == 0) scale[r0 / kBlk * ld_s + c0 / kBlk] = (uint8_t)scale_byte(m);
+    }
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) {
+        const int c = (tid >> 2) + k * 64;
+        const unsigned byte = scale_byte(amax[k]);
+        const float inv = inverse_scale(byte);
+        if (WC == 64 && seg == 0) bytes[c] = (uint8_t)byte;
+        if (c0 + c >= x_cols) continue;
+        unsigned w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float t[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = no_infinity(tile[(seg * 32 + i * 4 + e) * LD + c] * inv);
+            w[i] = pack4_e4m3(t[0], t[1], t[2], t[3]);
+        }
+        intx4* dst = reinterpret_cast<intx4*>(q + (c0 + c) * ld_q + r0 + seg * 32);
+        dst[0] = intx4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+        dst[1] = intx4{(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
+    }
+    if (WC == 64) {
+        __syncthreads();
+        if (tid < 64 && c0 + tid < x_cols) scale[r0 / kBlk * ld_s + c0 + tid] = bytes[tid];
     }
 }
 
@@ -109,7 +278,6 @@ struct GemmArgs {
     int64_t lda, ldas, ldb, ldbs, ldc;
     int64_t M;
     int N, K;
-    bool vec;            // rows of C (in linear_fp8's kernel: of A) start on the width of a vector access
 };
 
 // scale byte -> the float whose exponent field it is (what the conversion below reads)
@@ -129,51 +297,19 @@ __device__ __forceinline__ void store_c(void* c, int64_t at, float v) {
     else
         reinterpret_cast<__bf16*>(c)[at] = (__bf16)v;
 }
-// 4 neighbouring columns of a row, of which `left` exist; wide: rows start on the vector's alignment
+// 4 neighbouring columns of a row, of which `left` exist
 template <bool OUT_F32>
-__device__ __forceinline__ void store_c4(void* c, int64_t at, floatx4 v, int left, bool wide) {
-    if (wide && left >= 4) {
+__device__ __forceinline__ void store_c4(void* c, int64_t at, floatx4 v, int left) {
+    if (left >= 4) {
         if (OUT_F32)
-            *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(c) + at) = v;
+            *reinterpret_cast<floatx4_any*>(reinterpret_cast<float*>(c) + at) = v;
         else
-            *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(c) + at) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+            *reinterpret_cast<bf16x4_any*>(reinterpret_cast<__bf16*>(c) + at) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (e < left) store_c<OUT_F32>(c, at + e, v[e]);
-}
-
-// NV values x[k0 ..] of a row of K (zeros beyond); vec: rows start on 16 bytes
-template <int NV>
-__device__ __forceinline__ void load_run(const float* x, int k0, int K, bool vec, float* v) {
-    if (vec && k0 + NV <= K) {
-#pragma unroll
-        for (int e = 0; e < NV; e += 4) {
-            const floatx4 t = *reinterpret_cast<const floatx4*>(x + k0 + e);
-            v[e] = t[0]; v[e + 1] = t[1]; v[e + 2] = t[2]; v[e + 3] = t[3];
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < NV; ++e) v[e] = k0 + e < K ? x[k0 + e] : 0.0f;
-}
-template <int NV>
-__device__ __forceinline__ void load_run(const uint16_t* x, int k0, int K, bool vec, float* v) {
-    if (vec && k0 + NV <= K) {
-#pragma unroll
-        for (int e = 0; e < NV; e += 8) {
-            const intx4 t = *reinterpret_cast<const intx4*>(x + k0 + e);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[e + 2 * i] = __int_as_float(t[i] << 16);
-                v[e + 2 * i + 1] = __int_as_float(t[i] & (int)0xFFFF0000);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < NV; ++e) v[e] = k0 + e < K ? load_f32(x + k0 + e) : 0.0f;
 }
 
 // ---- few rows of A (M <= 64): bound by reading B once
@@ -212,7 +348,7 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k)
                 const XT* xp = reinterpret_cast<const XT*>(g.a) + m * g.lda;
                 const int k0 = kb * kBlk + kg * 32;
                 float v[32], amax = 0.0f;
-                load_run<32>(xp, k0, g.K, g.vec, v);
+                load_run<32>(xp, k0, g.K, v);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) amax = fmaxf(amax, finite_magnitude(v[e]));
                 amax = fmaxf(amax, __shfl_xor(amax, 16));
@@ -422,7 +558,6 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
     // lane (r, kg) holds C[m0 + wm TM + 16 i + r][n0 + wn TN + 16 j + 4 kg .. + 3]
     const bool partial = a.splits > 1;
     float* part = partial ? a.part + (int64_t)split * g.M * g.N : nullptr;
-    const bool wide = partial ? (g.N & 3) == 0 : g.vec;
 #pragma unroll
     for (int j = 0; j < IN; ++j) {
         const int n = n0 + wn * TN + j * 16 + kg * 4;
@@ -436,9 +571,9 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
             if (m >= g.M) continue;
             const floatx4 v = acc[i][j] + bias;
             if (partial)
-                store_c4<true>(part, m * g.N + n, v, g.N - n, wide);
+                store_c4<true>(part, m * g.N + n, v, g.N - n);
             else
-                store_c4<OUT_F32>(g.c, m * g.ldc + n, v, g.N - n, wide);
+                store_c4<OUT_F32>(g.c, m * g.ldc + n, v, g.N - n);
         }
     }
 }
@@ -456,8 +591,6 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const float* __restrict_
     }
 }
 
-std::mutex g_tile_mutex;
-
 template <int BM, int BN, int WGM, int WGN, bool OUT_F32, int BROWS>
 int launch_tile(const TileArgs& a, hipStream_t s) {
     constexpr int bytes = 2 * tile_stage_bytes<BM, BN>();
@@ -466,7 +599,7 @@ int launch_tile(const TileArgs& a, hipStream_t s) {
     int dev = 0;
     OCR_HIP_CHECK(hipGetDevice(&dev));
     {
-        std::lock_guard<std::mutex> lock(g_tile_mutex);
+        std::lock_guard<std::mutex> lock(g_lds_mutex);
         if (!opted[dev & 63]) {
             OCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
             opted[dev & 63] = true;
@@ -531,6 +664,44 @@ int launch_rows_any(const GemmArgs& g, bool f32, int b_block_rows, hipStream_t s
 constexpr int kMaxRows = 64;          // gemm_rows_kernel: rows of A
 constexpr int kMaxOwnRows = 32;       // the same, quantising them itself
 
+template <class T>
+int launch_quantize(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int block_rows, bool transpose, uint8_t* q, int64_t ld_q, uint8_t* scale,
+                    int64_t ld_s, hipStream_t s) {
+    const int64_t nkb = (cols + kBlk - 1) / kBlk, nrb = (rows + kBlk - 1) / kBlk;
+    int64_t grid;
+    if (transpose) {
+        const int wc = block_rows == 1 ? 64 : 128;
+        const int64_t col_tiles = (cols + wc - 1) / wc;
+        grid = nrb * col_tiles;
+        OCR_REQUIRE(grid * 256 < (1ll << 32), "quantize_fp8: too many blocks");
+        const size_t lds = (size_t)kBlk * (wc + 1) * sizeof(float);
+        if (wc == 64) {
+            hipLaunchKernelGGL((quantize_transpose_kernel<T, 64>), dim3((unsigned)grid), dim3(256), lds, s, x, ld_x, rows, cols, q, ld_q, scale, ld_s, (unsigned)col_tiles);
+        } else {
+            static bool opted[64] = {};
+            int dev = 0;
+            OCR_HIP_CHECK(hipGetDevice(&dev));
+            std::lock_guard<std::mutex> lock(g_lds_mutex);
+            if (!opted[dev & 63]) {
+                OCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&quantize_transpose_kernel<T, 128>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+                opted[dev & 63] = true;
+            }
+            hipLaunchKernelGGL((quantize_transpose_kernel<T, 128>), dim3((unsigned)grid), dim3(256), lds, s, x, ld_x, rows, cols, q, ld_q, scale, ld_s, (unsigned)col_tiles);
+        }
+    } else if (block_rows == 1) {
+        const int64_t chunks = (nkb + kBlocksWg - 1) / kBlocksWg;
+        grid = (rows + kRowsWg - 1) / kRowsWg * chunks;
+        OCR_REQUIRE(grid * 256 < (1ll << 32), "quantize_fp8: too many blocks");
+        hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)grid), dim3(256), 0, s, x, ld_x, rows, cols, q, ld_q, scale, ld_s, (unsigned)chunks);
+    } else {
+        grid = nrb * nkb;
+        OCR_REQUIRE(grid * 256 < (1ll << 32), "quantize_fp8: too many blocks");
+        hipLaunchKernelGGL(quantize_block_kernel<T>, dim3((unsigned)grid), dim3(256), 0, s, x, ld_x, rows, cols, q, ld_q, scale, ld_s, (unsigned)nkb);
+    }
+    OCR_HIP_CHECK(hipGetLastError());
+    return OCRHIP_OK;
+}
+
 }  // namespace
 
 int launch_quantize_fp8(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, int block_rows, bool transpose,
@@ -540,13 +711,8 @@ int launch_quantize_fp8(const void* x, int x_dtype, int64_t rows, int64_t cols, 
     const int64_t rb = (R + block_rows - 1) / block_rows, cb = (C + kBlk - 1) / kBlk;
     const double n = (double)rows * cols;
     ProfScope prof(transpose ? "quantize_fp8<t>" : "quantize_fp8", 2.0 * n, n * ((x_dtype == OCRHIP_F32 ? 4.0 : 2.0) + 1.0) + (double)rb * cb, s);
-    const dim3 grid((unsigned)rb, (unsigned)cb);
-    if (x_dtype == OCRHIP_F32)
-        hipLaunchKernelGGL(quantize_simple_kernel<float>, grid, dim3(256), 0, s, (const float*)x, ld_x, R, C, block_rows, transpose ? 1 : 0, q, ld_q, scale, ld_scale);
-    else
-        hipLaunchKernelGGL(quantize_simple_kernel<uint16_t>, grid, dim3(256), 0, s, (const uint16_t*)x, ld_x, R, C, block_rows, transpose ? 1 : 0, q, ld_q, scale, ld_scale);
-    OCR_HIP_CHECK(hipGetLastError());
-    return OCRHIP_OK;
+    return x_dtype == OCRHIP_F32 ? launch_quantize((const float*)x, rows, cols, ld_x, block_rows, transpose, q, ld_q, scale, ld_scale, s)
+                                 : launch_quantize((const uint16_t*)x, rows, cols, ld_x, block_rows, transpose, q, ld_q, scale, ld_scale, s);
 }
 
 size_t gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) {
@@ -559,8 +725,7 @@ int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, 
                     void* c, int c_dtype, int64_t ld_c, void* ws, hipStream_t s) {
     if (M == 0 || N == 0) return OCRHIP_OK;
     const bool f32 = c_dtype == OCRHIP_F32;
-    const bool vec = ld_c % 4 == 0 && reinterpret_cast<uintptr_t>(c) % (f32 ? 16 : 8) == 0;
-    GemmArgs g{a.q, a.scale, b.q, b.scale, bias, c, a.ld, a.ld_scale, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K, vec};
+    GemmArgs g{a.q, a.scale, b.q, b.scale, bias, c, a.ld, a.ld_scale, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K};
     const double flops = 2.0 * (double)M * N * K, bytes = (double)(M + N) * K + (f32 ? 4.0 : 2.0) * (double)M * N;
     if (M <= kMaxRows) {
         ProfScope prof(f32 ? "gemm_fp8<rows,f32>" : "gemm_fp8<rows,bf16>", flops, bytes, s);
@@ -596,8 +761,7 @@ int launch_linear_fp8_rows(const void* x, int x_dtype, int64_t ld_x, const Fp8Op
                            void* c, int c_dtype, int64_t ld_c, hipStream_t s) {
     if (M == 0 || N == 0) return OCRHIP_OK;
     const bool f32 = c_dtype == OCRHIP_F32, xf32 = x_dtype == OCRHIP_F32;
-    const bool vec = ld_x % (xf32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    GemmArgs g{reinterpret_cast<const uint8_t*>(x), nullptr, b.q, b.scale, bias, c, ld_x, 0, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K, vec};
+    GemmArgs g{reinterpret_cast<const uint8_t*>(x), nullptr, b.q, b.scale, bias, c, ld_x, 0, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K};
     ProfScope prof("linear_fp8<rows>", 2.0 * (double)M * N * K, (xf32 ? 4.0 : 2.0) * (double)M * K + (double)N * K + (f32 ? 4.0 : 2.0) * (double)M * N, s);
     return xf32 ? launch_rows_any<float>(g, f32, b_block_rows, s) : launch_rows_any<uint16_t>(g, f32, b_block_rows, s);
 }
