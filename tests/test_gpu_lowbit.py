@@ -451,6 +451,17 @@ def test_distillation_of_a_nan_entry_is_nan(ctx):
         assert torch.isnan(out['grad'][1]).all() and not torch.isnan(out['grad'][[0, 2]]).any()
 
 
+@pytest.mark.parametrize('v', [97, 1000, 6719, 40000])
+def test_distillation_without_a_teacher_is_zero_whatever_the_logits_are(ctx, v):
+    x = logits(4, v, 1).cuda()
+    x[0, 1], x[1, v - 1], x[2] = float('nan'), float('inf'), float('nan')
+    z, i = torch.zeros(4, 3, device='cuda'), torch.full((4, 3), -1, dtype=torch.int32, device='cuda')
+    i[3] = torch.arange(3, dtype=torch.int32)
+    z[3] = -float('inf')
+    out = ctx.distill_loss(x, z, i, want_grad=True)
+    assert not out['loss'].any() and not out['grad'].any()
+
+
 @pytest.mark.parametrize('rest', [False, True])
 def test_distillation_where_teacher_and_student_nearly_agree(ctx, rest):
     """Losses of 1e-9 next to terms of order 1."""
