@@ -79,6 +79,7 @@ __device__ __forceinline__ float no_infinity(float v) { return fabsf(v) == INFIN
 typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int intx4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef __bf16 bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 bf16x8_any __attribute__((ext_vector_type(8), aligned(2)));
 
 // NV (a multiple of 8) values x[k0 ..] of a row of K, zeros beyond
 template <int NV>
@@ -497,13 +498,15 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
         for (int j = 0; j < IN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
     issue(kb0);
+    const bool two = kb1 - kb0 == 2;                    // both blocks fit the buffers: one wait for memory
+    if (two) issue(kb0 + 1);
     const int a_row = wm * TM + r, b_row = wn * TN + r;
     for (int kb = kb0; kb < kb1; ++kb) {
         // my copies have landed and my reads of the other buffer are done; behind the barrier everybody's
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (kb + 1 < kb1) issue(kb + 1);
+        if (!two && kb + 1 < kb1) issue(kb + 1);
         const unsigned char* base = lds + (kb & 1) * STAGE;
         const unsigned char* pa = base + a_row * kBlk;
         const unsigned char* pb = base + (BM + b_row) * kBlk;
@@ -555,25 +558,69 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
             }
         }
     }
-    // lane (r, kg) holds C[m0 + wm TM + 16 i + r][n0 + wn TN + 16 j + 4 kg .. + 3]
+    // Lane (r, kg) holds C[m0 + wm TM + 16 i + r][n0 + wn TN + 16 j + 4 kg .. + 3]: 16 bytes of 16 rows per store.  Every
+    // wave turns its 16-row slices through an LDS area of its own into runs of whole rows of its TN columns, which fill
+    // the lines they touch (rows of odd length start anywhere in one).
     const bool partial = a.splits > 1;
-    float* part = partial ? a.part + (int64_t)split * g.M * g.N : nullptr;
-#pragma unroll
-    for (int j = 0; j < IN; ++j) {
-        const int n = n0 + wn * TN + j * 16 + kg * 4;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();          // every wave is done with the operands
+    asm volatile("" ::: "memory");
+    if (partial || OUT_F32) {
+        constexpr int SROW = TN * 4 + 16, LANES = TN / 4;      // bytes of a staged row, lanes of a row
+        unsigned char* mine = lds + wave * (16 * SROW);
+        float* out = partial ? a.part + (int64_t)split * g.M * g.N : reinterpret_cast<float*>(g.c);
+        const int64_t ldo = partial ? g.N : g.ldc;
+        const int c4 = lane % LANES * 4, n = n0 + wn * TN + c4;
         floatx4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
         if (g.bias && !partial)
 #pragma unroll
             for (int e = 0; e < 4; ++e) bias[e] = n + e < g.N ? g.bias[n + e] : 0.0f;
 #pragma unroll
         for (int i = 0; i < IM; ++i) {
-            const int64_t m = m0 + wm * TM + i * 16 + r;
-            if (m >= g.M) continue;
-            const floatx4 v = acc[i][j] + bias;
-            if (partial)
-                store_c4<true>(part, m * g.N + n, v, g.N - n);
-            else
-                store_c4<OUT_F32>(g.c, m * g.ldc + n, v, g.N - n);
+#pragma unroll
+            for (int j = 0; j < IN; ++j) *reinterpret_cast<floatx4*>(mine + r * SROW + (j * 16 + kg * 4) * 4) = acc[i][j];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int t = 0; t < 16 * LANES / 64; ++t) {
+                const int row = t * (64 / LANES) + lane / LANES;
+                const int64_t m = m0 + wm * TM + i * 16 + row;
+                const floatx4 v = *reinterpret_cast<const floatx4*>(mine + row * SROW + c4 * 4) + bias;
+                if (m < g.M) store_c4<true>(out, m * ldo + n, v, g.N - n);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    } else {
+        constexpr int SROW = TN * 2 + 16, LANES = TN / 8;
+        unsigned char* mine = lds + wave * (16 * SROW);
+        const int c8 = lane % LANES * 8, nw = n0 + wn * TN + c8;
+#pragma unroll
+        for (int i = 0; i < IM; ++i) {
+#pragma unroll
+            for (int j = 0; j < IN; ++j) {
+                const int n = n0 + wn * TN + j * 16 + kg * 4;
+                floatx4 v = acc[i][j];
+                if (g.bias)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += n + e < g.N ? g.bias[n + e] : 0.0f;
+                *reinterpret_cast<bf16x4*>(mine + r * SROW + (j * 16 + kg * 4) * 2) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int t = 0; t < 16 * LANES / 64; ++t) {
+                const int row = t * (64 / LANES) + lane / LANES;
+                const int64_t m = m0 + wm * TM + i * 16 + row;
+                const bf16x8 v = *reinterpret_cast<const bf16x8*>(mine + row * SROW + c8 * 2);
+                if (m >= g.M) continue;
+                __bf16* dst = reinterpret_cast<__bf16*>(g.c) + m * g.ldc + nw;
+                if (nw + 8 <= g.N) {
+                    *reinterpret_cast<bf16x8_any*>(dst) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (nw + e < g.N) dst[e] = v[e];
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
