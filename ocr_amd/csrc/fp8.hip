@@ -408,9 +408,9 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k)
 //
 // A workgroup computes BM x BN of C.  Per block of 128 values of k its rows of A and B (whole 128-byte lines) and A's scale
 // bytes go straight from memory to LDS; the next block's copies are in flight while this one is multiplied (two buffers,
-// one barrier per block).  A row is 8 pieces of 16 bytes; piece c of row r lies at place c ^ (r / 2 % 8), so that the 16
-// lanes of a read phase (16 rows, the same piece) hit 16 different groups of banks; the copy writes lane after lane, so
-// the permutation is applied to the address it reads from.  Rows beyond M or N are offsets beyond the descriptor: zeros.
+// one barrier per block).  A row is 8 pieces of 16 bytes; piece c of row r lies at place c ^ place(r), chosen so that the 16
+// lanes of a read phase (lanes 0-3, 12-15 and 20-27 of a half wave, and the other 16) hit 16 different groups of banks; the
+// copy writes lane after lane, so the permutation is applied to the address it reads from.  Rows beyond M or N are offsets beyond the descriptor: zeros.
 // B is the matrix instruction's row operand, A its column operand: a lane then holds 4 neighbouring columns of one row.
 struct TileArgs {
     GemmArgs g;
@@ -427,6 +427,8 @@ __device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t rsrc, unsigned cha
 __device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t rsrc, unsigned char* dst, int voff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)dst, 4, voff, 0, 0, 0);
 }
+
+__device__ __forceinline__ int place(int row) { return (row >> 1 & 3) << 1 | (row >> 3 & 1); }
 
 template <int BM, int BN>
 constexpr int tile_stage_bytes() { return (BM + BN) * kBlk + 512; }      // operands, then 256 scale bytes of A and of B
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
     for (int i = 0; i < PER; ++i) {
         const int c = wave * PER + i;
         const int row = (c < NA ? c : c - NA) * 8 + (lane >> 3);
-        const int piece = (lane & 7) ^ (row >> 1 & 7);
+        const int piece = (lane & 7) ^ place(row);
         const bool ok = row < (c < NA ? rows_a : rows_b);
         src[i] = ok ? row * (int)(c < NA ? g.lda : g.ldb) + piece * 16 : (int)0x80000000;
     }
@@ -512,7 +514,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
         const unsigned char* pb = base + (BM + b_row) * kBlk;
         const unsigned char* psa = base + (BM + BN) * kBlk + a_row;
         const unsigned char* psb = base + (BM + BN) * kBlk + 256 + b_row;
-        const int sw = r >> 1;                          // rows 16 apart have the same permutation
+        const int sw = place(r);                        // rows 16 apart have the same permutation
         int sb = sb_next;
         if (BROWS != 1 && kb + 1 < kb1) sb_next = g.bs[(int64_t)(kb + 1) * g.ldbs + sb_col];
         if constexpr (OUT_F32) {
@@ -673,7 +675,9 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
     p.tiles_n = (N + p.bn - 1) / p.bn;
     const int64_t tiles = p.tiles_m * p.tiles_n;
     int64_t splits = 1;
-    if (tiles < 256 && nkb >= 8) splits = std::min<int64_t>(std::min<int64_t>(nkb / 4, (512 + tiles - 1) / tiles), 16);
+    // few tiles, long k: pieces of k until the device is full (two workgroups on each of 256 compute units) and no further,
+    // for the 513th would make a second round of them all
+    if (tiles < 256 && nkb >= 8) splits = std::min<int64_t>(std::min<int64_t>(nkb / 4, 512 / tiles), 16);
     p.kb_split = (int)((nkb + splits - 1) / splits);
     p.splits = (int)((nkb + p.kb_split - 1) / p.kb_split);
     return p;
