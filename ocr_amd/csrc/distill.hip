@@ -13,6 +13,7 @@
 // classes outside the entries are float32: an error there changes the loss only in proportion to q_rest - p_rest.  What
 // enters to first order (the entries' probabilities, the logarithms, the sum of the terms: K numbers per row) is float64.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -111,28 +112,69 @@ typedef __bf16 bf16x8_any __attribute__((ext_vector_type(8), aligned(2)));
 template <class T>
 constexpr int kPiece = 16 / sizeof(T);
 
-// piece c of a row of V; classes from V on are -infinity
-__device__ __forceinline__ void load_piece(const float* p, int c, int V, float* v) {
-    if (c * 4 + 4 <= V) {
-        const floatx4 t = *reinterpret_cast<const floatx4_any*>(p + c * 4);
-        v[0] = t[0]; v[1] = t[1]; v[2] = t[2]; v[3] = t[3];
-        return;
-    }
+// Piece q of a row of V classes, those from V on as -infinity.  The load has no branch - a load in one makes the compiler
+// wait for the one in front of it -: the last piece is read from V - P on and put in place when it is used, pieces behind
+// it are read like it.
+__device__ __forceinline__ void unpack_piece(uintx4 t, float (&v)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = c * 4 + e < V ? p[c * 4 + e] : -INFINITY;
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(t[i]);
 }
-__device__ __forceinline__ void load_piece(const uint16_t* p, int c, int V, float* v) {
-    if (c * 8 + 8 <= V) {
-        const uintx4 t = *reinterpret_cast<const uintx4_any*>(p + c * 8);
+__device__ __forceinline__ void unpack_piece(uintx4 t, float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(t[i] << 16);
-            v[2 * i + 1] = __uint_as_float(t[i] & 0xFFFF0000u);
-        }
-        return;
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(t[i] << 16);
+        v[2 * i + 1] = __uint_as_float(t[i] & 0xFFFF0000u);
     }
+}
+__device__ __forceinline__ uintx4 pack_piece(const float (&v)[4]) {
+    return uintx4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+__device__ __forceinline__ uintx4 pack_piece(const float (&v)[8]) {
+    return __builtin_bit_cast(uintx4, bf16x8{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3], (__bf16)v[4], (__bf16)v[5], (__bf16)v[6], (__bf16)v[7]});
+}
+template <class T>
+__device__ __forceinline__ uintx4 load_raw(const T* p, int q, int V) {
+    constexpr int P = kPiece<T>;
+    if (V < P) {                                    // uniform
+        float v[P];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c * 8 + e < V ? load_f32(p + c * 8 + e) : -INFINITY;
+        for (int e = 0; e < P; ++e) v[e] = e < V ? load_f32(p + e) : 0.0f;
+        return pack_piece(v);
+    }
+    return *reinterpret_cast<const uintx4_any*>(p + min(q * P, V - P));
+}
+// t without its first 1, 2 or 4 classes, -infinity behind
+template <int D>
+__device__ __forceinline__ uintx4 drop(uintx4 t, const float*) {
+    return D == 1 ? uintx4{t[1], t[2], t[3], 0xFF800000u} : uintx4{t[2], t[3], 0xFF800000u, 0xFF800000u};
+}
+template <int D>
+__device__ __forceinline__ uintx4 drop(uintx4 t, const uint16_t*) {
+    constexpr unsigned kNone = 0xFF80FF80u;
+    if (D == 1) return uintx4{t[0] >> 16 | t[1] << 16, t[1] >> 16 | t[2] << 16, t[2] >> 16 | t[3] << 16, t[3] >> 16 | 0xFF800000u};
+    return D == 2 ? uintx4{t[1], t[2], t[3], kNone} : uintx4{t[2], t[3], kNone, kNone};
+}
+template <class T>
+__device__ __forceinline__ uintx4 in_place(uintx4 t, const T* p, int q, int V) {
+    constexpr int P = kPiece<T>;
+    if ((q + 1) * P > V) {
+        if (V < P) {
+            float v[P];
+            unpack_piece(t, v);
+#pragma unroll
+            for (int e = 0; e < P; ++e) v[e] = q == 0 && e < V ? v[e] : -INFINITY;
+            return pack_piece(v);
+        }
+        const int d = q * P - (V - P);
+        if (d & 1) t = drop<1>(t, p);
+        if (d & 2) t = drop<2>(t, p);
+        if (P == 8 && d & 4) t = drop<4>(t, p);
+        if (d >= P) {
+            constexpr unsigned kNone = P == 8 ? 0xFF80FF80u : 0xFF800000u;
+            t = uintx4{kNone, kNone, kNone, kNone};
+        }
+    }
+    return t;
 }
 __device__ __forceinline__ void store_piece(float* p, int c, int V, const float* v) {
     if (c * 4 + 4 <= V) {
@@ -155,6 +197,59 @@ __device__ __forceinline__ void store_piece(uint16_t* p, int c, int V, const flo
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// ---- float64 for a row's few numbers: each a fraction of the library's instructions, which a short row is bound by
+//
+// 1 / x, x neither 0 nor infinite: two Newton steps from the instruction's estimate.
+__device__ __forceinline__ double rcp64(double x) {
+    double r = __builtin_amdgcn_rcp(x);
+    r = fma(fma(-x, r, 1.0), r, r);
+    return fma(fma(-x, r, 1.0), r, r);
+}
+// exp(x): x = n ln 2 + r, |r| <= ln 2 / 2, the series of exp to r^12 / 12! (the next term is 2e-16 of the value); 0 from
+// -infinity to -800, NaN stays NaN (and +infinity becomes one).
+__device__ __forceinline__ double exp64(double x) {
+    x = x < -800.0 ? -800.0 : x;
+    const double n = rint(x * 1.4426950408889634074);
+    const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.693147180369123816490, x));
+    double p = 1.0 / 479001600.0;
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
+}
+// log(x), x positive and finite: x = 2^e m, sqrt(1/2) <= m < sqrt(2), s = (m - 1) / (m + 1), |s| < 0.172, log m =
+// 2 (s + s^3 / 3 + ... + s^21 / 21).  NaN stays NaN.
+__device__ __forceinline__ double log64(double x) {
+    double m = __builtin_amdgcn_frexp_mant(x);
+    int e = __builtin_amdgcn_frexp_exp(x);
+    const bool low = m < 0.70710678118654752440;
+    m = low ? m + m : m;
+    e = low ? e - 1 : e;
+    const double s = (m - 1.0) * rcp64(m + 1.0), q = s * s;
+    double p = 2.0 / 21.0;
+    p = fma(p, q, 2.0 / 19.0);
+    p = fma(p, q, 2.0 / 17.0);
+    p = fma(p, q, 2.0 / 15.0);
+    p = fma(p, q, 2.0 / 13.0);
+    p = fma(p, q, 2.0 / 11.0);
+    p = fma(p, q, 2.0 / 9.0);
+    p = fma(p, q, 2.0 / 7.0);
+    p = fma(p, q, 2.0 / 5.0);
+    p = fma(p, q, 2.0 / 3.0);
+    return fma((double)e, 0.69314718055994530942, fma(p * q, s, 2.0 * s));
+}
+// log of a sum of exponentials, which may be 0 or infinite
+__device__ __forceinline__ double log_sum(double x) { return x == 0.0 ? -INFINITY : x == INFINITY ? x : log64(x); }
+
 // ---- top logits
 //
 // Bound by reading the logits once.  Rows of up to 128 classes and 16 entries: 16 lanes per row, the maximum taken away K
@@ -173,21 +268,20 @@ struct TopArgs {
     float* lse;
 };
 
-__device__ __forceinline__ float row_lse(float high, float inv_t, double sum) {
-    return fabsf(high) == INFINITY ? high : (float)((double)high * inv_t + log(sum));
-}
-
 template <class T>
 __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
     constexpr int P = kPiece<T>, N = 128 / 16 / P;
     const int part = threadIdx.x & 15;
     for (int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); row < a.rows; row += (int64_t)gridDim.x * 16) {
         const T* p = a.x + row * a.ld;
+        uintx4 raw[N];
         float v[N][P];
         unsigned key[N][P];
         unsigned best = 0, at = 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_piece(p, part + 16 * i, a.V, v[i]);
+        for (int i = 0; i < N; ++i) raw[i] = load_raw(p, part + 16 * i, a.V);
+#pragma unroll
+        for (int i = 0; i < N; ++i) unpack_piece(in_place(raw[i], p, part + 16 * i, a.V), v[i]);
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -219,184 +313,319 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
         }
         if (a.lse) {
             const float c = a.inv_t * kLog2e;
+            const float base = fabsf(high) == INFINITY || high != high ? 0.0f : high;
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int e = 0; e < P; ++e) sum += __builtin_amdgcn_exp2f((v[i][e] - high) * c);
+                for (int e = 0; e < P; ++e) sum += __builtin_amdgcn_exp2f((v[i][e] - base) * c);
             sum = group_sum<16>(sum);
-            if (part == 0) a.lse[row] = row_lse(high, a.inv_t, (double)sum);
+            if (part == 0) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)sum));
         }
     }
 }
 
+// Rows of up to kWaveClasses classes: in LDS, one wave's own, so nothing waits for another.
+constexpr int kWaveClasses = 2048;
+constexpr size_t kWaveBytes = 16384, kRowBytes = 32768;
+#ifndef KOCC
+#define KOCC 3
+#endif
+constexpr int kDistillOccupancy = KOCC;
 constexpr int kTopList = 512;          // candidates of a row that LDS holds
 
-// WAVES waves per row.  HELD > 0: pieces per thread kept in registers (rows of up to 64 * WAVES * HELD pieces, one read);
-// 0: the row is read twice, for the lanes' maxima and for the values that reach the bound.
-template <class T, int WAVES, int HELD>
-__global__ __launch_bounds__(WAVES * 64) void top_kernel(TopArgs<T> a) {
-    constexpr int P = kPiece<T>, THREADS = WAVES * 64, KEEP = HELD ? HELD : 1, AHEAD = 4;
+// what one lane wrote to LDS is what another reads: same wave, so the order of the instructions is enough
+__device__ __forceinline__ void lds_phase() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kBatch = 8;              // pieces a lane has in flight
+
+// the row to LDS (pieces of 16 bytes; classes behind the last are -infinity); returns the lane's maximum.  `between` runs
+// while the first pieces are on their way.
+template <int THREADS, class T, class F>
+__device__ __forceinline__ float row_to_lds(const T* p, int V, uintx4* buf, F between) {
+    constexpr int P = kPiece<T>;
+    const int pieces = (V + P - 1) / P, tid = threadIdx.x;
+    float m = -INFINITY;
+    for (int q = tid; q - tid < pieces; q += THREADS * kBatch) {
+        uintx4 t[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) t[i] = load_raw(p, q + i * THREADS, V);
+        if (q == tid) between();
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (q + i * THREADS < pieces) {
+                const uintx4 u = in_place(t[i], p, q + i * THREADS, V);
+                float v[P];
+                unpack_piece(u, v);
+#pragma unroll
+                for (int e = 0; e < P; ++e) m = fmaxf(m, v[e]);
+                buf[q + i * THREADS] = u;
+            }
+    }
+    return m;
+}
+
+// the largest bound of 20 leading bits that K of the wave's keys reach (0: fewer than K lanes have one)
+__device__ __forceinline__ unsigned bisect(const unsigned* keys, int n, int K) {
+    unsigned bound = 0;
+    for (int bit = 31; bit >= 12; --bit) {
+        const unsigned next = bound | 1u << bit;
+        int reach = 0;
+        for (int w = 0; w < n; ++w) reach += __popcll(__ballot(keys[w] >= next));
+        if (reach >= K) bound = next;
+    }
+    return bound;
+}
+
+// The K largest of the list, each at the rank that counting the larger ones gives it.
+template <class T>
+__device__ __forceinline__ void write_ranked(const TopArgs<T>& a, int64_t row, const unsigned long long* list, int n, int tid, int threads) {
+    for (int i = tid; i < n; i += threads) {
+        const unsigned long long own = list[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += list[j] > own ? 1 : 0;
+        if (rank < a.K) {
+            a.values[row * a.K + rank] = key_value((unsigned)(own >> 32));
+            a.index[row * a.K + rank] = (int)(0xFFFFFFFFu - (unsigned)own);
+        }
+    }
+}
+
+// The same without a list: the maxima one by one, a pass over the row each.
+template <int WAVES, class T>
+__device__ __forceinline__ void write_one_by_one(const TopArgs<T>& a, int64_t row, unsigned long long* wave_best) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const T* p = a.x + row * a.ld;
+    unsigned long long last = ~0ull;
+    for (int k = 0; k < a.K; ++k) {
+        unsigned long long best = 0;
+        for (int at = tid; at < a.V; at += WAVES * 64) {
+            const unsigned long long own = (unsigned long long)order_key(load_f32(p + at)) << 32 | (0xFFFFFFFFu - (unsigned)at);
+            if (own < last && own > best) best = own;
+        }
+        const unsigned hi = group_max<64>((unsigned)(best >> 32));
+        const unsigned lo = group_max<64>((unsigned)(best >> 32) == hi ? (unsigned)best : 0u);
+        if (lane == 0) wave_best[wave] = (unsigned long long)hi << 32 | lo;
+        __syncthreads();
+        last = wave_best[0];
+        for (int w = 1; w < WAVES; ++w) last = max(last, wave_best[w]);
+        __syncthreads();
+        if (tid == 0) {
+            a.values[row * a.K + k] = key_value((unsigned)(last >> 32));
+            a.index[row * a.K + k] = (int)(0xFFFFFFFFu - (unsigned)last);
+        }
+    }
+}
+
+// One wave per row.
+template <class T>
+__global__ __launch_bounds__(64) void top_wave_kernel(TopArgs<T> a) {
+    constexpr int P = kPiece<T>;
+    extern __shared__ uintx4 buf[];                        // the row
+    __shared__ unsigned long long list[kTopList], wave_best;
+    __shared__ int count;
+    const int lane = threadIdx.x, pieces = (a.V + P - 1) / P;
+    const float c = a.inv_t * kLog2e;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* p = a.x + row * a.ld;
+        if (lane == 0) count = 0;
+        const float mine = row_to_lds<64>(p, a.V, buf, [] {});
+        lds_phase();
+        const unsigned key = lane < pieces ? order_key(mine) : 0u;
+        const unsigned bits = bisect(&key, 1, a.K);
+        const float bound = bits ? key_value(bits) : -INFINITY;
+        const float high = group_max<64>(mine);            // NaN apart
+        const float base = fabsf(high) == INFINITY ? 0.0f : high;
+        float sum = 0.0f;
+        for (int q = lane; q < pieces; q += 64) {
+            float v[P];
+            unpack_piece(buf[q], v);
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                any |= !(v[e] < bound);                    // a NaN as well
+                sum += __builtin_amdgcn_exp2f((v[e] - base) * c);
+            }
+            if (any)
+#pragma unroll
+                for (int e = 0; e < P; ++e)
+                    if (!(v[e] < bound) && q * P + e < a.V) {
+                        const int slot = atomicAdd(&count, 1);
+                        if (slot < kTopList) list[slot] = (unsigned long long)order_key(v[e]) << 32 | (0xFFFFFFFFu - (unsigned)(q * P + e));
+                    }
+        }
+        lds_phase();
+        const int n = count;
+        if (n <= kTopList) {
+            write_ranked(a, row, list, n, lane, 64);
+        } else {
+            write_one_by_one<1>(a, row, &wave_best);
+        }
+        if (a.lse) {
+            sum = group_sum<64>(sum);
+            if (lane == 0) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)sum));
+        }
+        lds_phase();
+    }
+}
+
+// A workgroup of 4 waves per row, N pieces a thread in registers.  The bound: every wave bisects its own 64 maxima for the
+// ceil(K / 4)-th largest, the least of the four is reached by at least K values.
+template <class T, int N>
+__global__ __launch_bounds__(256) void top_block_kernel(TopArgs<T> a) {
+    constexpr int P = kPiece<T>;
+    __shared__ unsigned long long list[kTopList];
+    __shared__ unsigned wave_bits[4];
+    __shared__ float wave_high[4], wave_sum[4];
+    __shared__ unsigned long long wave_best[4];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
+    const float c = a.inv_t * kLog2e;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* p = a.x + row * a.ld;
+        if (tid == 0) count = 0;
+        uintx4 raw[N];
+        float v[N][P], mine = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw[i] = load_raw(p, tid + i * 256, a.V);
+#pragma unroll
+        for (int i = 0; i < N; ++i) unpack_piece(in_place(raw[i], p, tid + i * 256, a.V), v[i]);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < P; ++e) mine = fmaxf(mine, v[i][e]);
+        const unsigned key = tid < pieces ? order_key(mine) : 0u;
+        const unsigned bits = bisect(&key, 1, (a.K + 3) / 4);
+        const float wave_top = group_max<64>(mine);            // NaN apart
+        if (lane == 0) {
+            wave_bits[wave] = bits;
+            wave_high[wave] = wave_top;
+        }
+        __syncthreads();
+        const unsigned least = min(min(wave_bits[0], wave_bits[1]), min(wave_bits[2], wave_bits[3]));
+        const float bound = least ? key_value(least) : -INFINITY;
+        const float high = fmaxf(fmaxf(wave_high[0], wave_high[1]), fmaxf(wave_high[2], wave_high[3]));
+        const float base = fabsf(high) == INFINITY ? 0.0f : high;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                any |= !(v[i][e] < bound);                     // a NaN as well
+                sum += __builtin_amdgcn_exp2f((v[i][e] - base) * c);
+            }
+            if (any)
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    const int at = (tid + i * 256) * P + e;
+                    if (!(v[i][e] < bound) && at < a.V) {
+                        const int slot = atomicAdd(&count, 1);
+                        if (slot < kTopList) list[slot] = (unsigned long long)order_key(v[i][e]) << 32 | (0xFFFFFFFFu - (unsigned)at);
+                    }
+                }
+        }
+        sum = group_sum<64>(sum);
+        if (lane == 0) wave_sum[wave] = sum;
+        __syncthreads();
+        const int n = count;
+        if (n <= kTopList)
+            write_ranked(a, row, list, n, tid, 256);
+        else
+            write_one_by_one<4>(a, row, wave_best);
+        if (a.lse && tid == 255) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3]));
+        __syncthreads();
+    }
+}
+
+// Longer rows: 8 waves per row, which is read twice, for the threads' maxima (and the sum) and for the values that reach
+// the bound.
+template <class T>
+__global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
+    constexpr int P = kPiece<T>, WAVES = 8, THREADS = 512, AHEAD = 4;
     __shared__ unsigned long long list[kTopList];
     __shared__ unsigned maxima[THREADS];
     __shared__ float wave_sum[WAVES];
     __shared__ unsigned long long wave_best[WAVES];
     __shared__ unsigned shared_bound;
+    __shared__ float shared_high;
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int pieces = (a.V + P - 1) / P;
     const float c = a.inv_t * kLog2e;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* p = a.x + row * a.ld;
-        float v[KEEP][P];
-        unsigned mine = 0;
-        float m_own = -INFINITY, s_own = 0.0f;          // HELD 0: running maximum and sum of the thread
+        float m_own = -INFINITY, s_own = 0.0f;             // running maximum and sum of the thread
         if (tid == 0) count = 0;
-        if constexpr (HELD > 0) {
+        for (int q = tid; q < pieces; q += THREADS * AHEAD) {
+            uintx4 raw[AHEAD];
+            float w[AHEAD][P];
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) {
-                if (tid + i * THREADS < pieces)
-                    load_piece(p, tid + i * THREADS, a.V, v[i]);
-                else
+            for (int i = 0; i < AHEAD; ++i) raw[i] = load_raw(p, q + i * THREADS, a.V);
 #pragma unroll
-                    for (int e = 0; e < P; ++e) v[i][e] = -INFINITY;
-            }
+            for (int i = 0; i < AHEAD; ++i) unpack_piece(in_place(raw[i], p, q + i * THREADS, a.V), w[i]);
+            float m = m_own;
 #pragma unroll
-            for (int i = 0; i < HELD; ++i)
+            for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    const unsigned k = (tid + i * THREADS) * P + e < a.V ? order_key(v[i][e]) : 0u;
-                    mine = max(mine, k);
-                }
-        } else {
-            for (int q = tid; q < pieces; q += THREADS * AHEAD) {
-                float w[AHEAD][P];
+                for (int e = 0; e < P; ++e) m = fmaxf(m, w[i][e]);
+            const float base = fabsf(m) == INFINITY ? 0.0f : m;
+            s_own = fabsf(m_own) == INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((m_own - base) * c);
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    if (q + i * THREADS < pieces)
-                        load_piece(p, q + i * THREADS, a.V, w[i]);
-                    else
+            for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-                        for (int e = 0; e < P; ++e) w[i][e] = -INFINITY;
-                }
-                float m = m_own;
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-                    for (int e = 0; e < P; ++e) {
-                        const unsigned k = (q + i * THREADS) * P + e < a.V ? order_key(w[i][e]) : 0u;
-                        mine = max(mine, k);
-                        m = fmaxf(m, w[i][e]);
-                    }
-                const float base = m == -INFINITY ? 0.0f : m;
-                s_own = m_own == -INFINITY ? 0.0f : s_own * __builtin_amdgcn_exp2f((m_own - base) * c);
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-                    for (int e = 0; e < P; ++e) s_own += __builtin_amdgcn_exp2f((w[i][e] - base) * c);
-                m_own = m;
-            }
+                for (int e = 0; e < P; ++e) s_own += __builtin_amdgcn_exp2f((w[i][e] - base) * c);
+            m_own = m;
         }
-        maxima[tid] = mine;
+        maxima[tid] = tid < pieces ? order_key(m_own) : 0u;
         __syncthreads();
         if (wave == 0) {
-            // the largest bound of 20 leading bits that K of the maxima reach
             unsigned m[WAVES], top = 0;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 m[w] = maxima[w * 64 + lane];
                 top = max(top, m[w]);
             }
-            unsigned bound = 0;
-            for (int bit = 31; bit >= 12; --bit) {
-                const unsigned next = bound | 1u << bit;
-                int reach = 0;
-#pragma unroll
-                for (int w = 0; w < WAVES; ++w) reach += __popcll(__ballot(m[w] >= next));
-                if (reach >= a.K) bound = next;
-            }
+            const unsigned bits = bisect(m, WAVES, a.K);
             top = group_max<64>(top);
             if (lane == 0) {
-                shared_bound = max(bound, 1u);
-                wave_best[0] = top;
+                shared_bound = bits;
+                shared_high = key_value(top);
             }
         }
         __syncthreads();
-        const unsigned bound = shared_bound;
-        const float high = key_value((unsigned)wave_best[0]);
-        // the values that reach the bound
-        auto offer = [&](float x, int at) {
-            const unsigned k = order_key(x);
-            if (k >= bound && at < a.V) {
-                const int slot = atomicAdd(&count, 1);
-                if (slot < kTopList) list[slot] = (unsigned long long)k << 32 | (0xFFFFFFFFu - (unsigned)at);
+        const float bound = shared_bound ? key_value(shared_bound) : -INFINITY;
+        const float high = shared_high, base = fabsf(high) == INFINITY ? 0.0f : high;
+        // a thread whose values all lie below the bound has nothing to offer (one that met a NaN has it in its sum)
+        if (!(m_own < bound) || s_own != s_own)
+            for (int q = tid; q < pieces; q += THREADS) {
+                float v[P];
+                unpack_piece(in_place(load_raw(p, q, a.V), p, q, a.V), v);
+#pragma unroll
+                for (int e = 0; e < P; ++e)
+                    if (!(v[e] < bound) && q * P + e < a.V) {
+                        const int slot = atomicAdd(&count, 1);
+                        if (slot < kTopList) list[slot] = (unsigned long long)order_key(v[e]) << 32 | (0xFFFFFFFFu - (unsigned)(q * P + e));
+                    }
             }
-        };
-        if (mine >= bound) {
-            if constexpr (HELD > 0) {
-#pragma unroll
-                for (int i = 0; i < HELD; ++i)
-#pragma unroll
-                    for (int e = 0; e < P; ++e) offer(v[i][e], (tid + i * THREADS) * P + e);
-            } else {
-                for (int q = tid; q < pieces; q += THREADS) {
-                    float w[P];
-                    load_piece(p, q, a.V, w);
-#pragma unroll
-                    for (int e = 0; e < P; ++e) offer(w[e], q * P + e);
-                }
-            }
-        }
-        if (a.lse) {
-            float sum = 0.0f;
-            if constexpr (HELD > 0) {
-#pragma unroll
-                for (int i = 0; i < HELD; ++i)
-#pragma unroll
-                    for (int e = 0; e < P; ++e) sum += __builtin_amdgcn_exp2f((v[i][e] - high) * c);
-            } else {
-                sum = m_own == -INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((m_own - high) * c);
-            }
-            sum = group_sum<64>(sum);
-            if (lane == 0) wave_sum[wave] = sum;
-        }
+        const float own_base = fabsf(m_own) == INFINITY ? 0.0f : m_own;
+        const float sum = group_sum<64>(m_own == -INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((own_base - base) * c));
+        if (lane == 0) wave_sum[wave] = sum;
         __syncthreads();
         const int n = count;
         if (n <= kTopList) {
-            for (int i = tid; i < n; i += THREADS) {
-                const unsigned long long own = list[i];
-                int rank = 0;
-                for (int j = 0; j < n; ++j) rank += list[j] > own ? 1 : 0;
-                if (rank < a.K) {
-                    a.values[row * a.K + rank] = key_value((unsigned)(own >> 32));
-                    a.index[row * a.K + rank] = (int)(0xFFFFFFFFu - (unsigned)own);
-                }
-            }
+            write_ranked(a, row, list, n, tid, THREADS);
         } else {
-            unsigned long long last = ~0ull;
-            for (int k = 0; k < a.K; ++k) {
-                unsigned long long best = 0;
-                for (int at = tid; at < a.V; at += THREADS) {
-                    const unsigned long long key = (unsigned long long)order_key(load_f32(p + at)) << 32 | (0xFFFFFFFFu - (unsigned)at);
-                    if (key < last && key > best) best = key;
-                }
-                const unsigned hi = group_max<64>((unsigned)(best >> 32));
-                const unsigned lo = group_max<64>((unsigned)(best >> 32) == hi ? (unsigned)best : 0u);
-                if (lane == 0) wave_best[wave] = (unsigned long long)hi << 32 | lo;
-                __syncthreads();
-                last = wave_best[0];
-                for (int w = 1; w < WAVES; ++w) last = max(last, wave_best[w]);
-                __syncthreads();
-                if (tid == 0) {
-                    a.values[row * a.K + k] = key_value((unsigned)(last >> 32));
-                    a.index[row * a.K + k] = (int)(0xFFFFFFFFu - (unsigned)last);
-                }
-            }
+            write_one_by_one<WAVES>(a, row, wave_best);
         }
         if (a.lse && tid == 0) {
-            double sum = 0.0;
-            for (int w = 0; w < WAVES; ++w) sum += (double)wave_sum[w];
-            a.lse[row] = row_lse(high, a.inv_t, sum);
+            double total = 0.0;
+            for (int w = 0; w < WAVES; ++w) total += (double)wave_sum[w];
+            a.lse[row] = (float)((double)base * a.inv_t + log_sum(total));
         }
         __syncthreads();
     }
@@ -404,8 +633,42 @@ __global__ __launch_bounds__(WAVES * 64) void top_kernel(TopArgs<T> a) {
 
 // ---- distillation
 
-// What the K entries of a row and the sums over the rest (maximum m_r, sum of exp((s - m_r) / tau)) make of it.  A group of
-// G lanes (16 or 64, K <= G), lane k = entry k; float64 throughout.
+// A group of G lanes (16 or 64, K <= G), lane k = entry k; float64 throughout.
+//
+// With d_k = (s_k - m) / tau, S = sum of exp((s - m) / tau) over all classes and S_r over those outside the entries, so that
+// log q_k = d_k - log S and log q_rest = log S_r - log S:
+//   loss = sum p_k (log p_k - d_k) + p_rest (log(p_rest / S_r)) + (sum p_k + p_rest) log S
+// and without the rest, log p_k = z_k / tau - top - log E, E = sum of exp(z / tau - top), sum p_k = 1:
+//   loss = sum p_k (z_k / tau - top - d_k) + log(S / E).
+struct Teacher {        // what the teacher's entries alone make of a row
+    double p, log_p;    // of the lane's entry; without the rest log_p lacks - log E
+    double mass;        // sum of the p_k
+    double rest;        // p_rest, or 1 / E without the rest
+    bool any;           // there is some probability (always with the log normaliser)
+};
+template <int G>
+__device__ __forceinline__ Teacher teacher_of(bool there, float z, bool has_lse, float lse, double inv_t) {
+    Teacher o;
+    o.any = true;
+    if (has_lse) {
+        o.log_p = there ? fma((double)z, inv_t, -(double)lse) : -INFINITY;
+        o.p = exp64(o.log_p);
+        o.mass = group_sum<G>(o.p);
+        o.rest = o.mass >= 1.0 ? 0.0 : 1.0 - o.mass;
+    } else {
+        const float top = group_max<G>(there ? z : -INFINITY);
+        o.any = top != -INFINITY || group_ballot<G>(there && z != z) != 0;
+        o.log_p = there ? ((double)z - top) * inv_t : -INFINITY;
+        const double e = exp64(o.log_p);
+        o.rest = rcp64(group_sum<G>(e));
+        o.p = e * o.rest;
+        o.mass = 1.0;
+    }
+    return o;
+}
+
+// The row: the entries' logits s_k and, of the classes outside the entries, a base m_r and sum_r = sum of
+// exp((s - m_r) / tau).  m_r -infinity: nothing finite there.
 struct RowResult {
     double loss;        // without weight and tau^2
     double coef;        // gradient of a class outside the entries = coef * exp((s - m_r) / tau)
@@ -413,8 +676,8 @@ struct RowResult {
     bool first;         // the lane's entry is there and no lower lane names its class
 };
 template <int G>
-__device__ RowResult row_result(int K, bool there, bool again, int idx, float z, float s_k, bool has_lse, float t_lse, double inv_t, float m_r,
-                                double sum_r, int V) {
+__device__ __forceinline__ RowResult row_result(const Teacher& t, int K, bool there, bool again, int idx, float s_k, bool has_lse, double inv_t, float m_r,
+                                                double sum_r, int V) {
     RowResult out;
     const int lane = threadIdx.x & (G - 1);
     bool first = there;
@@ -424,50 +687,40 @@ __device__ RowResult row_result(int K, bool there, bool again, int idx, float z,
             const int other = __shfl(there ? idx : -1, j, G);
             if (j < lane && there && other == idx) first = false;
         }
-    const float m_i = group_max<G>(first ? s_k : -INFINITY);
-    const float m = fmaxf(m_r, m_i);
-    const double d_k = ((double)s_k - m) * inv_t;
-    const double e_k = first ? exp(d_k) : 0.0;
-    const double shift = m_r == -INFINITY ? 0.0 : exp(((double)m_r - m) * inv_t);
-    const double total = group_sum<G>(e_k) + sum_r * shift;
-    const double log_total = log(total);
-    const double log_q = d_k - log_total;
-    const double zt = there ? (double)z * inv_t : -INFINITY;
-    double log_p, p, rest = 0.0;
-    bool teacher = true;
+    const float m = fmaxf(m_r, group_max<G>(first ? s_k : -INFINITY));
+    const double d_k = ((double)s_k - m) * inv_t, d_r = ((double)m_r - m) * inv_t;
+    const double e_k = first ? exp64(d_k) : 0.0;
+    double shift = m_r == -INFINITY ? 0.0 : 1.0;
+    if (m_r != m && m_r != -INFINITY) shift = exp64(d_r);
+    const double total = group_sum<G>(e_k) + sum_r * shift, inv_total = rcp64(total);
+    double loss = group_sum<G>(t.p == 0.0 ? 0.0 : t.p * (t.log_p - d_k));
+    double coef = shift * inv_total;
     if (has_lse) {
-        log_p = zt - t_lse;
-        p = exp(log_p);
-        const double sum_p = group_sum<G>(p);
-        rest = sum_p >= 1.0 ? 0.0 : 1.0 - sum_p;
-        if (__popcll(group_ballot<G>(first)) == V) rest = 0.0;
+        const bool rest = t.rest != 0.0 && __popcll(group_ballot<G>(first)) != V;
+        loss += (t.mass + (rest ? t.rest : 0.0)) * log64(total);
+        if (rest && m_r == -INFINITY)
+            loss = INFINITY;
+        else if (rest) {
+            const double ratio = t.rest * rcp64(sum_r);
+            loss += t.rest * (log64(ratio) - d_r);
+            coef -= ratio;
+        }
     } else {
-        const double top = group_max<G>(zt);
-        teacher = top != -INFINITY || group_ballot<G>(zt != zt) != 0;
-        const double e = exp(zt - top), sum_e = group_sum<G>(e);
-        p = e / sum_e;
-        log_p = zt - top - log(sum_e);
+        loss += log64(total * t.rest);
     }
-    double loss = group_sum<G>(p == 0.0 ? 0.0 : p * (log_p - log_q));
-    double coef = m_r == -INFINITY ? 0.0 : shift / total;
-    if (has_lse && rest != 0.0) {
-        const double log_rest = m_r == -INFINITY ? -INFINITY : log(sum_r) + ((double)m_r - m) * inv_t;
-        loss += rest * (log(rest) - (log_rest - log_total));
-        if (m_r != -INFINITY) coef -= rest / sum_r;
-    }
-    double sum_same = p;
+    double sum_same = t.p;
     if (doubled) {
         sum_same = 0.0;
         for (int j = 0; j < K; ++j) {
             const int other = __shfl(there ? idx : -1, j, G);
-            const double pj = __shfl(p, j, G);
+            const double pj = __shfl(t.p, j, G);
             if (there && other == idx) sum_same += pj;
         }
     }
     out.first = first;
-    out.loss = teacher ? loss : 0.0;
-    out.coef = !teacher ? 0.0 : loss != loss ? loss : coef;
-    out.grad_k = !teacher ? 0.0 : loss != loss ? loss : exp(log_q) - sum_same;
+    out.loss = t.any ? loss : 0.0;
+    out.coef = !t.any ? 0.0 : loss != loss ? loss : coef;
+    out.grad_k = !t.any ? 0.0 : loss != loss ? loss : e_k * inv_total - sum_same;
     return out;
 }
 
@@ -489,15 +742,11 @@ struct RowPieces {
     static constexpr int P = kPiece<T>;
     float v[N][P];
     __device__ __forceinline__ void load(const T* p, int part, int V) {
-        const int pieces = (V + P - 1) / P;
+        uintx4 raw[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (part + i * LANES < pieces)
-                load_piece(p, part + i * LANES, V, v[i]);
-            else
+        for (int i = 0; i < N; ++i) raw[i] = load_raw(p, part + i * LANES, V);
 #pragma unroll
-                for (int e = 0; e < P; ++e) v[i][e] = -INFINITY;
-        }
+        for (int i = 0; i < N; ++i) unpack_piece(in_place(raw[i], p, part + i * LANES, V), v[i]);
     }
     // the classes that are entries (a bit each) leave the sums; returns the lane's maximum of the rest
     __device__ __forceinline__ float mask(const unsigned* member, int part, int V) {
@@ -593,8 +842,8 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs<T> a) {
         const float base = m_r == -INFINITY ? 0.0f : m_r;
         const float sum_r = group_sum<G>(row_v.exponentials(base, c));
         // no finite class outside the entries, but a NaN among them: the maximum does not see it, the sum does
-        const RowResult r = row_result<G>(a.K, there, again, idx, z, s_k, a.lse != nullptr, a.lse && live ? a.lse[row] : 0.0f, inv_t, sum_r != sum_r ? NAN : m_r,
-                                          (double)sum_r, a.V);
+        const Teacher t = teacher_of<G>(there, z, a.lse != nullptr, a.lse && live ? a.lse[row] : 0.0f, inv_t);
+        const RowResult r = row_result<G>(t, a.K, there, again, idx, s_k, a.lse != nullptr, inv_t, sum_r != sum_r ? NAN : m_r, (double)sum_r, a.V);
         const double scale = (double)w * a.t;
         if (a.loss && in_range && part == 0) a.loss[row] = live ? (float)(r.loss * scale * a.t) : 0.0f;
         if (a.grad && in_range) {
@@ -611,69 +860,133 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs<T> a) {
     }
 }
 
-// A workgroup of 4 waves per row of up to 8192 classes, the row in registers.
-constexpr int kBlockClasses = 8192;
-template <class T>
-__global__ __launch_bounds__(256) void distill_block_kernel(DistillArgs<T> a) {
-    extern __shared__ unsigned dynamic_lds[];             // a bit per class, then (for the gradient) a float per class
-    __shared__ float wave_part[4];
+// A row in LDS, W waves on it: read from memory once.  The first wave has the entries, and does the teacher's part while
+// the row is on its way.  The entries' places hold -infinity during the sum, so that nothing has to be tested per class;
+// every wave turns its own pieces into gradients in place, puts the entries' gradients among them and stores whole pieces.
+template <class T, int W>
+__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(kDistillOccupancy))) void distill_lds_kernel(DistillArgs<T> a) {
+    constexpr int P = kPiece<T>, THREADS = W * 64;
+    typedef T __attribute__((may_alias)) slot_t;
+    typedef __attribute__((may_alias)) typename std::conditional<sizeof(T) == 4, unsigned, uint16_t>::type mark_t;
+    extern __shared__ uintx4 buf[];
+    __shared__ float wave_top[W], wave_part[W], entry_grad[64];
+    __shared__ int entry_class[64];
     __shared__ float shared_coef;
-    const int words = (a.V + 31) / 32;
-    unsigned* member = dynamic_lds;
-    float* inside = reinterpret_cast<float*>(dynamic_lds + words);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
+    slot_t* slots = reinterpret_cast<slot_t*>(buf);
+    mark_t* marks = reinterpret_cast<mark_t*>(buf);
+    const double inv_t = 1.0 / a.t;
     const float c = kLog2e / a.t;
-    RowPieces<T, 256, kBlockClasses / 256 / kPiece<T>> row_v;
+    auto over_waves = [&](float* part, float v, bool sum) {            // sum or maximum of the waves' values, in their order
+        if (W == 1) return v;
+        if (lane == 0) part[wave] = v;
+        __syncthreads();
+        float o = part[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) o = sum ? o + part[i] : fmaxf(o, part[i]);
+        return o;
+    };
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* p = a.x + row * a.ld;
         T* g = a.grad ? a.grad + row * a.ld_grad : nullptr;
         const float w = a.weight ? a.weight[row] : 1.0f;
         if (w == 0.0f) {
             if (tid == 0 && a.loss) a.loss[row] = 0.0f;
-            if (g) row_v.store_zeros(g, tid, a.V);
+            float zeros[P] = {};
+            if (g)
+                for (int q = tid; q < pieces; q += THREADS) store_piece(g, q, a.V, zeros);
             continue;
         }
-        row_v.load(p, tid, a.V);
         int idx = -1;
-        float z = 0.0f, s_k = -INFINITY;
+        float z = 0.0f;
         if (wave == 0 && lane < a.K) {
             idx = a.index[row * a.K + lane];
             z = a.values[row * a.K + lane];
         }
-        for (int i = tid; i < words; i += 256) member[i] = 0;
-        __syncthreads();
+        const float lse = a.lse ? a.lse[row] : 0.0f;
         const bool there = idx >= 0 && idx < a.V;
+        Teacher t;
+        const float own_top = row_to_lds<THREADS>(a.x + row * a.ld, a.V, buf, [&] {
+            if (wave == 0) t = teacher_of<64>(there, z, a.lse != nullptr, lse, inv_t);
+        });
+        float m_r = over_waves(wave_top, group_max<64>(own_top), false);
+        if (W == 1) lds_phase();
+        float s_k = -INFINITY;
         bool again = false;
-        if (there) {
-            s_k = load_f32(p + idx);
-            again = atomicOr(&member[idx >> 5], 1u << (idx & 31)) >> (idx & 31) & 1;
-        }
-        __syncthreads();
-        float m_r = group_max<64>(row_v.mask(member, tid, a.V));
-        if (lane == 0) wave_part[wave] = m_r;
-        __syncthreads();
-        m_r = fmaxf(fmaxf(wave_part[0], wave_part[1]), fmaxf(wave_part[2], wave_part[3]));
-        const float base = m_r == -INFINITY ? 0.0f : m_r;
-        const float part = group_sum<64>(row_v.exponentials(base, c));
-        __syncthreads();
-        if (lane == 0) wave_part[wave] = part;
-        __syncthreads();
         if (wave == 0) {
-            const double sum_r = (double)wave_part[0] + wave_part[1] + wave_part[2] + wave_part[3], scale = (double)w * a.t;
-            const RowResult r = row_result<64>(a.K, there, again, idx, z, s_k, a.lse != nullptr, a.lse ? a.lse[row] : 0.0f, 1.0 / a.t, sum_r != sum_r ? NAN : m_r, sum_r, a.V);
+            // the entries' logits; which of them name a class that another lane names: all but the one whose mark stays
+            if (there) s_k = load_f32(reinterpret_cast<const T*>(slots + idx));
+            lds_phase();
+            if (there) marks[idx] = (mark_t)lane;
+            lds_phase();
+            again = there && (int)marks[idx] != lane;
+            lds_phase();
+            if (there) marks[idx] = sizeof(T) == 4 ? (mark_t)0xFF800000u : (mark_t)0xFF80u;
+            lds_phase();
+        }
+        if (W > 1) __syncthreads();
+        auto sum_of = [&](float base) {
+            float sum = 0.0f;
+            for (int q = tid; q < pieces; q += THREADS) {
+                float v[P];
+                unpack_piece(buf[q], v);
+#pragma unroll
+                for (int e = 0; e < P; ++e) sum += __builtin_amdgcn_exp2f((v[e] - base) * c);
+            }
+            return over_waves(wave_part, group_sum<64>(sum), true);
+        };
+        float base = m_r == -INFINITY ? 0.0f : m_r;
+        float sum_r = sum_of(base);
+        if (sum_r < 1e-20f) {               // far below the entries: from their own maximum
+            m_r = -INFINITY;
+            for (int q = tid; q < pieces; q += THREADS) {
+                float v[P];
+                unpack_piece(buf[q], v);
+#pragma unroll
+                for (int e = 0; e < P; ++e) m_r = fmaxf(m_r, v[e]);
+            }
+            m_r = over_waves(wave_top, group_max<64>(m_r), false);
+            base = m_r == -INFINITY ? 0.0f : m_r;
+            sum_r = sum_of(base);
+        }
+        if (wave == 0) {
+            // a NaN outside the entries: the maximum does not see it, the sum does
+            const RowResult r = row_result<64>(t, a.K, there, again, idx, s_k, a.lse != nullptr, inv_t, sum_r != sum_r ? NAN : m_r, (double)sum_r, a.V);
+            const double scale = (double)w * a.t;
             if (lane == 0) {
                 if (a.loss) a.loss[row] = (float)(r.loss * scale * a.t);
                 shared_coef = (float)(r.coef * scale);
             }
-            if (g && r.first) inside[idx] = (float)(r.grad_k * scale);
+            entry_class[lane] = r.first ? idx : -1;
+            entry_grad[lane] = (float)(r.grad_k * scale);
         }
-        if (!g) {
-            __syncthreads();
-            continue;
+        if (W > 1) __syncthreads();
+        if (W == 1) lds_phase();
+        if (g) {
+            const float coef = shared_coef;
+            for (int q = tid; q < pieces; q += THREADS) {
+                float v[P];
+                unpack_piece(buf[q], v);
+#pragma unroll
+                for (int e = 0; e < P; ++e) v[e] = coef != 0.0f ? coef * __builtin_amdgcn_exp2f((v[e] - base) * c) : 0.0f;
+                buf[q] = pack_piece(v);
+            }
+            lds_phase();
+            const int mine = entry_class[lane];
+            if (mine >= 0 && mine / P % THREADS / 64 == wave) store_f32(reinterpret_cast<T*>(slots + mine), entry_grad[lane]);
+            lds_phase();
+            for (int q = tid; q < pieces; q += THREADS) {
+                const uintx4 t4 = buf[q];
+                if ((q + 1) * P <= a.V) {
+                    *reinterpret_cast<uintx4_any*>(g + q * P) = t4;
+                } else {
+                    float v[P];
+                    unpack_piece(t4, v);
+                    store_piece(g, q, a.V, v);
+                }
+            }
         }
-        __syncthreads();
-        row_v.store(g, tid, a.V, member, inside, shared_coef);
-        __syncthreads();
+        if (W > 1) __syncthreads();
+        if (W == 1) lds_phase();
     }
 }
 
@@ -716,15 +1029,12 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
         __syncthreads();
         float m_own = -INFINITY, s_own = 0.0f;
         for (int q = tid; q < pieces; q += THREADS * AHEAD) {
+            uintx4 raw[AHEAD];
             float v[AHEAD][P];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                if (q + i * THREADS < pieces)
-                    load_piece(p, q + i * THREADS, a.V, v[i]);
-                else
+            for (int i = 0; i < AHEAD; ++i) raw[i] = load_raw(p, q + i * THREADS, a.V);
 #pragma unroll
-                    for (int e = 0; e < P; ++e) v[i][e] = -INFINITY;
-            }
+            for (int i = 0; i < AHEAD; ++i) unpack_piece(in_place(raw[i], p, q + i * THREADS, a.V), v[i]);
             float m = m_own;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
@@ -758,7 +1068,9 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
             double sum_r = 0.0;
             for (int i = 0; i < WAVES; ++i) sum_r += (double)wave_part[i];
             const double scale = (double)w * a.t;
-            const RowResult r = row_result<64>(a.K, there, again, idx, z, s_k, a.lse != nullptr, a.lse ? a.lse[row] : 0.0f, 1.0 / a.t, sum_r != sum_r ? NAN : m_r, sum_r, a.V);
+            const double inv_t = 1.0 / a.t;
+            const Teacher t = teacher_of<64>(there, z, a.lse != nullptr, a.lse ? a.lse[row] : 0.0f, inv_t);
+            const RowResult r = row_result<64>(t, a.K, there, again, idx, s_k, a.lse != nullptr, inv_t, sum_r != sum_r ? NAN : m_r, sum_r, a.V);
             if (lane == 0) {
                 if (a.loss) a.loss[row] = (float)(r.loss * scale * a.t);
                 shared_coef = (float)(r.coef * scale);
@@ -770,7 +1082,7 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
             const float coef = shared_coef;
             for (int q = tid; q < pieces; q += THREADS) {
                 float v[P];
-                load_piece(p, q, a.V, v);
+                unpack_piece(in_place(load_raw(p, q, a.V), p, q, a.V), v);
 #pragma unroll
                 for (int e = 0; e < P; ++e) v[e] = coef != 0.0f ? coef * __builtin_amdgcn_exp2f((v[e] - base) * c) : 0.0f;
                 const unsigned bits = member[q * P >> 5] >> (q * P & 31) & ((1u << P) - 1);
@@ -795,26 +1107,29 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
     constexpr int P = kPiece<T>;
     if (a.V <= 128 && a.K <= 16)
         hipLaunchKernelGGL(top16_kernel<T>, dim3((unsigned)std::min((a.rows + 15) / 16, kMaxGrid)), dim3(256), 0, s, a);
-    else if (a.V <= 1024)
-        hipLaunchKernelGGL((top_kernel<T, 1, 1024 / 64 / P>), dim3(grid), dim3(64), 0, s, a);
-    else if (a.V <= kBlockClasses)
-        hipLaunchKernelGGL((top_kernel<T, 4, kBlockClasses / 256 / P>), dim3(grid), dim3(256), 0, s, a);
+    else if (a.V <= kWaveClasses)
+        hipLaunchKernelGGL(top_wave_kernel<T>, dim3(grid), dim3(64), (size_t)(a.V + P - 1) / P * 16, s, a);
+    else if (a.V <= 4096)
+        hipLaunchKernelGGL((top_block_kernel<T, 4096 / 256 / P>), dim3(grid), dim3(256), 0, s, a);
+    else if (a.V <= 8192)
+        hipLaunchKernelGGL((top_block_kernel<T, 8192 / 256 / P>), dim3(grid), dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((top_kernel<T, 8, 0>), dim3(grid), dim3(512), 0, s, a);
+        hipLaunchKernelGGL(top_stream_kernel<T>, dim3(grid), dim3(512), 0, s, a);
     OCR_HIP_CHECK(hipGetLastError());
     return OCRHIP_OK;
 }
 
 template <class T>
 int launch_distill(const DistillArgs<T>& a, hipStream_t s) {
-    const size_t bits = (size_t)(a.V + 31) / 32 * 4;
+    constexpr int P = kPiece<T>;
+    const size_t bits = (size_t)(a.V + 31) / 32 * 4, row_lds = (size_t)(a.V + P - 1) / P * 16;
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
     if (a.V <= 128 && a.K <= 16)
         hipLaunchKernelGGL((distill_group_kernel<T, 16, 128>), dim3((unsigned)std::min((a.rows + 15) / 16, kMaxGrid)), dim3(256), 0, s, a);
-    else if (a.V <= 1024)
-        hipLaunchKernelGGL((distill_group_kernel<T, 64, 1024>), dim3((unsigned)std::min((a.rows + 3) / 4, kMaxGrid)), dim3(256), 0, s, a);
-    else if (a.V <= kBlockClasses)
-        hipLaunchKernelGGL(distill_block_kernel<T>, dim3(grid), dim3(256), bits + (a.grad ? (size_t)a.V * 4 : 0), s, a);
+    else if (row_lds <= kWaveBytes)
+        hipLaunchKernelGGL((distill_lds_kernel<T, 1>), dim3(grid), dim3(64), row_lds, s, a);
+    else if (row_lds <= kRowBytes)
+        hipLaunchKernelGGL((distill_lds_kernel<T, 4>), dim3(grid), dim3(256), row_lds, s, a);
     else
         hipLaunchKernelGGL(distill_stream_kernel<T>, dim3(grid), dim3(512), bits, s, a);
     OCR_HIP_CHECK(hipGetLastError());
