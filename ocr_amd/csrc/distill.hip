@@ -132,16 +132,18 @@ __device__ __forceinline__ uintx4 pack_piece(const float (&v)[4]) {
 __device__ __forceinline__ uintx4 pack_piece(const float (&v)[8]) {
     return __builtin_bit_cast(uintx4, bf16x8{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3], (__bf16)v[4], (__bf16)v[5], (__bf16)v[6], (__bf16)v[7]});
 }
-template <class T>
+// TINY: rows shorter than a piece, element by element.
+template <bool TINY, class T>
 __device__ __forceinline__ uintx4 load_raw(const T* p, int q, int V) {
     constexpr int P = kPiece<T>;
-    if (V < P) {                                    // uniform
+    if constexpr (TINY) {
         float v[P];
 #pragma unroll
-        for (int e = 0; e < P; ++e) v[e] = e < V ? load_f32(p + e) : 0.0f;
+        for (int e = 0; e < P; ++e) v[e] = load_f32(p + min(e, V - 1));
         return pack_piece(v);
+    } else {
+        return *reinterpret_cast<const uintx4_any*>(p + min(q * P, V - P));
     }
-    return *reinterpret_cast<const uintx4_any*>(p + min(q * P, V - P));
 }
 // t without its first 1, 2 or 4 classes, -infinity behind
 template <int D>
@@ -154,17 +156,17 @@ __device__ __forceinline__ uintx4 drop(uintx4 t, const uint16_t*) {
     if (D == 1) return uintx4{t[0] >> 16 | t[1] << 16, t[1] >> 16 | t[2] << 16, t[2] >> 16 | t[3] << 16, t[3] >> 16 | 0xFF800000u};
     return D == 2 ? uintx4{t[1], t[2], t[3], kNone} : uintx4{t[2], t[3], kNone, kNone};
 }
-template <class T>
+template <bool TINY, class T>
 __device__ __forceinline__ uintx4 in_place(uintx4 t, const T* p, int q, int V) {
     constexpr int P = kPiece<T>;
-    if ((q + 1) * P > V) {
-        if (V < P) {
-            float v[P];
-            unpack_piece(t, v);
+    if constexpr (TINY) {
+        float v[P];
+        unpack_piece(t, v);
 #pragma unroll
-            for (int e = 0; e < P; ++e) v[e] = q == 0 && e < V ? v[e] : -INFINITY;
-            return pack_piece(v);
-        }
+        for (int e = 0; e < P; ++e) v[e] = q == 0 && e < V ? v[e] : -INFINITY;
+        return pack_piece(v);
+    }
+    if ((q + 1) * P > V) {
         const int d = q * P - (V - P);
         if (d & 1) t = drop<1>(t, p);
         if (d & 2) t = drop<2>(t, p);
@@ -268,7 +270,7 @@ struct TopArgs {
     float* lse;
 };
 
-template <class T>
+template <class T, bool TINY>
 __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
     constexpr int P = kPiece<T>, N = 128 / 16 / P;
     const int part = threadIdx.x & 15;
@@ -279,9 +281,9 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
         unsigned key[N][P];
         unsigned best = 0, at = 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = 0; i < N; ++i) raw[i] = load_raw(p, part + 16 * i, a.V);
+        for (int i = 0; i < N; ++i) raw[i] = load_raw<TINY>(p, part + 16 * i, a.V);
 #pragma unroll
-        for (int i = 0; i < N; ++i) unpack_piece(in_place(raw[i], p, part + 16 * i, a.V), v[i]);
+        for (int i = 0; i < N; ++i) unpack_piece(in_place<TINY>(raw[i], p, part + 16 * i, a.V), v[i]);
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -328,10 +330,6 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
 // Rows of up to kWaveClasses classes: in LDS, one wave's own, so nothing waits for another.
 constexpr int kWaveClasses = 2048;
 constexpr size_t kWaveBytes = 16384, kRowBytes = 32768;
-#ifndef KOCC
-#define KOCC 3
-#endif
-constexpr int kDistillOccupancy = KOCC;
 constexpr int kTopList = 512;          // candidates of a row that LDS holds
 
 // what one lane wrote to LDS is what another reads: same wave, so the order of the instructions is enough
@@ -340,24 +338,24 @@ __device__ __forceinline__ void lds_phase() {
     __builtin_amdgcn_wave_barrier();
 }
 
-constexpr int kBatch = 8;              // pieces a lane has in flight
-
-// the row to LDS (pieces of 16 bytes; classes behind the last are -infinity); returns the lane's maximum.  `between` runs
+constexpr int kShort = 128;            // classes of a row that 16 lanes share
+// The row to LDS, BATCH pieces of a lane in flight (pieces of 16 bytes; classes behind the last are -infinity); returns the lane's maximum.  `between` runs
 // while the first pieces are on their way.
-template <int THREADS, class T, class F>
+template <int THREADS, int BATCH, bool TINY, class T, class F>
 __device__ __forceinline__ float row_to_lds(const T* p, int V, uintx4* buf, F between) {
     constexpr int P = kPiece<T>;
     const int pieces = (V + P - 1) / P, tid = threadIdx.x;
     float m = -INFINITY;
-    for (int q = tid; q - tid < pieces; q += THREADS * kBatch) {
-        uintx4 t[kBatch];
+    for (int q = tid; q - tid < pieces; q += THREADS * BATCH) {
+        uintx4 t[BATCH];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) t[i] = load_raw(p, q + i * THREADS, V);
+        for (int i = 0; i < BATCH; ++i)
+            t[i] = load_raw<TINY>(p, q + i * THREADS, V);
         if (q == tid) between();
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
+        for (int i = 0; i < BATCH; ++i)
             if (q + i * THREADS < pieces) {
-                const uintx4 u = in_place(t[i], p, q + i * THREADS, V);
+                const uintx4 u = in_place<TINY>(t[i], p, q + i * THREADS, V);
                 float v[P];
                 unpack_piece(u, v);
 #pragma unroll
@@ -433,7 +431,7 @@ __global__ __launch_bounds__(64) void top_wave_kernel(TopArgs<T> a) {
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* p = a.x + row * a.ld;
         if (lane == 0) count = 0;
-        const float mine = row_to_lds<64>(p, a.V, buf, [] {});
+        const float mine = row_to_lds<64, 8, false>(p, a.V, buf, [] {});
         lds_phase();
         const unsigned key = lane < pieces ? order_key(mine) : 0u;
         const unsigned bits = bisect(&key, 1, a.K);
@@ -491,9 +489,9 @@ __global__ __launch_bounds__(256) void top_block_kernel(TopArgs<T> a) {
         uintx4 raw[N];
         float v[N][P], mine = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < N; ++i) raw[i] = load_raw(p, tid + i * 256, a.V);
+        for (int i = 0; i < N; ++i) raw[i] = load_raw<false>(p, tid + i * 256, a.V);
 #pragma unroll
-        for (int i = 0; i < N; ++i) unpack_piece(in_place(raw[i], p, tid + i * 256, a.V), v[i]);
+        for (int i = 0; i < N; ++i) unpack_piece(in_place<false>(raw[i], p, tid + i * 256, a.V), v[i]);
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -565,9 +563,9 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
             uintx4 raw[AHEAD];
             float w[AHEAD][P];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) raw[i] = load_raw(p, q + i * THREADS, a.V);
+            for (int i = 0; i < AHEAD; ++i) raw[i] = load_raw<false>(p, q + i * THREADS, a.V);
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) unpack_piece(in_place(raw[i], p, q + i * THREADS, a.V), w[i]);
+            for (int i = 0; i < AHEAD; ++i) unpack_piece(in_place<false>(raw[i], p, q + i * THREADS, a.V), w[i]);
             float m = m_own;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
@@ -604,7 +602,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
         if (!(m_own < bound) || s_own != s_own)
             for (int q = tid; q < pieces; q += THREADS) {
                 float v[P];
-                unpack_piece(in_place(load_raw(p, q, a.V), p, q, a.V), v);
+                unpack_piece(in_place<false>(load_raw<false>(p, q, a.V), p, q, a.V), v);
 #pragma unroll
                 for (int e = 0; e < P; ++e)
                     if (!(v[e] < bound) && q * P + e < a.V) {
@@ -736,145 +734,147 @@ struct DistillArgs {
     float t;
 };
 
-// A row in registers: pieces lane + i * LANES, i < N, of LANES lanes (or threads) share it.
-template <class T, int LANES, int N>
-struct RowPieces {
-    static constexpr int P = kPiece<T>;
-    float v[N][P];
-    __device__ __forceinline__ void load(const T* p, int part, int V) {
-        uintx4 raw[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) raw[i] = load_raw(p, part + i * LANES, V);
-#pragma unroll
-        for (int i = 0; i < N; ++i) unpack_piece(in_place(raw[i], p, part + i * LANES, V), v[i]);
-    }
-    // the classes that are entries (a bit each) leave the sums; returns the lane's maximum of the rest
-    __device__ __forceinline__ float mask(const unsigned* member, int part, int V) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = (part + i * LANES) * P;
-            const unsigned bits = at < V ? member[at >> 5] >> (at & 31) : 0u;
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                v[i][e] = bits >> e & 1 ? -INFINITY : v[i][e];
-                m = fmaxf(m, v[i][e]);
-            }
-        }
-        return m;
-    }
-    // v = exp((v - base) / tau), c = log2 e / tau; returns the lane's sum
-    __device__ __forceinline__ float exponentials(float base, float c) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                v[i][e] = __builtin_amdgcn_exp2f((v[i][e] - base) * c);
-                sum += v[i][e];
-            }
-        }
-        return sum;
-    }
-    // gradient: coef * v outside the entries (0 for coef 0, whatever v is), the value of `inside` (by class) for them
-    __device__ __forceinline__ void store(T* g, int part, int V, const unsigned* member, const float* inside, float coef) {
-        const int pieces = (V + P - 1) / P;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (part + i * LANES >= pieces) break;
-            const int at = (part + i * LANES) * P;
-            const unsigned bits = member[at >> 5] >> (at & 31) & ((1u << P) - 1);
-            float o[P];
-#pragma unroll
-            for (int e = 0; e < P; ++e) o[e] = coef != 0.0f ? coef * v[i][e] : 0.0f;
-            if (bits)
-#pragma unroll
-                for (int e = 0; e < P; ++e)
-                    if (bits >> e & 1) o[e] = inside[at + e];
-            store_piece(g, part + i * LANES, V, o);
-        }
-    }
-    __device__ __forceinline__ void store_zeros(T* g, int part, int V) {
-        const int pieces = (V + P - 1) / P;
-        float o[P];
-#pragma unroll
-        for (int e = 0; e < P; ++e) o[e] = 0.0f;
-        for (int q = part; q < pieces; q += LANES) store_piece(g, q, V, o);
-    }
-};
+// What the entries do to a row in LDS, a group of lanes, lane k = entry k: returns its class's logit and leaves -infinity in
+// its place.  `again`: the lane's class is named by another lane too, whose mark stayed.
+template <class T>
+__device__ __forceinline__ float take_entry(void* row, bool there, int idx, int lane, bool& again) {
+    typedef T __attribute__((may_alias)) slot_t;
+    typedef __attribute__((may_alias)) typename std::conditional<sizeof(T) == 4, unsigned, uint16_t>::type mark_t;
+    mark_t* marks = reinterpret_cast<mark_t*>(row);
+    const float s_k = there ? load_f32(reinterpret_cast<const T*>(reinterpret_cast<slot_t*>(row) + idx)) : -INFINITY;
+    lds_phase();
+    if (there) marks[idx] = (mark_t)lane;
+    lds_phase();
+    again = there && (int)marks[idx] != lane;
+    lds_phase();
+    if (there) marks[idx] = sizeof(T) == 4 ? (mark_t)0xFF800000u : (mark_t)0xFF80u;
+    lds_phase();
+    return s_k;
+}
+template <class T>
+__device__ __forceinline__ void put_entry(void* row, int idx, float v) {
+    typedef T __attribute__((may_alias)) slot_t;
+    store_f32(reinterpret_cast<T*>(reinterpret_cast<slot_t*>(row) + idx), v);
+}
 
-// G lanes of one wave per row (rows of up to CAP classes): the row is read once and stays in registers, its entries' bits
-// and gradients are in LDS of the group's own, nothing waits for another wave.
-template <class T, int G, int CAP>
-__global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs<T> a) {
-    constexpr int ROWS = 256 / G, WORDS = CAP / 32;
-    __shared__ unsigned member_all[ROWS][WORDS];
-    __shared__ float inside_all[ROWS][CAP];
-    const int part = threadIdx.x & (G - 1), sub = threadIdx.x / G;
-    unsigned* member = member_all[sub];
-    float* inside = inside_all[sub];
+// Rows of up to 128 classes and 16 entries: 16 lanes per row, four rows a wave, in LDS of the group's own.  Such a row is 776
+// bytes and a few hundred float64 instructions, so the next row's loads (and the weight of the one after it, which says
+// whether to load it) are on their way while one is worked on.
+template <class T, bool TINY>
+__global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs<T> a) {
+    constexpr int G = 16, ROWS = 256 / G, P = kPiece<T>, N = kShort / G / P;
+    __shared__ uintx4 rows_lds[ROWS][N * G];
+    const int part = threadIdx.x & (G - 1), sub = threadIdx.x / G, pieces = (a.V + P - 1) / P;
+    uintx4* buf = rows_lds[sub];
     const double inv_t = 1.0 / a.t;
     const float c = kLog2e / a.t;
-    RowPieces<T, G, CAP / G / kPiece<T>> row_v;
-    for (int64_t first_row = (int64_t)blockIdx.x * ROWS; first_row < a.rows; first_row += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = first_row + sub;
-        const bool in_range = row < a.rows;
-        const float w = !in_range ? 0.0f : a.weight ? a.weight[row] : 1.0f;
-        const T* p = a.x + row * a.ld;
-        const bool live = w != 0.0f;               // the others of the wave may be: everything below runs for all lanes
-        if (live) row_v.load(p, part, a.V);
-        int idx = -1;
-        float z = 0.0f, s_k = -INFINITY;
-        if (live && part < a.K) {
-            idx = a.index[row * a.K + part];
-            z = a.values[row * a.K + part];
-        }
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    auto weight_of = [&](int64_t row) { return row >= a.rows ? 0.0f : a.weight ? a.weight[row] : 1.0f; };
+    uintx4 next[N];
+    int next_idx;
+    float next_z, next_lse = 0.0f;
+    auto fetch = [&](int64_t row, bool live) {                 // no branch: a row that is not wanted loads the first one
+        const int64_t r = live ? row : 0;
+        const T* p = a.x + r * a.ld;
+#pragma unroll
+        for (int i = 0; i < N; ++i) next[i] = load_raw<TINY>(p, part + i * G, a.V);
+        const int64_t k = r * a.K + min(part, a.K - 1);
+        next_idx = a.index[k];
+        next_z = a.values[k];
+        if (a.lse) next_lse = a.lse[r];
+    };
+    int64_t row = (int64_t)blockIdx.x * ROWS + sub;
+    float w_next = weight_of(row);
+    fetch(row, w_next != 0.0f);
+    float w_after = weight_of(row + step);
+    for (int64_t first_row = (int64_t)blockIdx.x * ROWS; first_row < a.rows; first_row += step, row += step) {
+        const float w = w_next;
+        const bool in_range = row < a.rows, live = w != 0.0f;  // lanes without a row run along
+        const int idx = live && part < a.K ? next_idx : -1;
+        const float z = next_z, lse = next_lse;
         const bool there = idx >= 0 && idx < a.V;
-        for (int i = part; i < WORDS; i += G) member[i] = 0;
-        __builtin_amdgcn_wave_barrier();
-        bool again = false;
-        if (there) {
-            s_k = load_f32(p + idx);
-            again = atomicOr(&member[idx >> 5], 1u << (idx & 31)) >> (idx & 31) & 1;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float v[P];
+            const uintx4 u = in_place<TINY>(next[i], a.x, part + i * G, a.V);
+            unpack_piece(u, v);
+#pragma unroll
+            for (int e = 0; e < P; ++e) top = fmaxf(top, v[e]);
+            buf[part + i * G] = u;
         }
-        __builtin_amdgcn_wave_barrier();
-        const float m_r = group_max<G>(row_v.mask(member, part, a.V));
-        const float base = m_r == -INFINITY ? 0.0f : m_r;
-        const float sum_r = group_sum<G>(row_v.exponentials(base, c));
-        // no finite class outside the entries, but a NaN among them: the maximum does not see it, the sum does
-        const Teacher t = teacher_of<G>(there, z, a.lse != nullptr, a.lse && live ? a.lse[row] : 0.0f, inv_t);
+        w_next = w_after;
+        fetch(row + step, w_next != 0.0f);
+        w_after = weight_of(row + 2 * step);
+        lds_phase();
+        bool again;
+        const float s_k = take_entry<T>(buf, there, idx, part, again);
+        float v[N][P], m_r = group_max<G>(top);
+        auto sum_of = [&](float base) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                unpack_piece(buf[part + i * G], v[i]);
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    v[i][e] = __builtin_amdgcn_exp2f((v[i][e] - base) * c);
+                    sum += v[i][e];
+                }
+            }
+            return group_sum<G>(sum);
+        };
+        float sum_r = sum_of(m_r == -INFINITY ? 0.0f : m_r);
+        if (__ballot(sum_r < 1e-20f)) {      // some row of the wave: far below its entries, so from its own maximum
+            float own = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float u[P];
+                unpack_piece(buf[part + i * G], u);
+#pragma unroll
+                for (int e = 0; e < P; ++e) own = fmaxf(own, u[e]);
+            }
+            own = group_max<G>(own);
+            m_r = sum_r < 1e-20f ? own : m_r;
+            sum_r = sum_of(m_r == -INFINITY ? 0.0f : m_r);
+        }
+        const Teacher t = teacher_of<G>(there, z, a.lse != nullptr, lse, inv_t);
+        // a NaN outside the entries: the maximum does not see it, the sum does
         const RowResult r = row_result<G>(t, a.K, there, again, idx, s_k, a.lse != nullptr, inv_t, sum_r != sum_r ? NAN : m_r, (double)sum_r, a.V);
         const double scale = (double)w * a.t;
         if (a.loss && in_range && part == 0) a.loss[row] = live ? (float)(r.loss * scale * a.t) : 0.0f;
-        if (a.grad && in_range) {
+        if (a.grad) {
+            const float coef = live ? (float)(r.coef * scale) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+#pragma unroll
+                for (int e = 0; e < P; ++e) v[i][e] = coef != 0.0f ? coef * v[i][e] : 0.0f;
+                buf[part + i * G] = pack_piece(v[i]);
+            }
+            lds_phase();
+            if (r.first) put_entry<T>(buf, idx, (float)(r.grad_k * scale));
+            lds_phase();
             T* g = a.grad + row * a.ld_grad;
-            if (live) {
-                if (r.first) inside[idx] = (float)(r.grad_k * scale);
-                __builtin_amdgcn_wave_barrier();
-                row_v.store(g, part, a.V, member, inside, (float)(r.coef * scale));
-            } else {
-                row_v.store_zeros(g, part, a.V);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                unpack_piece(buf[part + i * G], v[i]);
+                if (in_range && part + i * G < pieces) store_piece(g, part + i * G, a.V, v[i]);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        lds_phase();
     }
 }
 
 // A row in LDS, W waves on it: read from memory once.  The first wave has the entries, and does the teacher's part while
 // the row is on its way.  The entries' places hold -infinity during the sum, so that nothing has to be tested per class;
 // every wave turns its own pieces into gradients in place, puts the entries' gradients among them and stores whole pieces.
-template <class T, int W>
-__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(kDistillOccupancy))) void distill_lds_kernel(DistillArgs<T> a) {
+template <class T, int W, int BATCH, bool TINY>
+__global__ __launch_bounds__(W * 64) void distill_lds_kernel(DistillArgs<T> a) {
     constexpr int P = kPiece<T>, THREADS = W * 64;
-    typedef T __attribute__((may_alias)) slot_t;
-    typedef __attribute__((may_alias)) typename std::conditional<sizeof(T) == 4, unsigned, uint16_t>::type mark_t;
     extern __shared__ uintx4 buf[];
     __shared__ float wave_top[W], wave_part[W], entry_grad[64];
     __shared__ int entry_class[64];
     __shared__ float shared_coef;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
-    slot_t* slots = reinterpret_cast<slot_t*>(buf);
-    mark_t* marks = reinterpret_cast<mark_t*>(buf);
     const double inv_t = 1.0 / a.t;
     const float c = kLog2e / a.t;
     auto over_waves = [&](float* part, float v, bool sum) {            // sum or maximum of the waves' values, in their order
@@ -905,24 +905,14 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(kDistill
         const float lse = a.lse ? a.lse[row] : 0.0f;
         const bool there = idx >= 0 && idx < a.V;
         Teacher t;
-        const float own_top = row_to_lds<THREADS>(a.x + row * a.ld, a.V, buf, [&] {
+        const float own_top = row_to_lds<THREADS, BATCH, TINY>(a.x + row * a.ld, a.V, buf, [&] {
             if (wave == 0) t = teacher_of<64>(there, z, a.lse != nullptr, lse, inv_t);
         });
         float m_r = over_waves(wave_top, group_max<64>(own_top), false);
         if (W == 1) lds_phase();
         float s_k = -INFINITY;
         bool again = false;
-        if (wave == 0) {
-            // the entries' logits; which of them name a class that another lane names: all but the one whose mark stays
-            if (there) s_k = load_f32(reinterpret_cast<const T*>(slots + idx));
-            lds_phase();
-            if (there) marks[idx] = (mark_t)lane;
-            lds_phase();
-            again = there && (int)marks[idx] != lane;
-            lds_phase();
-            if (there) marks[idx] = sizeof(T) == 4 ? (mark_t)0xFF800000u : (mark_t)0xFF80u;
-            lds_phase();
-        }
+        if (wave == 0) s_k = take_entry<T>(buf, there, idx, lane, again);
         if (W > 1) __syncthreads();
         auto sum_of = [&](float base) {
             float sum = 0.0f;
@@ -972,7 +962,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(kDistill
             }
             lds_phase();
             const int mine = entry_class[lane];
-            if (mine >= 0 && mine / P % THREADS / 64 == wave) store_f32(reinterpret_cast<T*>(slots + mine), entry_grad[lane]);
+            if (mine >= 0 && mine / P % THREADS / 64 == wave) put_entry<T>(buf, mine, entry_grad[lane]);
             lds_phase();
             for (int q = tid; q < pieces; q += THREADS) {
                 const uintx4 t4 = buf[q];
@@ -1032,9 +1022,9 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
             uintx4 raw[AHEAD];
             float v[AHEAD][P];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) raw[i] = load_raw(p, q + i * THREADS, a.V);
+            for (int i = 0; i < AHEAD; ++i) raw[i] = load_raw<false>(p, q + i * THREADS, a.V);
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) unpack_piece(in_place(raw[i], p, q + i * THREADS, a.V), v[i]);
+            for (int i = 0; i < AHEAD; ++i) unpack_piece(in_place<false>(raw[i], p, q + i * THREADS, a.V), v[i]);
             float m = m_own;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
@@ -1082,7 +1072,7 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
             const float coef = shared_coef;
             for (int q = tid; q < pieces; q += THREADS) {
                 float v[P];
-                unpack_piece(in_place(load_raw(p, q, a.V), p, q, a.V), v);
+                unpack_piece(in_place<false>(load_raw<false>(p, q, a.V), p, q, a.V), v);
 #pragma unroll
                 for (int e = 0; e < P; ++e) v[e] = coef != 0.0f ? coef * __builtin_amdgcn_exp2f((v[e] - base) * c) : 0.0f;
                 const unsigned bits = member[q * P >> 5] >> (q * P & 31) & ((1u << P) - 1);
@@ -1105,8 +1095,11 @@ template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
     constexpr int P = kPiece<T>;
-    if (a.V <= 128 && a.K <= 16)
-        hipLaunchKernelGGL(top16_kernel<T>, dim3((unsigned)std::min((a.rows + 15) / 16, kMaxGrid)), dim3(256), 0, s, a);
+    const unsigned groups = (unsigned)std::min((a.rows + 15) / 16, kMaxGrid);
+    if (a.V < P)                       // K <= V
+        hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
+    else if (a.V <= kShort && a.K <= 16)
+        hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
     else if (a.V <= kWaveClasses)
         hipLaunchKernelGGL(top_wave_kernel<T>, dim3(grid), dim3(64), (size_t)(a.V + P - 1) / P * 16, s, a);
     else if (a.V <= 4096)
@@ -1124,12 +1117,21 @@ int launch_distill(const DistillArgs<T>& a, hipStream_t s) {
     constexpr int P = kPiece<T>;
     const size_t bits = (size_t)(a.V + 31) / 32 * 4, row_lds = (size_t)(a.V + P - 1) / P * 16;
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
-    if (a.V <= 128 && a.K <= 16)
-        hipLaunchKernelGGL((distill_group_kernel<T, 16, 128>), dim3((unsigned)std::min((a.rows + 15) / 16, kMaxGrid)), dim3(256), 0, s, a);
+    const unsigned groups = (unsigned)std::min<int64_t>((a.rows + 15) / 16, 2048);          // 8 per compute unit, which walk the rows
+    if (a.K <= 16 && a.V < P)
+        hipLaunchKernelGGL((distill_short_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
+    else if (a.K <= 16 && a.V <= kShort)
+        hipLaunchKernelGGL((distill_short_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
+    else if (a.V < P)
+        hipLaunchKernelGGL((distill_lds_kernel<T, 1, 1, true>), dim3(grid), dim3(64), row_lds, s, a);
+    else if (row_lds <= 2048)
+        hipLaunchKernelGGL((distill_lds_kernel<T, 1, 2, false>), dim3(grid), dim3(64), row_lds, s, a);
+    else if (row_lds <= 4096)
+        hipLaunchKernelGGL((distill_lds_kernel<T, 1, 4, false>), dim3(grid), dim3(64), row_lds, s, a);
     else if (row_lds <= kWaveBytes)
-        hipLaunchKernelGGL((distill_lds_kernel<T, 1>), dim3(grid), dim3(64), row_lds, s, a);
+        hipLaunchKernelGGL((distill_lds_kernel<T, 1, 8, false>), dim3(grid), dim3(64), row_lds, s, a);
     else if (row_lds <= kRowBytes)
-        hipLaunchKernelGGL((distill_lds_kernel<T, 4>), dim3(grid), dim3(256), row_lds, s, a);
+        hipLaunchKernelGGL((distill_lds_kernel<T, 4, 8, false>), dim3(grid), dim3(256), row_lds, s, a);
     else
         hipLaunchKernelGGL(distill_stream_kernel<T>, dim3(grid), dim3(512), bits, s, a);
     OCR_HIP_CHECK(hipGetLastError());
