@@ -1224,7 +1224,10 @@ namespace {
 struct DeviceScope {
     int before = -1;
     DeviceScope() { if (hipGetDevice(&before) != hipSuccess) before = -1; }
-    ~DeviceScope() { if (before >= 0) (void)hipSetDevice(before); }
+    ~DeviceScope() {
+        int now = before;
+        if (before >= 0 && hipGetDevice(&now) == hipSuccess && now != before) (void)hipSetDevice(before);
+    }
 };
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }

@@ -327,8 +327,8 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
     }
 }
 
-// Rows of up to kWaveClasses classes: in LDS, one wave's own, so nothing waits for another.
-constexpr int kWaveClasses = 2048;
+// Rows in LDS: up to kWaveBytes one wave's own, so that nothing waits for another; longer ones are shared by four waves, for
+// few fit a compute unit.
 constexpr size_t kWaveBytes = 16384, kRowBytes = 32768;
 constexpr int kTopList = 512;          // candidates of a row that LDS holds
 
@@ -419,27 +419,41 @@ __device__ __forceinline__ void write_one_by_one(const TopArgs<T>& a, int64_t ro
     }
 }
 
-// One wave per row.
-template <class T>
-__global__ __launch_bounds__(64) void top_wave_kernel(TopArgs<T> a) {
-    constexpr int P = kPiece<T>;
+// A row in LDS, W waves on it.  The bound: every wave bisects its own 64 maxima for the ceil(K / W)-th largest, the least
+// of those is reached by at least K values.
+template <class T, int W, int BATCH>
+__global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
+    constexpr int P = kPiece<T>, THREADS = W * 64;
     extern __shared__ uintx4 buf[];                        // the row
-    __shared__ unsigned long long list[kTopList], wave_best;
+    __shared__ unsigned long long list[kTopList], wave_best[W];
+    __shared__ unsigned wave_bits[W];
+    __shared__ float wave_top[W], wave_sum[W];
     __shared__ int count;
-    const int lane = threadIdx.x, pieces = (a.V + P - 1) / P;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
     const float c = a.inv_t * kLog2e;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* p = a.x + row * a.ld;
-        if (lane == 0) count = 0;
-        const float mine = row_to_lds<64, 8, false>(p, a.V, buf, [] {});
+        if (tid == 0) count = 0;
+        const float mine = row_to_lds<THREADS, BATCH, false>(a.x + row * a.ld, a.V, buf, [] {});
+        const unsigned key = tid < pieces ? order_key(mine) : 0u;
+        unsigned least = bisect(&key, 1, (a.K + W - 1) / W);
+        float high = group_max<64>(mine);                  // NaN apart
+        if (W > 1) {
+            if (lane == 0) {
+                wave_bits[wave] = least;
+                wave_top[wave] = high;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                least = min(least, wave_bits[i]);
+                high = fmaxf(high, wave_top[i]);
+            }
+        }
         lds_phase();
-        const unsigned key = lane < pieces ? order_key(mine) : 0u;
-        const unsigned bits = bisect(&key, 1, a.K);
-        const float bound = bits ? key_value(bits) : -INFINITY;
-        const float high = group_max<64>(mine);            // NaN apart
+        const float bound = least ? key_value(least) : -INFINITY;
         const float base = fabsf(high) == INFINITY ? 0.0f : high;
         float sum = 0.0f;
-        for (int q = lane; q < pieces; q += 64) {
+        for (int q = tid; q < pieces; q += THREADS) {      // its own pieces
             float v[P];
             unpack_piece(buf[q], v);
             bool any = false;
@@ -456,86 +470,19 @@ __global__ __launch_bounds__(64) void top_wave_kernel(TopArgs<T> a) {
                         if (slot < kTopList) list[slot] = (unsigned long long)order_key(v[e]) << 32 | (0xFFFFFFFFu - (unsigned)(q * P + e));
                     }
         }
-        lds_phase();
-        const int n = count;
-        if (n <= kTopList) {
-            write_ranked(a, row, list, n, lane, 64);
-        } else {
-            write_one_by_one<1>(a, row, &wave_best);
-        }
-        if (a.lse) {
-            sum = group_sum<64>(sum);
-            if (lane == 0) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)sum));
-        }
-        lds_phase();
-    }
-}
-
-// A workgroup of 4 waves per row, N pieces a thread in registers.  The bound: every wave bisects its own 64 maxima for the
-// ceil(K / 4)-th largest, the least of the four is reached by at least K values.
-template <class T, int N>
-__global__ __launch_bounds__(256) void top_block_kernel(TopArgs<T> a) {
-    constexpr int P = kPiece<T>;
-    __shared__ unsigned long long list[kTopList];
-    __shared__ unsigned wave_bits[4];
-    __shared__ float wave_high[4], wave_sum[4];
-    __shared__ unsigned long long wave_best[4];
-    __shared__ int count;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
-    const float c = a.inv_t * kLog2e;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* p = a.x + row * a.ld;
-        if (tid == 0) count = 0;
-        uintx4 raw[N];
-        float v[N][P], mine = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < N; ++i) raw[i] = load_raw<false>(p, tid + i * 256, a.V);
-#pragma unroll
-        for (int i = 0; i < N; ++i) unpack_piece(in_place<false>(raw[i], p, tid + i * 256, a.V), v[i]);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int e = 0; e < P; ++e) mine = fmaxf(mine, v[i][e]);
-        const unsigned key = tid < pieces ? order_key(mine) : 0u;
-        const unsigned bits = bisect(&key, 1, (a.K + 3) / 4);
-        const float wave_top = group_max<64>(mine);            // NaN apart
-        if (lane == 0) {
-            wave_bits[wave] = bits;
-            wave_high[wave] = wave_top;
-        }
-        __syncthreads();
-        const unsigned least = min(min(wave_bits[0], wave_bits[1]), min(wave_bits[2], wave_bits[3]));
-        const float bound = least ? key_value(least) : -INFINITY;
-        const float high = fmaxf(fmaxf(wave_high[0], wave_high[1]), fmaxf(wave_high[2], wave_high[3]));
-        const float base = fabsf(high) == INFINITY ? 0.0f : high;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                any |= !(v[i][e] < bound);                     // a NaN as well
-                sum += __builtin_amdgcn_exp2f((v[i][e] - base) * c);
-            }
-            if (any)
-#pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    const int at = (tid + i * 256) * P + e;
-                    if (!(v[i][e] < bound) && at < a.V) {
-                        const int slot = atomicAdd(&count, 1);
-                        if (slot < kTopList) list[slot] = (unsigned long long)order_key(v[i][e]) << 32 | (0xFFFFFFFFu - (unsigned)at);
-                    }
-                }
-        }
         sum = group_sum<64>(sum);
         if (lane == 0) wave_sum[wave] = sum;
         __syncthreads();
         const int n = count;
         if (n <= kTopList)
-            write_ranked(a, row, list, n, tid, 256);
+            write_ranked(a, row, list, n, tid, THREADS);
         else
-            write_one_by_one<4>(a, row, wave_best);
-        if (a.lse && tid == 255) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3]));
+            write_one_by_one<W>(a, row, wave_best);
+        if (a.lse && tid == THREADS - 1) {
+            double total = 0.0;
+            for (int i = 0; i < W; ++i) total += (double)wave_sum[i];
+            a.lse[row] = (float)((double)base * a.inv_t + log_sum(total));
+        }
         __syncthreads();
     }
 }
@@ -1095,17 +1042,23 @@ template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
     constexpr int P = kPiece<T>;
+    const size_t row_lds = (size_t)(a.V + P - 1) / P * 16;
     const unsigned groups = (unsigned)std::min((a.rows + 15) / 16, kMaxGrid);
     if (a.V < P)                       // K <= V
         hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
     else if (a.V <= kShort && a.K <= 16)
         hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
-    else if (a.V <= kWaveClasses)
-        hipLaunchKernelGGL(top_wave_kernel<T>, dim3(grid), dim3(64), (size_t)(a.V + P - 1) / P * 16, s, a);
-    else if (a.V <= 4096)
-        hipLaunchKernelGGL((top_block_kernel<T, 4096 / 256 / P>), dim3(grid), dim3(256), 0, s, a);
-    else if (a.V <= 8192)
-        hipLaunchKernelGGL((top_block_kernel<T, 8192 / 256 / P>), dim3(grid), dim3(256), 0, s, a);
+    else if (row_lds <= 8192 && (a.K <= 32 || a.V <= kTopList)) {      // one wave: K of 64 maxima have to be a useful bound
+        if (row_lds <= 2048)
+            hipLaunchKernelGGL((top_lds_kernel<T, 1, 2>), dim3(grid), dim3(64), row_lds, s, a);
+        else if (row_lds <= 4096)
+            hipLaunchKernelGGL((top_lds_kernel<T, 1, 4>), dim3(grid), dim3(64), row_lds, s, a);
+        else
+            hipLaunchKernelGGL((top_lds_kernel<T, 1, 8>), dim3(grid), dim3(64), row_lds, s, a);
+    } else if (row_lds <= kWaveBytes)
+        hipLaunchKernelGGL((top_lds_kernel<T, 2, 8>), dim3(grid), dim3(128), row_lds, s, a);
+    else if (row_lds <= kRowBytes)
+        hipLaunchKernelGGL((top_lds_kernel<T, 4, 8>), dim3(grid), dim3(256), row_lds, s, a);
     else
         hipLaunchKernelGGL(top_stream_kernel<T>, dim3(grid), dim3(512), 0, s, a);
     OCR_HIP_CHECK(hipGetLastError());

@@ -17,6 +17,15 @@ _VALUES = {torch.float32: F32, torch.bfloat16: BF16}
 _MERGE = {'union': MERGE_UNION, 'average': MERGE_AVERAGE, 'weighted': MERGE_WEIGHTED}
 
 
+_BYTES = (torch.float8_e4m3fn, torch.uint8)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, '_cuda_getCurrentRawStream') else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
 def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
@@ -368,119 +377,123 @@ class HipContext:
         return tokens, scores
 
     # ------------------------------------------------------------------ 8-bit products
+    # (Operators of a few microseconds: addresses go to the library as plain integers, checks read a tensor's properties once.)
     def _on(self):
         """The stream these operators run on: the current one of the handle's device, whatever device is current."""
-        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return _raw_stream(self.device.index)
 
     def _rows(self, who, name, x):
-        """(values, rows, columns, elements between rows) of a float32 / bfloat16 tensor (..., columns) on the handle's
-        device; a tensor whose rows do not lie one row stride apart, or whose elements do not touch, is copied."""
+        """(values, type code, rows, columns, elements between rows) of a float32 / bfloat16 tensor (..., columns) on the
+        handle's device; a tensor whose rows do not lie one row stride apart, or whose elements do not touch, is copied."""
         code = _VALUES.get(x.dtype)
         if code is None:
             raise ValueError('{}: {} must be float32 or bfloat16, not {}'.format(who, name, x.dtype))
         if x.device != self.device:
             raise ValueError('{}: {} is on {}, the handle on {}'.format(who, name, x.device, self.device))
-        if x.dim() == 0:
-            raise ValueError('{}: {} has no dimensions'.format(who, name))
-        cols = x.shape[-1]
-        if x.dim() != 2:
-            x = x.reshape(-1, cols) if cols else x.reshape(x.shape[:-1].numel(), 0)
-        if (x.stride(1) != 1 and cols > 1) or (x.shape[0] > 1 and x.stride(0) < cols):
+        shape = x.shape
+        if len(shape) != 2:
+            if not shape:
+                raise ValueError('{}: {} has no dimensions'.format(who, name))
+            x = x.reshape(shape[:-1].numel(), shape[-1])
+        rows, cols = x.shape
+        ld, step = x.stride()
+        if (step != 1 and cols > 1) or (rows > 1 and ld < cols):
             x = x.contiguous()
-        rows = x.shape[0]
-        return x, code, rows, cols, (x.stride(0) if rows > 1 else cols)
+            ld = cols
+        return x, code, rows, cols, (ld if rows > 1 else cols)
 
     def _table(self, who, name, t, dtype, shape):
         if t.dtype != dtype or t.device != self.device:
             raise ValueError('{}: {} must be {} on {}, not {} on {}'.format(who, name, dtype, self.device, t.dtype, t.device))
-        if t.numel() != shape.numel() or t.shape != shape:
+        if t.shape != shape:
             raise ValueError('{}: {} must have the shape {}, not {}'.format(who, name, tuple(shape), tuple(t.shape)))
         return t if t.is_contiguous() else t.contiguous()
 
     def _blocks(self, who, name, m):
-        rows, cols, by = m.rows, m.cols, m.block_rows
-        if by not in (1, 128):
+        """(address of the bytes, row stride, address of the scales, their row stride) of an `Fp8Matrix`."""
+        q, scale, rows, cols, by = m
+        if by != 1 and by != 128:
             raise ValueError('{}: {} has a scale per {} rows (1 or 128)'.format(who, name, by))
-        q, scale = m.q, m.scale
         if q.device != self.device or scale.device != self.device:
             raise ValueError('{}: {} is on {} / {}, the handle on {}'.format(who, name, q.device, scale.device, self.device))
-        if q.element_size() != 1 or scale.dtype != torch.uint8 or q.dim() != 2 or scale.dim() != 2:
-            raise ValueError('{}: {} must hold 8-bit values and uint8 scales in two dimensions each'.format(who, name))
-        if q.dtype != torch.float8_e4m3fn and q.dtype != torch.uint8:
-            raise ValueError('{}: {} must hold float8_e4m3fn values (or their bytes)'.format(who, name))
-        if (q.shape[0] != rows or q.shape[1] != (cols + 127) // 128 * 128 or scale.shape[0] != (cols + 127) // 128
-                or scale.shape[1] < (rows + by - 1) // by):
-            raise ValueError('{}: {} of {} x {} has values {} and scales {}'.format(who, name, rows, cols, tuple(q.shape),
-                                                                                  tuple(scale.shape)))
-        if (q.shape[1] > 0 and q.stride(1) != 1) or scale.stride(1) != 1:
+        if q.dtype not in _BYTES or scale.dtype != torch.uint8:
+            raise ValueError('{}: {} must hold float8_e4m3fn values (or their bytes) and uint8 scales, not {} and {}'.format(
+                who, name, q.dtype, scale.dtype))
+        qs, ss, kb = q.shape, scale.shape, (cols + 127) // 128
+        if len(qs) != 2 or len(ss) != 2 or qs[0] != rows or qs[1] != kb * 128 or ss[0] != kb or ss[1] < (rows + by - 1) // by:
+            raise ValueError('{}: {} of {} x {} has values {} and scales {}'.format(who, name, rows, cols, tuple(qs), tuple(ss)))
+        ld, step = q.stride()
+        ld_s, step_s = scale.stride()
+        if (step != 1 and kb) or (step_s != 1 and ss[1] > 1):
             raise ValueError('{}: the rows of {} must be contiguous'.format(who, name))
-        return _ptr(q), q.stride(0) if rows > 1 else q.shape[1], _ptr(scale), scale.stride(0) if scale.shape[1] else 0
+        return q.data_ptr(), ld if rows > 1 else kb * 128, scale.data_ptr(), ld_s if ss[1] else 0
 
     def quantize_fp8(self, x, block_rows=1, transpose=False):
         """x (..., cols) float32 / bfloat16 on the GPU, taken as a matrix (or its transpose) -> `Fp8Matrix`: e4m3 values
         with a power-of-two scale per `block_rows` x 128 block (1: activations and gradients, 128: weights)."""
         x, code, rows, cols, ld = self._rows('quantize_fp8', 'x', x)
-        if block_rows not in (1, 128):
+        if block_rows != 1 and block_rows != 128:
             raise ValueError('quantize_fp8: block_rows is 1 or 128, not {}'.format(block_rows))
         R, C = (cols, rows) if transpose else (rows, cols)
-        ld_q, kb, ld_s = (C + 127) // 128 * 128, (C + 127) // 128, ((R + block_rows - 1) // block_rows + 15) // 16 * 16
-        q = torch.empty((R, ld_q), dtype=torch.float8_e4m3fn, device=self.device)
+        kb, ld_s = (C + 127) // 128, ((R + block_rows - 1) // block_rows + 15) // 16 * 16
+        q = torch.empty((R, kb * 128), dtype=torch.float8_e4m3fn, device=self.device)
         scale = torch.empty((kb, ld_s), dtype=torch.uint8, device=self.device)
-        check(self.lib.ocrhip_quantize_fp8(self._h, _ptr(x), code, rows, cols, ld, block_rows, 1 if transpose else 0, _ptr(q),
-                                           ld_q, _ptr(scale), ld_s, self._on()))
+        check(self.lib.ocrhip_quantize_fp8(self._h, x.data_ptr(), code, rows, cols, ld, block_rows, 1 if transpose else 0, q.data_ptr(),
+                                           kb * 128, scale.data_ptr(), ld_s, self._on()))
         return Fp8Matrix(q, scale, R, C, block_rows)
 
     def _product(self, who, rows, n, k, bias, out_dtype, need):
-        if out_dtype not in _VALUES:
+        """(address of the bias, output, its type code, workspace, its size)"""
+        code = _VALUES.get(out_dtype)
+        if code is None:
             raise ValueError('{}: out_dtype must be float32 or bfloat16, not {}'.format(who, out_dtype))
         if bias is not None:
-            bias = self._table(who, 'bias', bias, torch.float32, torch.Size((n,)))
+            bias = self._table(who, 'bias', bias, torch.float32, (n,))
         out = torch.empty((rows, n), dtype=out_dtype, device=self.device)
-        ws_bytes = need(rows, n, k)
-        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=self.device) if ws_bytes else None
-        return bias, out, ws, ws_bytes
+        size = need(rows, n, k)
+        return bias, out, code, torch.empty(size, dtype=torch.uint8, device=self.device) if size else None, size
 
     def gemm_fp8(self, a, b, bias=None, out_dtype=torch.float32):
         """a (M, K) with block_rows 1, b (N, K) with block_rows 1 or 128 (`Fp8Matrix`), bias (N,) float32 or None ->
         a . b^T + bias (M, N) in float32 or bfloat16, float32 sums."""
+        m, n, k = a.rows, b.rows, a.cols
         if a.block_rows != 1:
             raise ValueError('gemm_fp8: a needs a scale per row (block_rows 1, not {})'.format(a.block_rows))
-        if a.cols != b.cols:
-            raise ValueError('gemm_fp8: a has {} columns, b {}'.format(a.cols, b.cols))
+        if k != b.cols:
+            raise ValueError('gemm_fp8: a has {} columns, b {}'.format(k, b.cols))
         pa, lda, pas, ldas = self._blocks('gemm_fp8', 'a', a)
         pb, ldb, pbs, ldbs = self._blocks('gemm_fp8', 'b', b)
-        bias, out, ws, ws_bytes = self._product('gemm_fp8', a.rows, b.rows, a.cols, bias, out_dtype, self.lib.ocrhip_gemm_fp8_workspace)
-        check(self.lib.ocrhip_gemm_fp8(self._h, pa, lda, pas, ldas, pb, ldb, pbs, ldbs, b.block_rows, a.rows, b.rows, a.cols,
-                                       _ptr(bias), _ptr(out), _VALUES[out_dtype], b.rows, _ptr(ws), ws_bytes, self._on()))
+        bias, out, code, ws, size = self._product('gemm_fp8', m, n, k, bias, out_dtype, self.lib.ocrhip_gemm_fp8_workspace)
+        check(self.lib.ocrhip_gemm_fp8(self._h, pa, lda, pas, ldas, pb, ldb, pbs, ldbs, b.block_rows, m, n, k, _address(bias),
+                                       out.data_ptr(), code, n, _address(ws), size, self._on()))
         return out
 
     def linear_fp8(self, x, weight, bias=None, out_dtype=torch.float32):
         """Dense layer on 8-bit weights: x (..., K) float32 / bfloat16, quantised by rows in the call, weight (N, K)
         `Fp8Matrix`, bias (N,) float32 or None -> (..., N) in float32 or bfloat16."""
-        shape = x.shape[:-1] + (weight.rows,)
-        x, code, rows, cols, ld = self._rows('linear_fp8', 'x', x)
-        if cols != weight.cols:
-            raise ValueError('linear_fp8: x has {} columns, the weight {}'.format(cols, weight.cols))
+        shape, n = x.shape, weight.rows
+        x, x_code, rows, k, ld = self._rows('linear_fp8', 'x', x)
+        if k != weight.cols:
+            raise ValueError('linear_fp8: x has {} columns, the weight {}'.format(k, weight.cols))
         pb, ldb, pbs, ldbs = self._blocks('linear_fp8', 'weight', weight)
-        bias, out, ws, ws_bytes = self._product('linear_fp8', rows, weight.rows, cols, bias, out_dtype, self.lib.ocrhip_linear_fp8_workspace)
-        check(self.lib.ocrhip_linear_fp8(self._h, _ptr(x), code, ld, pb, ldb, pbs, ldbs, weight.block_rows, rows, weight.rows,
-                                         cols, _ptr(bias), _ptr(out), _VALUES[out_dtype], weight.rows, _ptr(ws), ws_bytes, self._on()))
-        return out.view(shape)
+        bias, out, code, ws, size = self._product('linear_fp8', rows, n, k, bias, out_dtype, self.lib.ocrhip_linear_fp8_workspace)
+        check(self.lib.ocrhip_linear_fp8(self._h, x.data_ptr(), x_code, ld, pb, ldb, pbs, ldbs, weight.block_rows, rows, n, k,
+                                         _address(bias), out.data_ptr(), code, n, _address(ws), size, self._on()))
+        return out if len(shape) == 2 else out.view(shape[:-1] + (n,))
 
     # ------------------------------------------------------------------ distillation
     def top_logits(self, logits, k, temperature=1.0, want_lse=True):
         """logits (..., V) float32 / bfloat16 -> (values (..., k) float32, index (..., k) int32, lse (...) float32): the k
         largest of every row in descending order (lower class first among equals) and log sum exp(logits / temperature)."""
-        shape = logits.shape[:-1]
         x, code, rows, V, ld = self._rows('top_logits', 'logits', logits)
-        k = int(k)
+        k, shape = int(k), logits.shape[:-1]
         if not 1 <= k <= 64:
             raise ValueError('top_logits: {} entries per row (1 .. 64)'.format(k))
         values = torch.empty(shape + (k,), dtype=torch.float32, device=self.device)
         index = torch.empty(shape + (k,), dtype=torch.int32, device=self.device)
         lse = torch.empty(shape, dtype=torch.float32, device=self.device) if want_lse else None
-        check(self.lib.ocrhip_top_logits(self._h, _ptr(x), code, rows, V, ld, k, float(temperature), _ptr(values), _ptr(index),
-                                         _ptr(lse), self._on()))
+        check(self.lib.ocrhip_top_logits(self._h, x.data_ptr(), code, rows, V, ld, k, float(temperature), values.data_ptr(), index.data_ptr(),
+                                         _address(lse), self._on()))
         return values, index, lse
 
     def distill_loss(self, logits, top_values, top_index, top_lse=None, temperature=1.0, row_weight=None, want_loss=True,
@@ -489,11 +502,11 @@ class HipContext:
         float32, top_index (..., K) int32 (a class outside [0, V) is no entry), in one pass with its gradient ->
         dict(loss (...) float32, grad like logits).  top_lse None: the teacher's probabilities are the softmax over its
         entries; the teacher's lse (...) at this temperature: everything outside them is one more class.  row_weight (...)
-        float32 scales loss and gradient of a row (0: a padded step, not read); the loss carries temperature ** 2.  For a
-        batch's backward pass hand the gradient of the summed loss in as row_weight."""
-        who, shape = 'distill_loss', logits.shape[:-1]
+        float32 scales loss and gradient of a row (0: a padded step); the loss carries temperature ** 2.  For a batch's
+        backward pass hand the gradient of the summed loss in as row_weight."""
+        who, full = 'distill_loss', logits.shape
         x, code, rows, V, ld = self._rows(who, 'logits', logits)
-        K = int(top_values.shape[-1]) if top_values.dim() else 0
+        shape, K = full[:-1], int(top_values.shape[-1]) if top_values.dim() else 0
         top_values = self._table(who, 'top_values', top_values, torch.float32, shape + (K,))
         top_index = self._table(who, 'top_index', top_index, torch.int32, shape + (K,))
         if top_lse is not None:
@@ -501,9 +514,10 @@ class HipContext:
         if row_weight is not None:
             row_weight = self._table(who, 'row_weight', row_weight, torch.float32, shape)
         loss = torch.empty(shape, dtype=torch.float32, device=self.device) if want_loss else None
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=self.device) if want_grad else None
-        check(self.lib.ocrhip_distill_loss(self._h, _ptr(x), code, rows, V, ld, _ptr(top_values), _ptr(top_index), K, _ptr(top_lse),
-                                           float(temperature), _ptr(row_weight), _ptr(loss), _ptr(grad), V, self._on()))
+        grad = torch.empty(full, dtype=logits.dtype, device=self.device) if want_grad else None
+        check(self.lib.ocrhip_distill_loss(self._h, x.data_ptr(), code, rows, V, ld, top_values.data_ptr(), top_index.data_ptr(), K,
+                                           _address(top_lse), float(temperature), _address(row_weight), _address(loss), _address(grad), V,
+                                           self._on()))
         return {'loss': loss, 'grad': grad}
 
     def ctc_greedy(self, logits, lengths=None, blank=0):

@@ -208,7 +208,7 @@ def test_refusals_of_the_python_callers(ctx):
         (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 100)), 'columns'),
         (lambda: ctx.gemm_fp8(_matrix(4, 200)._replace(rows=5), _matrix(7, 200)), 'of 5 x 200'),
         (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 200, by=128, block_rows=16)), 'scale per 16'),
-        (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 200, q=torch.zeros(7, 256))), '8-bit'),
+        (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 200, q=torch.zeros(7, 256))), 'float8_e4m3fn'),
         (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 200, q=torch.zeros(7, 256, dtype=torch.int8))), 'float8_e4m3fn'),
         (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 200, scale=torch.zeros(2, 16))), 'uint8'),
         (lambda: ctx.gemm_fp8(_matrix(4, 200), _matrix(7, 200, scale=torch.zeros(1, 16, dtype=torch.uint8))), 'scales (1, 16)'),
