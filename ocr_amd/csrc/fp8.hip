@@ -35,6 +35,12 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+#ifndef FBM
+#define FBM 128
+#define FBN 128
+#define FWM 2
+#define FWN 2
+#endif
 std::mutex g_lds_mutex;              // guards the once-per-device LDS opt-in of the kernels that need more than 64 KB
 
 constexpr int kBlk = 128;            // values of k that share a scale
@@ -279,6 +285,7 @@ struct GemmArgs {
     int64_t lda, ldas, ldb, ldbs, ldc;
     int64_t M;
     int N, K;
+    bool stream;         // rows of C are whole 128-byte lines: stored past the caches
 };
 
 // scale byte -> the float whose exponent field it is (what the conversion below reads)
@@ -433,90 +440,150 @@ __device__ __forceinline__ int place(int row) { return (row >> 1 & 3) << 1 | (ro
 template <int BM, int BN>
 constexpr int tile_stage_bytes() { return (BM + BN) * kBlk + 512; }      // operands, then 256 scale bytes of A and of B
 
+// one 16-byte piece of a row of float32 results; STREAM: it leaves the caches first (a result that is not read here)
+template <bool STREAM>
+__device__ __forceinline__ void store_f32x4(float* p, floatx4 v) {
+    if (STREAM)
+        __builtin_nontemporal_store(v, reinterpret_cast<floatx4_any*>(p));
+    else
+        *reinterpret_cast<floatx4_any*>(p) = v;
+}
+template <bool STREAM>
+__device__ __forceinline__ void store_bf16x8(__bf16* p, bf16x8 v) {
+    if (STREAM)
+        __builtin_nontemporal_store(v, reinterpret_cast<bf16x8_any*>(p));
+    else
+        *reinterpret_cast<bf16x8_any*>(p) = v;
+}
+
+// A workgroup walks its share of the tiles as one sequence of blocks of k: the first block of the next tile is on its way
+// while the last of this one is multiplied and the results leave.
 template <int BM, int BN, int WGM, int WGN, bool OUT_F32, int BROWS>
 __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
     constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, IM = TM / 16, IN = TN / 16;
     constexpr int NA = BM / 8, NI = (BM + BN) / 8, PER = NI / WAVES;     // copies of 8 rows: A's, all, per wave
     constexpr int STAGE = tile_stage_bytes<BM, BN>();
     static_assert(NI % WAVES == 0 && BM <= 256 && BN <= 256 && (BROWS == 1 || TN <= 128), "tile");
+    constexpr int F32_LANES = TN / 4, F32_STORES = 16 * F32_LANES / 64;  // lanes of a row of results, stores per 16 rows
+    constexpr int B16_LANES = TN / 8, B16_STORES = 16 * B16_LANES / 64;
+    constexpr int F32_ROW = TN * 4 + 16, B16_ROW = TN * 2 + 16;          // bytes of a staged row
+    static_assert(WAVES * 16 * F32_ROW <= STAGE, "staged rows");
+    // the fewest stores a full tile's wave makes: a wait that leaves so many operations out waits for everything in front
+    constexpr int BEHIND = IM * (OUT_F32 ? F32_STORES : B16_STORES);
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const GemmArgs& g = a.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
     const int r = lane & 15, kg = lane >> 4;
-
-    // workgroups go to the 8 dies in turn: every die gets a contiguous range of the work, in bands of 8 tile rows, so that
-    // the tiles it computes at one time share their rows of A and B in its L2
-    const unsigned total = gridDim.x, xcd = blockIdx.x & 7u;
-    unsigned work = xcd * (total >> 3) + min(xcd, total & 7u) + (blockIdx.x >> 3);
-    const unsigned per_split = (unsigned)a.tiles_m * a.tiles_n;
-    const int split = (int)(work / per_split);
-    work %= per_split;
-    const unsigned band = work / (8u * a.tiles_n), rows_in_band = min(8u, a.tiles_m - band * 8);
-    const unsigned in_band = work - band * 8u * a.tiles_n;
-    const int64_t m0 = (int64_t)(band * 8 + in_band % rows_in_band) * BM;
-    const int n0 = (int)(in_band / rows_in_band) * BN;
-
     const int nkb = (g.K + kBlk - 1) / kBlk;
-    const int kb0 = split * a.kb_split, kb1 = min(nkb, kb0 + a.kb_split);
+    const bool partial = a.splits > 1;
 
-    const int rows_a = (int)min((int64_t)BM, g.M - m0), rows_b = min(BN, g.N - n0);
-    const int k_bytes = (kb1 - kb0) * kBlk;
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(g.a + m0 * g.lda + (int64_t)kb0 * kBlk), 0, (unsigned)((rows_a - 1) * (int)g.lda + k_bytes), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)(g.b + n0 * g.ldb + (int64_t)kb0 * kBlk), 0, (unsigned)((rows_b - 1) * (int)g.ldb + k_bytes), 0x00020000);
+    // Workgroups go to the 8 dies in turn: every die gets a contiguous range of the tiles, its workgroups take them in
+    // turn, in bands of 8 tile rows, so that what a die computes at one time shares rows of A and B in its L2.
+    const unsigned total = (unsigned)a.tiles_m * a.tiles_n * a.splits, xcd = blockIdx.x & 7u;
+    const unsigned lo = xcd * (total >> 3) + min(xcd, total & 7u), hi = lo + (total >> 3) + (xcd < (total & 7u) ? 1u : 0u);
+    const unsigned stride = (gridDim.x >> 3) + (xcd < (gridDim.x & 7u) ? 1u : 0u);       // workgroups of this die
+    unsigned job = lo + (blockIdx.x >> 3);
+    if (job >= hi) return;
+    struct Job {
+        int64_t m0;
+        int n0, kb0, kb1, split;
+    };
+    auto job_of = [&](unsigned work) {
+        Job j;
+        const unsigned per_split = (unsigned)a.tiles_m * a.tiles_n;
+        j.split = (int)(work / per_split);
+        work %= per_split;
+        const unsigned band = work / (8u * a.tiles_n), rows_in_band = min(8u, a.tiles_m - band * 8);
+        const unsigned in_band = work - band * 8u * a.tiles_n;
+        j.m0 = (int64_t)(band * 8 + in_band % rows_in_band) * BM;
+        j.n0 = (int)(in_band / rows_in_band) * BN;
+        j.kb0 = j.split * a.kb_split;
+        j.kb1 = min(nkb, j.kb0 + a.kb_split);
+        return j;
+    };
+
+    // ---- the tile whose operands are being fetched
+    Job in = job_of(job);
+    __amdgpu_buffer_rsrc_t ra, rb;
     int src[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int c = wave * PER + i;
-        const int row = (c < NA ? c : c - NA) * 8 + (lane >> 3);
-        const int piece = (lane & 7) ^ place(row);
-        const bool ok = row < (c < NA ? rows_a : rows_b);
-        src[i] = ok ? row * (int)(c < NA ? g.lda : g.ldb) + piece * 16 : (int)0x80000000;
-    }
-    auto issue = [&](int kb) {
-        unsigned char* base = lds + (kb & 1) * STAGE;
+    int64_t sb_col = 0;
+    auto open = [&] {
+        const int rows_a = (int)min((int64_t)BM, g.M - in.m0), rows_b = min(BN, g.N - in.n0), k_bytes = (in.kb1 - in.kb0) * kBlk;
+        ra = __builtin_amdgcn_make_buffer_rsrc((void*)(g.a + in.m0 * g.lda + (int64_t)in.kb0 * kBlk), 0, (unsigned)((rows_a - 1) * (int)g.lda + k_bytes), 0x00020000);
+        rb = __builtin_amdgcn_make_buffer_rsrc((void*)(g.b + in.n0 * g.ldb + (int64_t)in.kb0 * kBlk), 0, (unsigned)((rows_b - 1) * (int)g.ldb + k_bytes), 0x00020000);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = wave * PER + i;
-            copy16(c < NA ? ra : rb, base + c * 1024, src[i], (kb - kb0) * kBlk);
+            const int row = (c < NA ? c : c - NA) * 8 + (lane >> 3);
+            const int piece = (lane & 7) ^ place(row);
+            const bool ok = row < (c < NA ? rows_a : rows_b);
+            src[i] = ok ? row * (int)(c < NA ? g.lda : g.ldb) + piece * 16 : (int)0x80000000;
+        }
+        // the wave's columns lie within one block of 128: its scale is a scalar load
+        sb_col = min(in.n0 + wn * TN, g.N - 1) / kBlk;
+    };
+    auto issue = [&](int kb, int half) {
+        unsigned char* base = lds + half * STAGE;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = wave * PER + i;
+            copy16(c < NA ? ra : rb, base + c * 1024, src[i], (kb - in.kb0) * kBlk);
         }
         if (wave == 0) {
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.as + (int64_t)kb * g.ldas + m0), 0, (unsigned)min((int64_t)BM, g.ldas - m0), 0x00020000);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.as + (int64_t)kb * g.ldas + in.m0), 0, (unsigned)min((int64_t)BM, g.ldas - in.m0), 0x00020000);
             copy4(rs, base + (BM + BN) * kBlk, lane * 4);
         }
         if (BROWS == 1 && wave == WAVES - 1) {
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.bs + (int64_t)kb * g.ldbs + n0), 0, (unsigned)min((int64_t)BN, g.ldbs - n0), 0x00020000);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.bs + (int64_t)kb * g.ldbs + in.n0), 0, (unsigned)min((int64_t)BN, g.ldbs - in.n0), 0x00020000);
             copy4(rs, base + (BM + BN) * kBlk + 256, lane * 4);
         }
     };
-    // the wave's columns lie within one block of 128: its scale is a scalar load, one block ahead
-    const int64_t sb_col = min(n0 + wn * TN, g.N - 1) / kBlk;
-    int sb_next = BROWS == 1 ? 0 : g.bs[(int64_t)kb0 * g.ldbs + sb_col];
+    open();
+    int kb_in = in.kb0, half = 0;
+    issue(kb_in, 0);
+    int sb_next = BROWS == 1 ? 0 : g.bs[(int64_t)kb_in * g.ldbs + sb_col];
 
+    // ---- the tile that is being multiplied
+    Job out = in;
+    bool more = true;                                   // blocks left to fetch
+    bool behind = false;                                // BEHIND stores or more have been issued since the last copies
+    const int a_row = wm * TM + r, b_row = wn * TN + r;
+    for (;;) {
     floatx4 acc[IM][IN];
 #pragma unroll
     for (int i = 0; i < IM; ++i)
 #pragma unroll
         for (int j = 0; j < IN; ++j) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    issue(kb0);
-    const bool two = kb1 - kb0 == 2;                    // both blocks fit the buffers: one wait for memory
-    if (two) issue(kb0 + 1);
-    const int a_row = wm * TM + r, b_row = wn * TN + r;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    for (int kb = out.kb0; kb < out.kb1; ++kb, half ^= 1) {
         // my copies have landed and my reads of the other buffer are done; behind the barrier everybody's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (behind)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BEHIND) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (!two && kb + 1 < kb1) issue(kb + 1);
-        const unsigned char* base = lds + (kb & 1) * STAGE;
+        behind = false;
+        const int sb = sb_next;
+        if (++kb_in == in.kb1) {
+            job += stride;
+            more = job < hi;
+            if (more) {
+                in = job_of(job);
+                open();
+                kb_in = in.kb0;
+            }
+        }
+        if (more) {
+            issue(kb_in, half ^ 1);
+            if (BROWS != 1) sb_next = g.bs[(int64_t)kb_in * g.ldbs + sb_col];
+        }
+        const unsigned char* base = lds + half * STAGE;
         const unsigned char* pa = base + a_row * kBlk;
         const unsigned char* pb = base + (BM + b_row) * kBlk;
         const unsigned char* psa = base + (BM + BN) * kBlk + a_row;
         const unsigned char* psb = base + (BM + BN) * kBlk + 256 + b_row;
         const int sw = place(r);                        // rows 16 apart have the same permutation
-        int sb = sb_next;
-        if (BROWS != 1 && kb + 1 < kb1) sb_next = g.bs[(int64_t)(kb + 1) * g.ldbs + sb_col];
         if constexpr (OUT_F32) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {               // 16 of the lane's 32 bytes: two instructions of 32 values of k
@@ -546,84 +613,101 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
             int sbv[IN];
 #pragma unroll
             for (int j = 0; j < IN; ++j) {
-                const intx4 lo = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at0), hi = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at1);
-                bv[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                const intx4 lo4 = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at0), hi4 = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at1);
+                bv[j] = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
                 sbv[j] = BROWS == 1 ? (int)psb[j * 16] : sb;
             }
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
-                const intx4 lo = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at0), hi = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at1);
-                const intx8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                const intx4 lo4 = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at0), hi4 = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at1);
+                const intx8 av = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
                 const int sa = psa[i * 16];
 #pragma unroll
                 for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv[j], av, acc[i][j], 0, 0, 0, sbv[j], 0, sa);
             }
         }
     }
-    // Lane (r, kg) holds C[m0 + wm TM + 16 i + r][n0 + wn TN + 16 j + 4 kg .. + 3]: 16 bytes of 16 rows per store.  Every
-    // wave turns its 16-row slices through an LDS area of its own into runs of whole rows of its TN columns, which fill
-    // the lines they touch (rows of odd length start anywhere in one).
-    const bool partial = a.splits > 1;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();          // every wave is done with the operands
-    asm volatile("" ::: "memory");
-    if (partial || OUT_F32) {
-        constexpr int SROW = TN * 4 + 16, LANES = TN / 4;      // bytes of a staged row, lanes of a row
-        unsigned char* mine = lds + wave * (16 * SROW);
-        float* out = partial ? a.part + (int64_t)split * g.M * g.N : reinterpret_cast<float*>(g.c);
-        const int64_t ldo = partial ? g.N : g.ldc;
-        const int c4 = lane % LANES * 4, n = n0 + wn * TN + c4;
-        floatx4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (g.bias && !partial)
+    {
+        const int used = half ^ 1;                      // the buffer of the last block
+        // Lane (r, kg) holds C[m0 + wm TM + 16 i + r][n0 + wn TN + 16 j + 4 kg .. + 3]: 16 bytes of 16 rows per store.  Every
+        // wave turns its 16-row slices through an area of its own in the buffer just used into runs of whole rows of its
+        // TN columns, which fill the lines they touch (rows of odd length start anywhere in one).
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                   // every wave is done with that buffer's operands
+        asm volatile("" ::: "memory");
+        const bool full = out.m0 + BM <= g.M && out.n0 + BN <= g.N;
+        if (partial || OUT_F32) {
+            unsigned char* mine = lds + used * STAGE + wave * (16 * F32_ROW);
+            const int64_t ldo = partial ? g.N : g.ldc;
+            const int c4 = lane % F32_LANES * 4, n = out.n0 + wn * TN + c4;
+            const int64_t m_first = out.m0 + wm * TM + lane / F32_LANES;
+            float* dst = (partial ? a.part + (int64_t)out.split * g.M * g.N : reinterpret_cast<float*>(g.c)) + m_first * ldo + n;
+            floatx4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (g.bias && !partial)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = n + e < g.N ? g.bias[n + e] : 0.0f;
+                for (int e = 0; e < 4; ++e) bias[e] = n + e < g.N ? g.bias[n + e] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < IM; ++i) {
+            for (int i = 0; i < IM; ++i) {
 #pragma unroll
-            for (int j = 0; j < IN; ++j) *reinterpret_cast<floatx4*>(mine + r * SROW + (j * 16 + kg * 4) * 4) = acc[i][j];
-            __builtin_amdgcn_wave_barrier();
+                for (int j = 0; j < IN; ++j) *reinterpret_cast<floatx4*>(mine + r * F32_ROW + (j * 16 + kg * 4) * 4) = acc[i][j];
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int t = 0; t < 16 * LANES / 64; ++t) {
-                const int row = t * (64 / LANES) + lane / LANES;
-                const int64_t m = m0 + wm * TM + i * 16 + row;
-                const floatx4 v = *reinterpret_cast<const floatx4*>(mine + row * SROW + c4 * 4) + bias;
-                if (m < g.M) store_c4<true>(out, m * ldo + n, v, g.N - n);
-            }
-            __builtin_amdgcn_wave_barrier();
-        }
-    } else {
-        constexpr int SROW = TN * 2 + 16, LANES = TN / 8;
-        unsigned char* mine = lds + wave * (16 * SROW);
-        const int c8 = lane % LANES * 8, nw = n0 + wn * TN + c8;
-#pragma unroll
-        for (int i = 0; i < IM; ++i) {
-#pragma unroll
-            for (int j = 0; j < IN; ++j) {
-                const int n = n0 + wn * TN + j * 16 + kg * 4;
-                floatx4 v = acc[i][j];
-                if (g.bias)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += n + e < g.N ? g.bias[n + e] : 0.0f;
-                *reinterpret_cast<bf16x4*>(mine + r * SROW + (j * 16 + kg * 4) * 2) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-            }
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int t = 0; t < 16 * LANES / 64; ++t) {
-                const int row = t * (64 / LANES) + lane / LANES;
-                const int64_t m = m0 + wm * TM + i * 16 + row;
-                const bf16x8 v = *reinterpret_cast<const bf16x8*>(mine + row * SROW + c8 * 2);
-                if (m >= g.M) continue;
-                __bf16* dst = reinterpret_cast<__bf16*>(g.c) + m * g.ldc + nw;
-                if (nw + 8 <= g.N) {
-                    *reinterpret_cast<bf16x8_any*>(dst) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (nw + e < g.N) dst[e] = v[e];
+                for (int t = 0; t < F32_STORES; ++t) {
+                    constexpr int STEP = 64 / F32_LANES;
+                    const floatx4 v = *reinterpret_cast<const floatx4*>(mine + (t * STEP + lane / F32_LANES) * F32_ROW + c4 * 4) + bias;
+                    float* at = dst + (i * 16 + t * STEP) * ldo;
+                    if (full && g.stream)
+                        store_f32x4<true>(at, v);
+                    else if (full)
+                        store_f32x4<false>(at, v);
+                    else if (m_first + i * 16 + t * STEP < g.M)
+                        store_c4<true>(at, 0, v, g.N - n);
                 }
+                __builtin_amdgcn_wave_barrier();
             }
-            __builtin_amdgcn_wave_barrier();
+        } else {
+            unsigned char* mine = lds + used * STAGE + wave * (16 * B16_ROW);
+            const int c8 = lane % B16_LANES * 8, n8 = out.n0 + wn * TN + c8;
+            const int64_t m_first = out.m0 + wm * TM + lane / B16_LANES;
+            __bf16* dst = reinterpret_cast<__bf16*>(g.c) + m_first * g.ldc + n8;
+#pragma unroll
+            for (int i = 0; i < IM; ++i) {
+#pragma unroll
+                for (int j = 0; j < IN; ++j) {
+                    const int n = out.n0 + wn * TN + j * 16 + kg * 4;
+                    floatx4 v = acc[i][j];
+                    if (g.bias)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += n + e < g.N ? g.bias[n + e] : 0.0f;
+                    *reinterpret_cast<bf16x4*>(mine + r * B16_ROW + (j * 16 + kg * 4) * 2) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int t = 0; t < B16_STORES; ++t) {
+                    constexpr int STEP = 64 / B16_LANES;
+                    const bf16x8 v = *reinterpret_cast<const bf16x8*>(mine + (t * STEP + lane / B16_LANES) * B16_ROW + c8 * 2);
+                    __bf16* at = dst + (i * 16 + t * STEP) * g.ldc;
+                    if (full && g.stream) {
+                        store_bf16x8<true>(at, v);
+                    } else if (full) {
+                        store_bf16x8<false>(at, v);
+                    } else if (m_first + i * 16 + t * STEP < g.M) {
+                        if (n8 + 8 <= g.N) {
+                            *reinterpret_cast<bf16x8_any*>(at) = v;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (n8 + e < g.N) at[e] = v[e];
+                        }
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
         }
+        if (!more) return;
+        behind = full;
+        out = in;
+    }
     }
 }
 
@@ -643,6 +727,9 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const float* __restrict_
 template <int BM, int BN, int WGM, int WGN, bool OUT_F32, int BROWS>
 int launch_tile(const TileArgs& a, hipStream_t s) {
     constexpr int bytes = 2 * tile_stage_bytes<BM, BN>();
+    OCR_REQUIRE(a.tiles_m == (a.g.M + BM - 1) / BM && a.tiles_n == (a.g.N + BN - 1) / BN && a.splits >= 1 &&
+                    (int64_t)(a.splits - 1) * a.kb_split < (a.g.K + kBlk - 1) / kBlk,
+                "gemm_fp8: %d x %d tiles and %d splits do not fit the kernel", a.tiles_m, a.tiles_n, a.splits);
     auto kernel = &gemm_tile_kernel<BM, BN, WGM, WGN, OUT_F32, BROWS>;
     static bool opted[64] = {};
     int dev = 0;
@@ -654,7 +741,7 @@ int launch_tile(const TileArgs& a, hipStream_t s) {
             opted[dev & 63] = true;
         }
     }
-    hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WGM, WGN, OUT_F32, BROWS>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(WGM * WGN * 64), bytes, s, a);
+    hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WGM, WGN, OUT_F32, BROWS>), dim3((unsigned)std::min<int64_t>((int64_t)a.tiles_m * a.tiles_n * a.splits, BM * BN > 128 * 128 ? 256 : 512)), dim3(WGM * WGN * 64), bytes, s, a);
     OCR_HIP_CHECK(hipGetLastError());
     return OCRHIP_OK;
 }
@@ -670,7 +757,8 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
     const int64_t nkb = (K + kBlk - 1) / kBlk;
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
     const bool large = !out_f32 && big >= 192;
-    p.bm = p.bn = large ? 256 : 128;
+    p.bm = large ? 256 : out_f32 ? FBM : 128;
+    p.bn = large ? 256 : out_f32 ? FBN : 128;
     p.tiles_m = (M + p.bm - 1) / p.bm;
     p.tiles_n = (N + p.bn - 1) / p.bn;
     const int64_t tiles = p.tiles_m * p.tiles_n;
@@ -776,7 +864,8 @@ int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, 
                     void* c, int c_dtype, int64_t ld_c, void* ws, hipStream_t s) {
     if (M == 0 || N == 0) return OCRHIP_OK;
     const bool f32 = c_dtype == OCRHIP_F32;
-    GemmArgs g{a.q, a.scale, b.q, b.scale, bias, c, a.ld, a.ld_scale, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K};
+    const int64_t row_bytes = ld_c * (f32 ? 4 : 2);
+    GemmArgs g{a.q, a.scale, b.q, b.scale, bias, c, a.ld, a.ld_scale, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K, row_bytes % 128 == 0 && reinterpret_cast<uintptr_t>(c) % 128 == 0};
     const double flops = 2.0 * (double)M * N * K, bytes = (double)(M + N) * K + (f32 ? 4.0 : 2.0) * (double)M * N;
     if (M <= kMaxRows) {
         ProfScope prof(f32 ? "gemm_fp8<rows,f32>" : "gemm_fp8<rows,bf16>", flops, bytes, s);
@@ -787,10 +876,10 @@ int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, 
     TileArgs t{g, (int)p.tiles_m, (int)p.tiles_n, p.splits, p.kb_split, reinterpret_cast<float*>(ws)};
     {
         ProfScope prof(p.bm == 256 ? "gemm_fp8<256,bf16>" : f32 ? "gemm_fp8<128,f32>" : "gemm_fp8<128,bf16>", flops, bytes, s);
-        if (p.bm == 256)
+        if (f32)
+            OCR_TRY(b_block_rows == 1 ? (launch_tile<FBM, FBN, FWM, FWN, true, 1>(t, s)) : (launch_tile<FBM, FBN, FWM, FWN, true, kBlk>(t, s)));
+        else if (p.bm == 256)
             OCR_TRY(b_block_rows == 1 ? (launch_tile<256, 256, 2, 4, false, 1>(t, s)) : (launch_tile<256, 256, 2, 4, false, kBlk>(t, s)));
-        else if (f32)
-            OCR_TRY(b_block_rows == 1 ? (launch_tile<128, 128, 2, 2, true, 1>(t, s)) : (launch_tile<128, 128, 2, 2, true, kBlk>(t, s)));
         else
             OCR_TRY(b_block_rows == 1 ? (launch_tile<128, 128, 2, 2, false, 1>(t, s)) : (launch_tile<128, 128, 2, 2, false, kBlk>(t, s)));
     }
@@ -812,7 +901,7 @@ int launch_linear_fp8_rows(const void* x, int x_dtype, int64_t ld_x, const Fp8Op
                            void* c, int c_dtype, int64_t ld_c, hipStream_t s) {
     if (M == 0 || N == 0) return OCRHIP_OK;
     const bool f32 = c_dtype == OCRHIP_F32, xf32 = x_dtype == OCRHIP_F32;
-    GemmArgs g{reinterpret_cast<const uint8_t*>(x), nullptr, b.q, b.scale, bias, c, ld_x, 0, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K};
+    GemmArgs g{reinterpret_cast<const uint8_t*>(x), nullptr, b.q, b.scale, bias, c, ld_x, 0, b.ld, b.ld_scale, ld_c, M, (int)N, (int)K, false};
     ProfScope prof("linear_fp8<rows>", 2.0 * (double)M * N * K, (xf32 ? 4.0 : 2.0) * (double)M * K + (double)N * K + (f32 ? 4.0 : 2.0) * (double)M * N, s);
     return xf32 ? launch_rows_any<float>(g, f32, b_block_rows, s) : launch_rows_any<uint16_t>(g, f32, b_block_rows, s);
 }
