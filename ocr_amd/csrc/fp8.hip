@@ -35,12 +35,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-#ifndef FBM
-#define FBM 128
-#define FBN 128
-#define FWM 2
-#define FWN 2
-#endif
 std::mutex g_lds_mutex;              // guards the once-per-device LDS opt-in of the kernels that need more than 64 KB
 
 constexpr int kBlk = 128;            // values of k that share a scale
@@ -60,8 +54,8 @@ __device__ __forceinline__ unsigned scale_byte(float amax) {
     return (unsigned)(max(e, -127) + kBias);
 }
 
-// 2^-(byte - 127) as a product of two floats: 2^127 is one, but the factor of a byte 0 block's subnormals is 2^127 and the
-// one of byte 247 is 2^-120, so one float holds every factor that occurs.
+// 2^-(byte - 127): between 2^127 (byte 0, the clamped exponent) and 2^-120 (byte 247, the largest finite float's), a float
+// for every byte that occurs
 __device__ __forceinline__ float inverse_scale(unsigned byte) { return ldexpf(1.0f, kBias - (int)byte); }
 
 // what counts for amax: infinities and NaN become NaN in e4m3 whatever the scale
@@ -417,7 +411,8 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k)
 // bytes go straight from memory to LDS; the next block's copies are in flight while this one is multiplied (two buffers,
 // one barrier per block).  A row is 8 pieces of 16 bytes; piece c of row r lies at place c ^ place(r), chosen so that the 16
 // lanes of a read phase (lanes 0-3, 12-15 and 20-27 of a half wave, and the other 16) hit 16 different groups of banks; the
-// copy writes lane after lane, so the permutation is applied to the address it reads from.  Rows beyond M or N are offsets beyond the descriptor: zeros.
+// copy writes lane after lane, so the permutation is applied to the address it reads from.  Rows beyond M or N are offsets
+// beyond the descriptor: zeros.
 // B is the matrix instruction's row operand, A its column operand: a lane then holds 4 neighbouring columns of one row.
 struct TileArgs {
     GemmArgs g;
@@ -757,8 +752,8 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
     const int64_t nkb = (K + kBlk - 1) / kBlk;
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
     const bool large = !out_f32 && big >= 192;
-    p.bm = large ? 256 : out_f32 ? FBM : 128;
-    p.bn = large ? 256 : out_f32 ? FBN : 128;
+    p.bm = large ? 256 : 128;
+    p.bn = large ? 256 : 128;
     p.tiles_m = (M + p.bm - 1) / p.bm;
     p.tiles_n = (N + p.bn - 1) / p.bn;
     const int64_t tiles = p.tiles_m * p.tiles_n;
@@ -877,7 +872,7 @@ int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, 
     {
         ProfScope prof(p.bm == 256 ? "gemm_fp8<256,bf16>" : f32 ? "gemm_fp8<128,f32>" : "gemm_fp8<128,bf16>", flops, bytes, s);
         if (f32)
-            OCR_TRY(b_block_rows == 1 ? (launch_tile<FBM, FBN, FWM, FWN, true, 1>(t, s)) : (launch_tile<FBM, FBN, FWM, FWN, true, kBlk>(t, s)));
+            OCR_TRY(b_block_rows == 1 ? (launch_tile<128, 128, 2, 2, true, 1>(t, s)) : (launch_tile<128, 128, 2, 2, true, kBlk>(t, s)));
         else if (p.bm == 256)
             OCR_TRY(b_block_rows == 1 ? (launch_tile<256, 256, 2, 4, false, 1>(t, s)) : (launch_tile<256, 256, 2, 4, false, kBlk>(t, s)));
         else
