@@ -123,7 +123,12 @@ int ocrhip_destroy(ocrhip_handle h);
  *   "fuse_ctc": 1 (default): when ocrhip_crnn_forward* is asked for tokens but not for logits, the class layer
  *   Dense(vocab) reduces every row to one (maximum, class) pair per block of 128 classes in its epilogue and the CTC
  *   kernel finishes the argmax over those pairs: the (rows, vocab) logits are never written or read.  0: logits go
- *   through a buffer of the handle.  Same tokens and scores bit for bit. */
+ *   through a buffer of the handle.  Same tokens and scores bit for bit.
+ *   "fp8_dense": 0 (default) | 1: the bfloat16-tensor recogniser (compute_dtype OCRHIP_BF16, bf16_tensors = 1, VGG
+ *   extractor) computes its dense layers - the LSTM input projections, the linear layers, Dense(vocab) - as
+ *   ocrhip_linear_fp8 does: input rows quantised with a scale per 128 values, weights (quantised by
+ *   ocrhip_crnn_load_weights) with a scale per 128 x 128.  Every operand is then off by up to 2^-4 of itself: logits within
+ *   0.2 of the bfloat16 recogniser's in norm (measured: 0.06).  Other forward calls do not read it. */
 int ocrhip_set_option(ocrhip_handle h, const char* name, int value);
 
 /* ------------------------------------------------------------------------------------ EAST --

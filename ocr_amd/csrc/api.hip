@@ -315,7 +315,7 @@ int ocrhip_destroy(ocrhip_handle h) {
     if (!h) return OCRHIP_OK;
     (void)hipSetDevice(h->device);
     (void)hipDeviceSynchronize();
-    auto free_layer = [](ConvLayer& L) { L.w_f32.release(); L.w_wino.release(); L.w_wino4.release(); L.w_wino4b.release(); L.w_wino4c.release(); L.w_bf16.release(); L.w_bf16t.release(); L.bias.release(); L.w_gemm.release(); L.bias_gemm.release(); };
+    auto free_layer = [](ConvLayer& L) { L.w_f32.release(); L.w_wino.release(); L.w_wino4.release(); L.w_wino4b.release(); L.w_wino4c.release(); L.w_bf16.release(); L.w_bf16t.release(); L.w_fp8.release(); L.s_fp8.release(); L.bias.release(); L.w_gemm.release(); L.bias_gemm.release(); };
     for (auto& L : h->crnn.rconv) free_layer(L);
     for (auto& L : h->east.vgg) free_layer(L);
     for (auto& L : h->east.merge) free_layer(L);
@@ -338,7 +338,7 @@ int ocrhip_destroy(ocrhip_handle h) {
         if (h->crnn.aux_join[i]) (void)hipEventDestroy(h->crnn.aux_join[i]);
     }
     if (h->crnn.aux_fork) (void)hipEventDestroy(h->crnn.aux_fork);
-    for (DevBuf* b : {&h->crnn.feats, &h->crnn.xw, &h->crnn.hbuf, &h->crnn.cbuf, &h->crnn.seq, &h->crnn.lin, &h->crnn.logits, &h->crnn.seq16, &h->crnn.meta, &h->crnn.lstm_counters, &h->crnn.pmax, &h->crnn.pidx})
+    for (DevBuf* b : {&h->crnn.feats, &h->crnn.xw, &h->crnn.hbuf, &h->crnn.cbuf, &h->crnn.seq, &h->crnn.lin, &h->crnn.logits, &h->crnn.seq16, &h->crnn.in8, &h->crnn.in8_scale, &h->crnn.ws8, &h->crnn.meta, &h->crnn.lstm_counters, &h->crnn.pmax, &h->crnn.pidx})
         b->release();
     h->crnn.ring.release();
     if (h->crnn.lstm_err_host) (void)hipHostFree(h->crnn.lstm_err_host);
@@ -642,6 +642,31 @@ static std::vector<ResLayer> resnet_layers() {
     return L;
 }
 
+// row strides of an 8-bit matrix of `cols` columns and of the scales of its `row_blocks` row blocks
+static int64_t fp8_ld(int64_t cols) { return (cols + 127) / 128 * 128; }
+static int64_t fp8_ld_scale(int64_t row_blocks) { return (row_blocks + 15) / 16 * 16; }
+
+// the 8-bit form of a dense layer's weights (cout, cin)
+static int prepare_dense_fp8(ConvLayer& L, const float* w, int cout, int cin) {
+    const int64_t ld = fp8_ld(cin), ld_scale = fp8_ld_scale((cout + 127) / 128);
+    OCR_TRY(L.w_fp8.reserve((size_t)cout * ld));
+    OCR_TRY(L.s_fp8.reserve((size_t)(ld / 128) * ld_scale));
+    DevBuf src;
+    int rc = src.reserve((size_t)cout * cin * sizeof(float));
+    if (rc == OCRHIP_OK && hipMemcpy(src.ptr, w, (size_t)cout * cin * sizeof(float), hipMemcpyHostToDevice) != hipSuccess) {
+        set_error("crnn_load_weights: copying a layer's weights failed");
+        rc = OCRHIP_EHIP;
+    }
+    if (rc == OCRHIP_OK) rc = launch_quantize_fp8(src.ptr, OCRHIP_F32, cout, cin, cin, 128, false, L.w_fp8.as<uint8_t>(), ld, L.s_fp8.as<uint8_t>(), ld_scale, nullptr);
+    // forward calls may run on streams that do not wait for the default one
+    if (rc == OCRHIP_OK && hipStreamSynchronize(nullptr) != hipSuccess) {
+        set_error("crnn_load_weights: quantising a layer's weights failed");
+        rc = OCRHIP_EHIP;
+    }
+    src.release();
+    return rc;
+}
+
 int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n) {
     OCR_HANDLE(h);
     OCR_REQUIRE(w && n > 0, "crnn_load_weights: no tensors");
@@ -703,6 +728,7 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
                     std::copy(wih + (size_t)(gq * Hd + u) * in_c, wih + (size_t)(gq * Hd + u + 1) * in_c, wperm.begin() + (size_t)(u * 4 + gq) * in_c);
                 }
             OCR_TRY(prepare_conv_mfma(net.wih[l][d], wperm.data(), bsum.data(), 4 * Hd, in_c, 1));
+            OCR_TRY(prepare_dense_fp8(net.wih[l][d], wperm.data(), 4 * Hd, in_c));
             OCR_TRY(net.whh[l][d].reserve((size_t)4 * Hd * Hd * sizeof(float)));
             OCR_HIP_CHECK(hipMemcpy(net.whh[l][d].ptr, whh, (size_t)4 * Hd * Hd * sizeof(float), hipMemcpyHostToDevice));
         }
@@ -710,6 +736,7 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
         OCR_TRY(get(W, pre + ".linear.weight", {Hd, 2 * Hd}, &lw));
         OCR_TRY(get(W, pre + ".linear.bias", {Hd}, &lb));
         OCR_TRY(prepare_conv_mfma(net.linear[l], lw, lb, Hd, 2 * Hd, 1));
+        OCR_TRY(prepare_dense_fp8(net.linear[l], lw, Hd, 2 * Hd));
     }
     {
         const ocrhip_tensor_desc* t = W.find("Prediction.weight");
@@ -719,6 +746,7 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
         const float* pb = nullptr;
         OCR_TRY(get(W, "Prediction.bias", {V}, &pb));
         OCR_TRY(prepare_conv_mfma(net.pred, t->data, pb, V, Hd, 1));
+        OCR_TRY(prepare_dense_fp8(net.pred, t->data, V, Hd));
         net.vocab = V;
         net.vocab_pad = net.pred.cout_pad;
     }
@@ -942,8 +970,19 @@ static int crnn_features16(CrnnNet& net, DevBuf* act, const float* x, int n, int
     return OCRHIP_OK;
 }
 
+// R rows of `cols` bfloat16 values -> net.in8, a scale per row and 128 columns
+static int crnn_quantize_rows(CrnnNet& net, const uint16_t* x, int64_t R, int cols, hipStream_t s) {
+    return launch_quantize_fp8(x, OCRHIP_BF16, R, cols, cols, 1, false, net.in8.as<uint8_t>(), fp8_ld(cols), net.in8_scale.as<uint8_t>(), fp8_ld_scale(R), s);
+}
+// out = (net.in8) W^T + bias
+static int crnn_dense_fp8(CrnnNet& net, const ConvLayer& L, void* out, bool out_f32, int64_t R, hipStream_t s) {
+    const Fp8Operand a{net.in8.as<uint8_t>(), net.in8_scale.as<uint8_t>(), fp8_ld(L.cin), fp8_ld_scale(R)};
+    const Fp8Operand b{L.w_fp8.as<uint8_t>(), L.s_fp8.as<uint8_t>(), fp8_ld(L.cin), fp8_ld_scale((L.cout + 127) / 128)};
+    return launch_gemm_fp8(a, b, 128, R, L.cout, L.cin, L.bias.as<float>(), out, out_f32 ? OCRHIP_F32 : OCRHIP_BF16, L.cout, net.ws8.ptr, s);
+}
+
 static int crnn_sequence16(CrnnNet& net, const uint16_t* feats16, int n, int64_t R, int Tmax, const int* host_T,
-                           const int* d_T, const int* d_row0, const int* d_active, float* logits, hipStream_t s) {
+                           const int* d_T, const int* d_row0, const int* d_active, float* logits, bool fp8, hipStream_t s) {
     const int Hd = net.hidden;
     OCR_REQUIRE(R < (1ll << 31), "crnn: too many time steps in one batch");
     OCR_TRY(net.xw.reserve((size_t)2 * R * 4 * Hd * sizeof(float)));
@@ -952,6 +991,14 @@ static int crnn_sequence16(CrnnNet& net, const uint16_t* feats16, int n, int64_t
     OCR_TRY(net.seq.reserve((size_t)R * 2 * Hd * sizeof(float)));
     OCR_TRY(net.lin.reserve((size_t)2 * R * Hd * sizeof(float)));
     OCR_TRY(net.seq16.reserve((size_t)R * 2 * Hd * sizeof(uint16_t)));
+    if (fp8) {
+        const int64_t widest = fp8_ld(std::max(2 * Hd, net.feat_c));
+        OCR_TRY(net.in8.reserve((size_t)R * widest));
+        OCR_TRY(net.in8_scale.reserve((size_t)(widest / 128) * fp8_ld_scale(R)));
+        size_t ws = 0;
+        for (const ConvLayer* L : {&net.wih[0][0], &net.wih[1][0], &net.linear[0], &net.pred}) ws = std::max(ws, gemm_fp8_workspace(R, L->cout, L->cin));
+        if (ws) OCR_TRY(net.ws8.reserve(ws));
+    }
     if (!net.lstm_counters.ptr) {
         OCR_TRY(net.lstm_counters.reserve((kLstmCounterCount + kLstmErrorWords) * sizeof(unsigned)));
         OCR_HIP_CHECK(hipMemsetAsync(net.lstm_counters.ptr, 0, (kLstmCounterCount + kLstmErrorWords) * sizeof(unsigned), s));
@@ -966,8 +1013,14 @@ static int crnn_sequence16(CrnnNet& net, const uint16_t* feats16, int n, int64_t
     for (int l = 0; l < 2; ++l) {
         float* xw_f = net.xw.as<float>();
         float* xw_b = xw_f + (size_t)R * 4 * Hd;
-        OCR_TRY(launch_gemm_bf16t(net.wih[l][0], layer_in, xw_f, true, R, 0, 0, 0, false, s));
-        OCR_TRY(launch_gemm_bf16t(net.wih[l][1], layer_in, xw_b, true, R, 0, 0, 0, false, s));
+        if (fp8) {
+            OCR_TRY(crnn_quantize_rows(net, layer_in, R, net.wih[l][0].cin, s));
+            OCR_TRY(crnn_dense_fp8(net, net.wih[l][0], xw_f, true, R, s));
+            OCR_TRY(crnn_dense_fp8(net, net.wih[l][1], xw_b, true, R, s));
+        } else {
+            OCR_TRY(launch_gemm_bf16t(net.wih[l][0], layer_in, xw_f, true, R, 0, 0, 0, false, s));
+            OCR_TRY(launch_gemm_bf16t(net.wih[l][1], layer_in, xw_b, true, R, 0, 0, 0, false, s));
+        }
         {
             ProfScope prof("lstm_layer16(T steps)", 2.0 * 2 * 4.0 * Hd * Hd * (double)(R - n),
                            4.0 * (2.0 * R * 4 * Hd) + 2.0 * (double)R * 2 * Hd + 2.0 * 2 * 4 * Hd * Hd * Tmax, s);
@@ -992,11 +1045,21 @@ static int crnn_sequence16(CrnnNet& net, const uint16_t* feats16, int n, int64_t
             }
         }
         uint16_t* lin = net.lin.as<uint16_t>() + (size_t)l * R * Hd;
-        OCR_TRY(launch_gemm_bf16t(net.linear[l], seq16, lin, false, R, 0, 0, 0, false, s));
+        if (fp8) {
+            OCR_TRY(crnn_quantize_rows(net, seq16, R, 2 * Hd, s));
+            OCR_TRY(crnn_dense_fp8(net, net.linear[l], lin, false, R, s));
+        } else {
+            OCR_TRY(launch_gemm_bf16t(net.linear[l], seq16, lin, false, R, 0, 0, 0, false, s));
+        }
         record(net.taps, l == 0 ? "seq0" : "seq1", lin, 1, R, Hd, 1, true);
         layer_in = lin;
     }
-    OCR_TRY(launch_gemm_bf16t(net.pred, layer_in, logits, true, R, 0, 0, 0, false, s));
+    if (fp8) {
+        OCR_TRY(crnn_quantize_rows(net, layer_in, R, Hd, s));
+        OCR_TRY(crnn_dense_fp8(net, net.pred, logits, true, R, s));
+    } else {
+        OCR_TRY(launch_gemm_bf16t(net.pred, layer_in, logits, true, R, 0, 0, 0, false, s));
+    }
     if (net.calls_started - net.calls_checked >= (uint64_t)CrnnNet::kErrSlots) {
         OCR_HIP_CHECK(hipStreamSynchronize(s));
         OCR_TRY(crnn_report_timeout(net, s));
@@ -1047,7 +1110,7 @@ int ocrhip_crnn_forward(ocrhip_handle h, const void* d_crops, int n, int Wpad, i
             OCR_TRY(net.logits.reserve((size_t)R * net.vocab * sizeof(float)));
             lg = net.logits.as<float>();
         }
-        OCR_TRY(crnn_sequence16(net, feats16, n, R, T, nullptr, nullptr, nullptr, nullptr, lg, s));
+        OCR_TRY(crnn_sequence16(net, feats16, n, R, T, nullptr, nullptr, nullptr, nullptr, lg, h->fp8_dense != 0, s));
         if (d_tokens) OCR_TRY(launch_ctc_greedy(lg, n, T, net.vocab, net.vocab, nullptr, nullptr, 0, d_tokens, d_scores, s));
         return OCRHIP_OK;
     }
@@ -1175,7 +1238,7 @@ int ocrhip_crnn_forward_packed(ocrhip_handle h, const void* d_packed, const int*
             OCR_TRY(net.logits.reserve((size_t)R * net.vocab * sizeof(float)));
             lg = net.logits.as<float>();
         }
-        OCR_TRY(crnn_sequence16(net, net.feats.as<uint16_t>(), n, R, Tmax, meta.data(), d_T, d_row0, d_active, lg, s));
+        OCR_TRY(crnn_sequence16(net, net.feats.as<uint16_t>(), n, R, Tmax, meta.data(), d_T, d_row0, d_active, lg, h->fp8_dense != 0, s));
         if (d_tokens) OCR_TRY(launch_ctc_greedy(lg, n, t_stride, net.vocab, net.vocab, d_T, d_row0, 0, d_tokens, d_scores, s));
         return OCRHIP_OK;
     }
@@ -1448,6 +1511,11 @@ int ocrhip_set_option(ocrhip_handle h, const char* name, int value) {
     if (std::strcmp(name, "bf16_tensors") == 0) {
         OCR_REQUIRE(value == 0 || value == 1, "set_option: bf16_tensors is 0 or 1");
         h->bf16_tensors = value;
+        return OCRHIP_OK;
+    }
+    if (std::strcmp(name, "fp8_dense") == 0) {
+        OCR_REQUIRE(value == 0 || value == 1, "set_option: fp8_dense is 0 or 1");
+        h->fp8_dense = value;
         return OCRHIP_OK;
     }
     if (std::strcmp(name, "flat_gemm") == 0) {

@@ -117,6 +117,7 @@ struct ConvLayer {
     DevBuf w_wino4;         // the same layers: F(4x4,3x3)-transformed filters (see conv_wino4.hip)
     DevBuf w_wino4c;        // of those, layers with a multiple of 128 output channels: the layout of its MODE 4
     DevBuf w_wino4b;        // layers with < 256 input channels: the same filters in the layout of that kernel's MODE 3
+    DevBuf w_fp8, s_fp8;    // the recogniser's dense layers: e4m3 bytes and scales of 128 x 128 blocks (see fp8.hip)
     DevBuf bias;            // cout_pad floats, folded
     DevBuf w_gemm, bias_gemm;   // 1x1 and 2x2 layers: slabs and bias for the 256 x 128 flat GEMM (see gemm_f32.hip)
     bool direct = false;    // small-Cin direct kernel layout
@@ -165,6 +166,7 @@ struct CrnnNet {
     hipEvent_t aux_fork = nullptr, aux_join[kAux] = {nullptr, nullptr, nullptr};
     DevBuf feats, xw, hbuf, cbuf, seq, lin, logits, meta, lstm_counters;
     DevBuf seq16;            // bfloat16-tensor path: output rows of a BiLSTM layer (R, 2H)
+    DevBuf in8, in8_scale, ws8;  // option fp8_dense: a dense layer's quantised input rows and their scales; the product's workspace
     DevBuf pmax, pidx;       // greedy decoding without logits: per row and block of 128 classes the maximum and its class
     static constexpr int kErrSlots = 16;
     static constexpr unsigned kErrPending = 0xFFFFFFFFu;
@@ -200,6 +202,7 @@ struct ocrhip_ctx {
     ocrhip::DevBuf wino_ws;        // transformed tiles of the layer in flight
     int fuse_mean_rows = 1;        // float32 recogniser: the mean over the feature rows in the epilogue of the extractor's last convolution (1) or as a kernel of its own (0)
     int fuse_ctc = 1;              // tokens without a logits request: class layer reduced to per-block maxima in its epilogue (1) or logits written and re-read (0)
+    int fp8_dense = 0;             // bfloat16-tensor recogniser: dense layers as 8-bit block-scaled products (1) or on bfloat16 operands (0)
     int bf16_tensors = 1;          // compute_dtype = OCRHIP_BF16: bfloat16 activations in HBM, tile kernels, bfloat16 recurrence (1); or the float32-tensor kernels with operands rounded on their way into LDS and a float32 recurrence (0)
     int flat_gemm = 1;             // 1x1 / 2x2 layers on the 256 x 128 flat GEMM (1) or on the implicit-GEMM convolution kernel (0)
     ocrhip::Profiler prof;

@@ -146,7 +146,9 @@ class HipContext:
         'wino4_split': 0 (default) every F(4x4,3x3) layer fused, 1 layers with >= 512 input channels as transform kernel +
         multiply kernel.
         'flat_gemm': 1 (default) Dense layers / LSTM input projections / 2x2 convolutions on the 256 x 128 flat GEMM,
-        0 on the implicit-GEMM convolution kernel."""
+        0 on the implicit-GEMM convolution kernel.
+        'fp8_dense': 1 the dense layers of the bfloat16 recogniser as 8-bit block-scaled products (logits within 0.2 of the
+        bfloat16 ones in norm), 0 (default) on bfloat16 operands."""
         check(self.lib.ocrhip_set_option(self._h, name.encode(), int(value)))
         self.options[name] = int(value)
 
