@@ -252,13 +252,21 @@ __device__ __forceinline__ double log64(double x) {
 // log of a sum of exponentials, which may be 0 or infinite
 __device__ __forceinline__ double log_sum(double x) { return x == 0.0 ? -INFINITY : x == INFINITY ? x : log64(x); }
 
+constexpr int kShort = 128;            // classes of a row that 16 lanes share
+
+// what one lane wrote to LDS is what another reads: same wave, so the order of the instructions is enough
+__device__ __forceinline__ void lds_phase() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- top logits
 //
-// Bound by reading the logits once.  Rows of up to 128 classes and 16 entries: 16 lanes per row, the maximum taken away K
-// times.  Longer rows: the K-th largest of the lanes' own maxima is a lower bound of the K-th largest of all (K lanes hold
-// a value that large), and hardly more than K values reach it: it is found by bisection of its leading bits, the values
-// that reach it are put on a list in LDS and each finds its rank by counting the larger ones.  A row whose list overflows
-// (thousands of equal values) takes its maxima one by one.
+// Bound by reading the logits once.  Rows of up to 128 classes and 16 entries: 16 lanes per row (top16_kernel).  Longer rows:
+// the K-th largest of the lanes' own maxima is a lower bound of the K-th largest of all (K lanes hold a value that large),
+// and hardly more than K values reach it: it is found by bisection of its leading bits, the values that reach it are put on
+// a list in LDS and each finds its rank by counting the larger ones.  A row whose list overflows (hundreds of equal values)
+// takes its maxima one by one.
 template <class T>
 struct TopArgs {
     const T* x;
@@ -270,60 +278,88 @@ struct TopArgs {
     float* lse;
 };
 
+// Every lane sorts its 8 classes, the lists go to LDS, and the K largest of the row are K times the largest head of 16 lists;
+// the winner writes its class down and moves on.  Bound by the vector ALU: the next row's loads are on their way, and a
+// logit's key with its class (7 bits; among equals the lower class counts as the larger) is held as the bits of a float64
+// between 1 and 2, which order like the numbers: two instructions sort a pair.
+__device__ __forceinline__ double entry_of(unsigned key, unsigned at) {
+    return __hiloint2double((int)(0x3FF00000u | key >> 12), (int)(key << 20 | (127u - at) << 13));
+}
+__device__ __forceinline__ unsigned entry_key(unsigned hi, unsigned lo) { return hi << 12 | lo >> 20; }
+__device__ __forceinline__ unsigned entry_class(unsigned lo) { return 127u - (lo >> 13 & 127u); }
+
 template <class T, bool TINY>
 __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
-    constexpr int P = kPiece<T>, N = 128 / 16 / P;
-    const int part = threadIdx.x & 15;
-    for (int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); row < a.rows; row += (int64_t)gridDim.x * 16) {
-        const T* p = a.x + row * a.ld;
-        uintx4 raw[N];
-        float v[N][P];
-        unsigned key[N][P];
-        unsigned best = 0, at = 0xFFFFFFFFu;
+    constexpr int P = kPiece<T>, L = kShort / 16, N = L / P;
+    __shared__ double lists[L][256];                       // from the third on; two entries below all behind the last
+    __shared__ double found[16][16];                       // per row
+    const int tid = threadIdx.x, part = tid & 15, sub = tid >> 4;
+    const float c = a.inv_t * kLog2e;
+    const int64_t step = (int64_t)gridDim.x * 16;
+    uintx4 next[N];
+    auto fetch = [&](int64_t row) {
+        const T* p = a.x + min(row, a.rows - 1) * a.ld;
 #pragma unroll
-        for (int i = 0; i < N; ++i) raw[i] = load_raw<TINY>(p, part + 16 * i, a.V);
+        for (int i = 0; i < N; ++i) next[i] = load_raw<TINY>(p, part + 16 * i, a.V);
+    };
+    int64_t row = (int64_t)blockIdx.x * 16 + sub;
+    fetch(row);
+    lists[L - 2][tid] = 1.0;
+    lists[L - 1][tid] = 1.0;
+    for (int64_t first_row = (int64_t)blockIdx.x * 16; first_row < a.rows; first_row += step, row += step) {
+        float v[L];
+        double own[L];
 #pragma unroll
-        for (int i = 0; i < N; ++i) unpack_piece(in_place<TINY>(raw[i], p, part + 16 * i, a.V), v[i]);
+        for (int i = 0; i < N; ++i) {
+            float w[P];
+            unpack_piece(in_place<TINY>(next[i], a.x, part + 16 * i, a.V), w);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int e = 0; e < P; ++e) key[i][e] = (part + 16 * i) * P + e < a.V ? order_key(v[i][e]) : 0u;
-        float high = 0.0f;
-        for (int k = 0; k < a.K; ++k) {
-            best = 0;
-            at = 0xFFFFFFFFu;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int e = 0; e < P; ++e)
-                    if (key[i][e] > best) {
-                        best = key[i][e];
-                        at = (part + 16 * i) * P + e;
-                    }
-            const unsigned top = group_max<16>(best);
-            const unsigned where = group_min<16>(best == top ? at : 0xFFFFFFFFu);
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int e = 0; e < P; ++e)
-                    if ((unsigned)((part + 16 * i) * P + e) == where) key[i][e] = 0;
-            if (k == 0) high = key_value(top);
-            if (part == 0) {
-                a.values[row * a.K + k] = key_value(top);
-                a.index[row * a.K + k] = (int)where;
+            for (int e = 0; e < P; ++e) {
+                const unsigned at = (unsigned)((part + 16 * i) * P + e);
+                v[i * P + e] = w[e];
+                own[i * P + e] = at < (unsigned)a.V ? entry_of(order_key(w[e]), at) : 1.0;
             }
         }
+        fetch(row + step);
+        constexpr int order[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
+                                      {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+        for (int i = 0; i < 19; ++i) {
+            const double x = own[order[i][0]], y = own[order[i][1]];
+            own[order[i][0]] = __builtin_fmax(x, y);
+            own[order[i][1]] = __builtin_fmin(x, y);
+        }
+#pragma unroll
+        for (int i = 2; i < L; ++i) lists[i - 2][tid] = own[i];
+        unsigned hi = (unsigned)__double2hiint(own[0]), lo = (unsigned)__double2loint(own[0]);
+        double second = own[1];
+        const double* behind = &lists[0][tid];
+        for (int k = 0; k < a.K; ++k) {                    // K <= V: some head is a class
+            const unsigned top = group_max<16>(hi), which = group_max<16>(hi == top ? lo : 0u);
+            if (hi == top && lo == which) {
+                found[sub][k] = __hiloint2double((int)hi, (int)lo);
+                hi = (unsigned)__double2hiint(second);
+                lo = (unsigned)__double2loint(second);
+                second = *behind;
+                behind += 256;
+            }
+        }
+        lds_phase();
         if (a.lse) {
-            const float c = a.inv_t * kLog2e;
+            const float high = key_value(entry_key((unsigned)__double2hiint(found[sub][0]), (unsigned)__double2loint(found[sub][0])));
             const float base = fabsf(high) == INFINITY || high != high ? 0.0f : high;
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int e = 0; e < P; ++e) sum += __builtin_amdgcn_exp2f((v[i][e] - base) * c);
+            for (int i = 0; i < L; ++i) sum += __builtin_amdgcn_exp2f((v[i] - base) * c);
             sum = group_sum<16>(sum);
-            if (part == 0) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)sum));
+            if (part == 0 && row < a.rows) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)sum));
         }
+        if (part < a.K && row < a.rows) {
+            const unsigned h = (unsigned)__double2hiint(found[sub][part]), l = (unsigned)__double2loint(found[sub][part]);
+            a.values[row * a.K + part] = key_value(entry_key(h, l));
+            a.index[row * a.K + part] = (int)entry_class(l);
+        }
+        lds_phase();
     }
 }
 
@@ -332,13 +368,6 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
 constexpr size_t kWaveBytes = 16384, kRowBytes = 32768;
 constexpr int kTopList = 512;          // candidates of a row that LDS holds
 
-// what one lane wrote to LDS is what another reads: same wave, so the order of the instructions is enough
-__device__ __forceinline__ void lds_phase() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-}
-
-constexpr int kShort = 128;            // classes of a row that 16 lanes share
 // The row to LDS, BATCH pieces of a lane in flight (pieces of 16 bytes; classes behind the last are -infinity); returns the lane's maximum.  `between` runs
 // while the first pieces are on their way.
 template <int THREADS, int BATCH, bool TINY, class T, class F>
@@ -1043,7 +1072,7 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
     constexpr int P = kPiece<T>;
     const size_t row_lds = (size_t)(a.V + P - 1) / P * 16;
-    const unsigned groups = (unsigned)std::min((a.rows + 15) / 16, kMaxGrid);
+    const unsigned groups = (unsigned)std::min<int64_t>((a.rows + 15) / 16, 2048);          // 8 per compute unit, which walk the rows
     if (a.V < P)                       // K <= V
         hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
     else if (a.V <= kShort && a.K <= 16)
