@@ -367,7 +367,9 @@ int ocrhip_ctc_beam_search(ocrhip_handle h, const float* d_logits, int B, int T,
  * Operators for a recogniser whose dense layers multiply 8-bit floating point blocks, and for the distance of such a
  * (student's) logits from the float32 recogniser's (teacher's).  No counterpart in the reference.  All of them check
  * their arguments before anything else, allocate nothing, keep nothing of the handle's between calls (two calls on two
- * streams, or in two captured graphs, share no memory) and leave the current device as it was.
+ * streams, or in two captured graphs, share no memory) and leave the current device as it was.  An output or workspace that
+ * shares memory with an input or another output is refused; matrices side by side in one buffer, columns of the same rows,
+ * share none.
  *
  * Block-scaled 8-bit matrix of R rows and C columns: row r at d_q + r * ld_q, OCP e4m3 bytes (8 bits, no infinities),
  * the columns from C up to the next multiple of 128 zero; the scale of the block (row block i, column block j) is the
@@ -381,7 +383,7 @@ int ocrhip_ctc_beam_search(ocrhip_handle h, const float* d_logits, int B, int T,
  *   d_x    : device float32 or bfloat16 (x_dtype), row r at d_x + r * ld_x elements
  *   d_q    : (R, ld_q) bytes with R = transpose ? cols : rows; every row is written up to its columns rounded up to 128
  *   d_scale: (ceil(C / 128), ld_scale) bytes, the first ceil(R / block_rows) of a row are written
- * rows == 0 or cols == 0: nothing is written. */
+ * rows == 0 or cols == 0: nothing is written.  From about 2^28 rows on the grid is too large, an error. */
 int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x,
                         int block_rows, int transpose, uint8_t* d_q, int64_t ld_q, uint8_t* d_scale, int64_t ld_scale,
                         ocrhip_stream stream);

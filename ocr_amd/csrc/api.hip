@@ -1295,11 +1295,15 @@ struct DeviceScope {
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-// one past the last byte of `rows` rows of `row_bytes` bytes, `ld_bytes` apart
+// whether two matrices of rows of `row` bytes, `ld` bytes apart, share a byte: their whole extents do, unless rows of the same
+// stride lie side by side (columns of one buffer)
 bool overlap(const void* a, int64_t a_rows, int64_t a_ld, int64_t a_row, const void* b, int64_t b_rows, int64_t b_ld, int64_t b_row) {
-    if (!a || !b || a_rows == 0 || b_rows == 0) return false;
+    if (!a || !b || a_rows == 0 || b_rows == 0 || a_row == 0 || b_row == 0) return false;
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
-    return a0 < b0 + (uintptr_t)((b_rows - 1) * b_ld + b_row) && b0 < a0 + (uintptr_t)((a_rows - 1) * a_ld + a_row);
+    if (!(a0 < b0 + (uintptr_t)((b_rows - 1) * b_ld + b_row) && b0 < a0 + (uintptr_t)((a_rows - 1) * a_ld + a_row))) return false;
+    if (a_ld != b_ld || a_ld <= 0) return true;
+    const int64_t apart = (int64_t)(b0 - a0), d = (apart % a_ld + a_ld) % a_ld;
+    return d < a_row || d + b_row > a_ld;
 }
 
 constexpr int64_t kMaxDepth = 1ll << 22;         // K of a product, and the row strides of its operands: 256 rows stay within 31 bits
@@ -1342,6 +1346,19 @@ int check_product(const char* who, int64_t M, int64_t N, int64_t K, const float*
     return OCRHIP_OK;
 }
 
+// a product's output and workspace share no memory with its inputs or with each other (a: rows of any type)
+int check_apart(const char* who, const void* c, int64_t M, int64_t c_ld, int64_t c_row, const void* ws, size_t ws_bytes, const void* a, int64_t a_rows, int64_t a_ld, int64_t a_row,
+                const uint8_t* a_scale, int64_t ld_as, const uint8_t* b, int64_t ld_b, const uint8_t* b_scale, int64_t ld_bs, int64_t b_blocks, int64_t N, int64_t K, const float* bias) {
+    const int64_t kb = (K + 127) / 128;
+    const struct { const void* p; int64_t rows, ld, row; } in[5] = {{a, a_rows, a_ld, a_row}, {a_scale, kb, ld_as, M}, {b, N, ld_b, kb * 128}, {b_scale, kb, ld_bs, b_blocks}, {bias, 1, 0, N * 4}};
+    const int64_t ws_rows = ws_bytes ? 1 : 0;
+    for (const auto& i : in)
+        OCR_REQUIRE(!overlap(c, M, c_ld, c_row, i.p, i.rows, i.ld, i.row) && !overlap(ws, ws_rows, 0, (int64_t)ws_bytes, i.p, i.rows, i.ld, i.row),
+                    "%s: the output or the workspace overlaps an input", who);
+    OCR_REQUIRE(!overlap(c, M, c_ld, c_row, ws, ws_rows, 0, (int64_t)ws_bytes), "%s: the output overlaps the workspace", who);
+    return OCRHIP_OK;
+}
+
 int check_rows(const char* who, const void* x, int dtype, int64_t rows, int V, int64_t ld, int K, float temperature) {
     OCR_REQUIRE(V >= 1 && V <= 262144, "%s: %d classes (1 .. 262144)", who, V);
     OCR_REQUIRE(K >= 1 && K <= 64, "%s: %d entries per row (1 .. 64)", who, K);
@@ -1376,12 +1393,8 @@ int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uin
     OCR_TRY(check_product("gemm_fp8", M, N, K, d_bias, d_c, c_dtype, ld_c, d_ws, ws_bytes, ocrhip_gemm_fp8_workspace(M, N, K)));
     OCR_TRY(check_blocks("gemm_fp8", "a", d_a, ld_a, d_a_scale, ld_a_scale, 1, M, K, true));
     OCR_TRY(check_blocks("gemm_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K, true));
-    const int64_t c_ld = ld_c * esize(c_dtype), c_row = N * esize(c_dtype), kb = (K + 127) / 128;
-    OCR_REQUIRE(!overlap(d_c, M, c_ld, c_row, d_a, M, ld_a, K) && !overlap(d_c, M, c_ld, c_row, d_b, N, ld_b, K) &&
-                    !overlap(d_c, M, c_ld, c_row, d_a_scale, kb, ld_a_scale, M) && !overlap(d_c, M, c_ld, c_row, d_b_scale, kb, ld_b_scale, (N + b_block_rows - 1) / b_block_rows) &&
-                    !overlap(d_c, M, c_ld, c_row, d_bias, d_bias ? 1 : 0, 0, N * 4) &&
-                    !overlap(d_c, M, c_ld, c_row, d_ws, ws_bytes ? 1 : 0, 0, (int64_t)ws_bytes),
-                "gemm_fp8: the output overlaps an input or the workspace");
+    OCR_TRY(check_apart("gemm_fp8", d_c, M, ld_c * esize(c_dtype), N * esize(c_dtype), d_ws, ws_bytes, d_a, M, ld_a, round_up(K, 128), d_a_scale, ld_a_scale, d_b, ld_b, d_b_scale,
+                        ld_b_scale, (N + b_block_rows - 1) / b_block_rows, N, K, d_bias));
     OCR_OPERATOR(h);
     return launch_gemm_fp8(Fp8Operand{d_a, d_a_scale, ld_a, ld_a_scale}, Fp8Operand{d_b, d_b_scale, ld_b, ld_b_scale}, b_block_rows, M, N, K, d_bias,
                            d_c, c_dtype, ld_c, d_ws, (hipStream_t)stream);
@@ -1399,12 +1412,8 @@ int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_
     OCR_TRY(check_values("linear_fp8", "x", d_x, x_dtype, M, K, ld_x));
     OCR_TRY(check_product("linear_fp8", M, N, K, d_bias, d_c, c_dtype, ld_c, d_ws, ws_bytes, ocrhip_linear_fp8_workspace(M, N, K)));
     OCR_TRY(check_blocks("linear_fp8", "b", d_b, ld_b, d_b_scale, ld_b_scale, b_block_rows, N, K, true));
-    const int64_t c_ld = ld_c * esize(c_dtype), c_row = N * esize(c_dtype), x_ld = ld_x * esize(x_dtype), x_row = K * esize(x_dtype), kb = (K + 127) / 128;
-    OCR_REQUIRE(!overlap(d_c, M, c_ld, c_row, d_x, M, x_ld, x_row) && !overlap(d_c, M, c_ld, c_row, d_b, N, ld_b, K) &&
-                    !overlap(d_c, M, c_ld, c_row, d_b_scale, kb, ld_b_scale, (N + b_block_rows - 1) / b_block_rows) && !overlap(d_c, M, c_ld, c_row, d_bias, d_bias ? 1 : 0, 0, N * 4) &&
-                    !overlap(d_c, M, c_ld, c_row, d_ws, ws_bytes ? 1 : 0, 0, (int64_t)ws_bytes) &&
-                    !overlap(d_x, M, x_ld, x_row, d_ws, ws_bytes ? 1 : 0, 0, (int64_t)ws_bytes),
-                "linear_fp8: the output or the workspace overlaps an input");
+    OCR_TRY(check_apart("linear_fp8", d_c, M, ld_c * esize(c_dtype), N * esize(c_dtype), d_ws, ws_bytes, d_x, M, ld_x * esize(x_dtype), K * esize(x_dtype), nullptr, 0, d_b, ld_b, d_b_scale,
+                        ld_b_scale, (N + b_block_rows - 1) / b_block_rows, N, K, d_bias));
     OCR_OPERATOR(h);
     if (M == 0 || N == 0) return OCRHIP_OK;
     if (linear_fp8_fits_rows(M))
@@ -1412,6 +1421,7 @@ int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_
     uint8_t* q = reinterpret_cast<uint8_t*>(d_ws);
     const int64_t ld_q = round_up(K, 128), ld_s = round_up(M, 16);
     uint8_t* sc = q + M * ld_q;
+    const int64_t kb = (K + 127) / 128;
     OCR_TRY(launch_quantize_fp8(d_x, x_dtype, M, K, ld_x, 1, false, q, ld_q, sc, ld_s, (hipStream_t)stream));
     return launch_gemm_fp8(Fp8Operand{q, sc, ld_q, ld_s}, Fp8Operand{d_b, d_b_scale, ld_b, ld_b_scale}, b_block_rows, M, N, K, d_bias, d_c, c_dtype,
                            ld_c, sc + kb * ld_s, (hipStream_t)stream);
@@ -1423,6 +1433,13 @@ int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t 
     OCR_REQUIRE(K <= V, "top_logits: %d of %d classes", K, V);
     OCR_REQUIRE(rows == 0 || (d_values && d_index), "top_logits: null output");
     OCR_REQUIRE(aligned(d_values, 4) && aligned(d_index, 4) && aligned(d_lse, 4), "top_logits: an output is not aligned to its elements");
+    const int64_t list = (int64_t)K * 4, e = esize(dtype);
+    const struct { const void* p; int64_t row; } out[3] = {{d_values, list}, {d_index, list}, {d_lse, 4}};
+    for (int i = 0; i < 3; ++i) {
+        OCR_REQUIRE(!overlap(out[i].p, rows, out[i].row, out[i].row, d_logits, rows, ld * e, V * e), "top_logits: an output overlaps the logits");
+        for (int j = 0; j < i; ++j)
+            OCR_REQUIRE(!overlap(out[i].p, 1, 0, rows * out[i].row, out[j].p, 1, 0, rows * out[j].row), "top_logits: two outputs overlap");
+    }
     OCR_OPERATOR(h);
     return launch_top_logits(d_logits, dtype, rows, V, ld, K, temperature, d_values, d_index, d_lse, (hipStream_t)stream);
 }
@@ -1435,11 +1452,14 @@ int ocrhip_distill_loss(ocrhip_handle h, const void* d_logits, int dtype, int64_
     OCR_REQUIRE(rows == 0 || (d_top_values && d_top_index), "distill_loss: the teacher's entries are null");
     OCR_REQUIRE(aligned(d_top_values, 4) && aligned(d_top_index, 4) && aligned(d_top_lse, 4) && aligned(d_row_weight, 4) && aligned(d_loss, 4),
                 "distill_loss: a buffer is not aligned to its elements");
-    if (d_grad) {
-        OCR_TRY(check_values("distill_loss", "the gradient", d_grad, dtype, rows, V, ld_grad));
-        const int64_t e = esize(dtype);
-        OCR_REQUIRE(!overlap(d_grad, rows, ld_grad * e, V * e, d_logits, rows, ld * e, V * e), "distill_loss: the gradient overlaps the logits");
+    if (d_grad) OCR_TRY(check_values("distill_loss", "the gradient", d_grad, dtype, rows, V, ld_grad));
+    const int64_t list = (int64_t)K * 4, e = esize(dtype);
+    const struct { const void* p; int64_t ld, row; } in[5] = {{d_logits, ld * e, V * e}, {d_top_values, list, list}, {d_top_index, list, list}, {d_top_lse, 4, 4}, {d_row_weight, 4, 4}};
+    for (const auto& i : in) {
+        OCR_REQUIRE(!overlap(d_grad, rows, ld_grad * e, V * e, i.p, rows, i.ld, i.row), "distill_loss: the gradient overlaps an input");
+        OCR_REQUIRE(!overlap(d_loss, rows, 4, 4, i.p, rows, i.ld, i.row), "distill_loss: the loss overlaps an input");
     }
+    OCR_REQUIRE(!overlap(d_grad, rows, ld_grad * e, V * e, d_loss, rows, 4, 4), "distill_loss: the loss overlaps the gradient");
     OCR_OPERATOR(h);
     return launch_distill_loss(d_logits, dtype, rows, V, ld, d_top_values, d_top_index, K, d_top_lse, temperature, d_row_weight, d_loss, d_grad, ld_grad,
                                (hipStream_t)stream);

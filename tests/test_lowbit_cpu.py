@@ -161,6 +161,35 @@ def test_refusals_of_the_c_entries(name, over, part):
     assert rc == -1 and part in msg and msg.startswith(name), msg
 
 
+@pytest.mark.parametrize('name,over', [
+    ('gemm_fp8', dict(c=P + 9 * 256 + 200)),                   # the zeros behind the last row's columns
+    ('gemm_fp8', dict(M=500, ld_as=512, ws=P, c=60 * P)), ('gemm_fp8', dict(ws=16 * P + 64)), ('gemm_fp8', dict(ws=8 * P)), ('gemm_fp8', dict(ws=24 * P)),
+    ('gemm_fp8', dict(ws=32 * P)), ('linear_fp8', dict(ws=16 * P)), ('linear_fp8', dict(ws=32 * P)),
+    ('top_logits', dict(values=P + 64)), ('top_logits', dict(index=P + 64)), ('top_logits', dict(lse=P + 4 * 97 * 4 - 4)),
+    ('top_logits', dict(index=8 * P)), ('top_logits', dict(index=8 * P + 156)), ('top_logits', dict(lse=8 * P)), ('top_logits', dict(lse=16 * P + 8)),
+    ('distill_loss', dict(grad=8 * P)), ('distill_loss', dict(grad=16 * P + 40)), ('distill_loss', dict(grad=24 * P)), ('distill_loss', dict(lse=32 * P)),
+    ('distill_loss', dict(weight=32 * P)), ('distill_loss', dict(loss=P)), ('distill_loss', dict(loss=8 * P)), ('distill_loss', dict(loss=16 * P + 156)),
+    ('distill_loss', dict(weight=24 * P)), ('distill_loss', dict(lse=24 * P + 12)),
+    ('distill_loss', dict(ld=200, ld_grad=200, grad=P + 96 * 4)),
+])
+def test_outputs_that_share_memory_are_refused(name, over):
+    rc, msg = _call(name, **over)
+    assert rc == -1 and 'overlap' in msg and msg.startswith(name), msg
+
+
+@pytest.mark.parametrize('name,over', [
+    ('distill_loss', dict(ld=200, ld_grad=200, grad=P + 97 * 4)),            # logits and gradient side by side
+    ('distill_loss', dict(x=P + 103 * 4, ld=200, ld_grad=200, grad=P)),
+    ('linear_fp8', dict(ld_x=256, ld_c=256, c=P + 200 * 4)),
+    ('linear_fp8', dict(ld_x=256, ld_c=256, c=P - 7 * 4)),
+    ('top_logits', dict(lse=16 * P + 160)), ('top_logits', dict(index=8 * P + 160)),
+    ('gemm_fp8', dict(ld_a=384, ld_c=96, c=P + 256)),
+])
+def test_neighbours_in_one_buffer_are_no_overlap(name, over):
+    rc, msg = _call(name, **over)
+    assert rc == -1 and msg == 'null handle', msg
+
+
 def test_a_workspace_that_is_too_small_is_a_capacity_error():
     from ocr_amd import _lib
     need = _lib.load().ocrhip_linear_fp8_workspace(500, 7, 200)
