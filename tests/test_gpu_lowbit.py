@@ -232,6 +232,38 @@ def test_product_leaves_what_is_not_its_own(ctx):
             assert (out[m:] == -7).all() and (out[:, n:] == -7).all()
 
 
+# rows that start anywhere in a line, results that start anywhere, several tiles of a row per workgroup (2 and 14 for the last
+# two), few rows and columns, and whole lines: the same sums wherever they are put, and nothing beside them
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('block_rows', [1, 128])
+@pytest.mark.parametrize('mnk', [(65, 129, 128), (100, 160, 300), (129, 300, 128), (300, 520, 256), (200, 1000, 256), (130, 6719, 128),
+                                 (2000, 6719, 128), (17000, 6719, 64)])
+def test_product_lands_in_any_rows(ctx, mnk, block_rows, out_dtype):
+    import ctypes
+    from ocr_amd._lib import check
+    m, n, k = mnk
+    code, e = (0, 4) if out_dtype == torch.float32 else (1, 2)
+    a = ctx.quantize_fp8(torch.randn(m, k, generator=torch.Generator().manual_seed(m)).cuda())
+    w = ctx.quantize_fp8(torch.randn(n, k, generator=torch.Generator().manual_seed(n)).cuda(), block_rows=block_rows)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(k)).cuda()
+    ws_bytes = ctx.lib.ocrhip_gemm_fp8_workspace(m, n, k)
+    ws = torch.empty(max(1, ws_bytes), dtype=torch.uint8, device='cuda')
+
+    def run(ld, first):
+        buf = torch.full((first + (m + 1) * ld,), -7.0, dtype=out_dtype, device='cuda')
+        p = lambda t: ctypes.c_void_p(t.data_ptr())          # noqa: E731
+        check(ctx.lib.ocrhip_gemm_fp8(ctx._h, p(a.q), a.q.shape[1], p(a.scale), a.scale.shape[1], p(w.q), w.q.shape[1], p(w.scale), w.scale.shape[1],
+                                      block_rows, m, n, k, p(bias), ctypes.c_void_p(buf.data_ptr() + first * e), code, ld, p(ws), ws_bytes, ctx._on()))
+        rows = buf[first:].view(m + 1, ld)
+        assert (buf[:first] == -7).all() and (rows[m] == -7).all() and (rows[:, n:] == -7).all()
+        return rows[:m, :n]
+    whole = run(-(-n // 64) * 64, 0)
+    if m <= 300:
+        check_product(whole, a, w, bias, out_dtype)
+    for ld, first in ((n, 0), (n, 1), (n, 31), (n + 1, 0), (n + 3, 5), (-(-n // 64) * 64, 3)):
+        assert torch.equal(run(ld, first), whole), (ld, first)
+
+
 def test_product_beyond_32_bits(ctx):
     """A's bytes and C's elements lie beyond 2^31: the last rows equal those of a product of their own."""
     m, n, k = (1 << 24) + 300, 136, 128                       # A 2.1 GB, C 2.3 G elements (bfloat16)
