@@ -1402,7 +1402,7 @@ int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uin
 
 // workspace of linear_fp8: the quantised rows, their scales, then the product's own
 size_t ocrhip_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || linear_fp8_fits_rows(M)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || linear_fp8_fits_rows(M, K)) return 0;
     return (size_t)(M * round_up(K, 128) + (K + 127) / 128 * round_up(M, 16)) + gemm_fp8_workspace(M, N, K);
 }
 
@@ -1416,7 +1416,7 @@ int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_
                         ld_b_scale, (N + b_block_rows - 1) / b_block_rows, N, K, d_bias));
     OCR_OPERATOR(h);
     if (M == 0 || N == 0) return OCRHIP_OK;
-    if (linear_fp8_fits_rows(M))
+    if (linear_fp8_fits_rows(M, K))
         return launch_linear_fp8_rows(d_x, x_dtype, ld_x, Fp8Operand{d_b, d_b_scale, ld_b, ld_b_scale}, b_block_rows, M, N, K, d_bias, d_c, c_dtype, ld_c, (hipStream_t)stream);
     uint8_t* q = reinterpret_cast<uint8_t*>(d_ws);
     const int64_t ld_q = round_up(K, 128), ld_s = round_up(M, 16);

@@ -375,7 +375,7 @@ size_t gemm_fp8_workspace(int64_t M, int64_t N, int64_t K);
 int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* bias,
                     void* c, int c_dtype, int64_t ld_c, void* ws, hipStream_t s);
 //   a few rows of values, quantised by the product's kernel itself
-bool linear_fp8_fits_rows(int64_t M);
+bool linear_fp8_fits_rows(int64_t M, int64_t K);
 int launch_linear_fp8_rows(const void* x, int x_dtype, int64_t ld_x, const Fp8Operand& b, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* bias,
                            void* c, int c_dtype, int64_t ld_c, hipStream_t s);
 

@@ -321,8 +321,7 @@ __device__ __forceinline__ void store_c4(void* c, int64_t at, floatx4 v, int lef
 // of several blocks are in flight at once.  The waves_k partial sums meet in LDS, added in the order of the waves.
 // XT: type of A.  void: quantised operands.  float / uint16_t: values that the wave quantises itself - a lane holds 32
 // values of a row, the block's maximum is two lane exchanges away, and the bytes land in the registers the matrix
-// instruction reads - which saves linear_fp8 a launch; up to 32 rows, beyond that every wave's own quantisation costs more
-// than a launch of its own that does it once.
+// instruction reads - which saves linear_fp8 a launch (up to 32 rows, see linear_fp8_fits_rows).
 template <class XT, int IM, bool OUT_F32, int BROWS>
 __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k) {
     extern __shared__ float red[];               // [wave][IM][4][64]
@@ -706,13 +705,22 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
     }
 }
 
-// the partial sums of the splits, in their order, and the bias
-template <bool OUT_F32>
+// The partial sums of the splits, in their order, and the bias.  BATCH loads are in flight: 4 for few splits (more cost
+// occupancy: 6719 x 256 with 4 splits 72 us with the product, 76 with 16 in flight), 16 for many (65 x 64 with 64: 18 against
+// 31).
+template <bool OUT_F32, int BATCH>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const float* __restrict__ part, int splits, int64_t M, int N, const float* __restrict__ bias, void* c, int64_t ldc) {
     const int64_t count = M * N;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
         float v = part[i];
-        for (int z = 1; z < splits; ++z) v += part[z * count + i];
+        for (int z = 1; z < splits; z += BATCH) {
+            float t[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) t[u] = part[min(z + u, splits - 1) * count + i];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u)
+                if (z + u < splits) v += t[u];
+        }
         const int64_t m = i / N;
         const int n = (int)(i - m * N);
         store_c<OUT_F32>(c, m * ldc + n, v + (bias ? bias[n] : 0.0f));
@@ -747,6 +755,17 @@ struct TilePlan {
 };
 
 // Which tiles a product of M > kMaxRows rows takes, and into how many pieces of k it is split.
+//
+// Tiles of 256 x 256 (bfloat16 results; one workgroup per compute unit) read their operands half as often: from 192 tiles on
+// they win or are level (4096^3 67 us against 77 of 128 x 128, 131072 x 1024 x 256 67 against 77, 4096 x 3200 x 512 16 against
+// 15), below that they leave compute units idle (3000 x 3000 x 1024: 47 against 20).  float32 results need twice the
+// registers for the converted operands: 128 x 128 throughout.
+//
+// Pieces of k: a workgroup takes 1.05 us per block of k as long as it has its compute unit to itself and 1.6 us when two
+// share one; joining the pieces costs a launch, 2.5 us, and 0.27 us per MB of partial sums (written and read).  What comes
+// out least is taken, up to two workgroups per compute unit, for the 513th would make a second round of them all.  Measured
+// against one piece: 300 x 97 x 2048 10 us / 22, 256 x 256 x 131072 33 / 1087, 6719 x 256 x 16384 73 / 142; where one piece
+// stays, against two: 1900 x 1900 x 2048 26 / 32, 1000 x 1000 x 1024 14 / 16.
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
     TilePlan p;
     const int64_t nkb = (K + kBlk - 1) / kBlk;
@@ -757,12 +776,19 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
     p.tiles_m = (M + p.bm - 1) / p.bm;
     p.tiles_n = (N + p.bn - 1) / p.bn;
     const int64_t tiles = p.tiles_m * p.tiles_n;
-    int64_t splits = 1;
-    // few tiles, long k: pieces of k until the device is full (two workgroups on each of 256 compute units) and no further,
-    // for the 513th would make a second round of them all
-    if (tiles < 256 && nkb >= 8) splits = std::min<int64_t>(std::min<int64_t>(nkb / 4, 512 / tiles), 16);
-    p.kb_split = (int)((nkb + splits - 1) / splits);
-    p.splits = (int)((nkb + p.kb_split - 1) / p.kb_split);
+    p.splits = 1;
+    p.kb_split = (int)nkb;
+    double least = 1.05 * (double)nkb;
+    const int64_t most = large ? 1 : std::min<int64_t>(nkb, 512 / std::max<int64_t>(tiles, 1));
+    for (int64_t s = 2; s <= most; s += s < 4 ? 1 : s / 2) {
+        const int64_t per = (nkb + s - 1) / s, pieces = (nkb + per - 1) / per;
+        const double us = (pieces * tiles <= 256 ? 1.05 : 1.6) * (double)per + 2.5 + 0.27e-6 * 8.0 * (double)(pieces * M * N);
+        if (us < least) {
+            least = us;
+            p.splits = (int)pieces;
+            p.kb_split = (int)per;
+        }
+    }
     return p;
 }
 
@@ -795,8 +821,8 @@ int launch_rows_any(const GemmArgs& g, bool f32, int b_block_rows, hipStream_t s
     return f32 ? launch_rows<XT, true, kBlk>(g, s) : launch_rows<XT, false, kBlk>(g, s);
 }
 
-constexpr int kMaxRows = 64;          // gemm_rows_kernel: rows of A
-constexpr int kMaxOwnRows = 32;       // the same, quantising them itself
+// gemm_rows_kernel up to 64 rows of A (64 x 6719 x 256: 6.4 us against 7.3 of tiles, 64 x 1024 x 2048 9.7 against 11.5)
+constexpr int kMaxRows = 64;
 
 template <class T>
 int launch_quantize(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int block_rows, bool transpose, uint8_t* q, int64_t ld_q, uint8_t* scale,
@@ -881,16 +907,17 @@ int launch_gemm_fp8(const Fp8Operand& a, const Fp8Operand& b, int b_block_rows, 
     if (p.splits > 1) {
         ProfScope prof("gemm_fp8<join>", (double)p.splits * M * N, ((f32 ? 4.0 : 2.0) + 4.0 * p.splits) * (double)M * N, s);
         const dim3 grid((unsigned)std::min<int64_t>((M * N + 255) / 256, 4096));
-        if (f32)
-            hipLaunchKernelGGL(gemm_join_kernel<true>, grid, dim3(256), 0, s, t.part, p.splits, M, (int)N, bias, c, ld_c);
-        else
-            hipLaunchKernelGGL(gemm_join_kernel<false>, grid, dim3(256), 0, s, t.part, p.splits, M, (int)N, bias, c, ld_c);
+        auto join = f32 ? (p.splits > 16 ? &gemm_join_kernel<true, 16> : &gemm_join_kernel<true, 4>) : (p.splits > 16 ? &gemm_join_kernel<false, 16> : &gemm_join_kernel<false, 4>);
+        hipLaunchKernelGGL(join, grid, dim3(256), 0, s, t.part, p.splits, M, (int)N, bias, c, ld_c);
         OCR_HIP_CHECK(hipGetLastError());
     }
     return OCRHIP_OK;
 }
 
-bool linear_fp8_fits_rows(int64_t M) { return M <= kMaxOwnRows; }
+// Whether the kernel for few rows quantises them itself.  Up to 16 rows that saves the launch (1 x 6719 x 256: 3.8 us against
+// 5.5, 16 x 1024 x 2048 7.8 against 8.2); with 32 every wave quantises twice as much of each block, which costs more than the
+// launch when k is long (32 x 6719 x 256: 6.6 against 7.1; 32 x 1024 x 2048: 12.3 against 9.8).
+bool linear_fp8_fits_rows(int64_t M, int64_t K) { return M <= 16 || (M <= 32 && K <= 512); }
 
 int launch_linear_fp8_rows(const void* x, int x_dtype, int64_t ld_x, const Fp8Operand& b, int b_block_rows, int64_t M, int64_t N, int64_t K, const float* bias,
                            void* c, int c_dtype, int64_t ld_c, hipStream_t s) {

@@ -161,9 +161,22 @@ def test_product(ctx, mnk, block_rows, out_dtype):
     assert torch.equal(got, ctx.gemm_fp8(a, w, bias=bias, out_dtype=out_dtype))          # one order of the sums
 
 
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('mnk', [(65, 64, 66000), (130, 40, 20000), (300, 97, 2048), (100, 97, 512), (65, 1, 300000)])
+def test_product_of_few_tiles_and_many_blocks(ctx, mnk, out_dtype):
+    """k in pieces: a few, and more than the 16 of one batch of the join; a last piece that is shorter."""
+    m, n, k = mnk
+    a = ctx.quantize_fp8(values(m, k, k).cuda())
+    w = ctx.quantize_fp8(values(n, k, n).cuda() * 0.05, block_rows=128)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
+    got = ctx.gemm_fp8(a, w, bias=bias, out_dtype=out_dtype)
+    check_product(got, a, w, bias, out_dtype)
+    assert torch.equal(got, ctx.gemm_fp8(a, w, bias=bias, out_dtype=out_dtype))
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('mnk', [(1, 6719, 256), (1, 1, 1), (3, 97, 256), (16, 300, 200), (17, 129, 97), (40, 4096, 1000), (64, 256, 512), (8, 64, 8192),
-                                 (300, 97, 512), (2, 40, 20000)])
+                                 (300, 97, 512), (2, 40, 20000), (32, 97, 512), (32, 97, 513), (17, 40, 1000)])
 def test_linear_equals_quantise_and_product(ctx, mnk, dtype):
     m, n, k = mnk
     x = values(m, k, k + 1, dtype).cuda()
