@@ -279,9 +279,10 @@ struct TopArgs {
 };
 
 // Every lane sorts its 8 classes, the lists go to LDS, and the K largest of the row are K times the largest head of 16 lists;
-// the winner writes its class down and moves on.  Bound by the vector ALU: the next row's loads are on their way, and a
-// logit's key with its class (7 bits; among equals the lower class counts as the larger) is held as the bits of a float64
-// between 1 and 2, which order like the numbers: two instructions sort a pair.
+// the winner writes its class down and moves on.  Bound by the vector ALU (1.4M rows of 97 float32, 10 entries: 315 us, 1.8
+// TB/s): the next row's loads are on their way, and a logit's key with its class (7 bits; among equals the lower class counts
+// as the larger) is held as the bits of a float64 between 1 and 2, which order like the numbers: two instructions sort a
+// pair.
 __device__ __forceinline__ double entry_of(unsigned key, unsigned at) {
     return __hiloint2double((int)(0x3FF00000u | key >> 12), (int)(key << 20 | (127u - at) << 13));
 }
@@ -363,13 +364,13 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
     }
 }
 
-// Rows in LDS: up to kWaveBytes one wave's own, so that nothing waits for another; longer ones are shared by four waves, for
-// few fit a compute unit.
+// Rows in LDS: short ones are one wave's own, so that nothing waits for another; longer ones are shared, for few fit a compute
+// unit (which waves take which rows: launch_top, launch_distill).
 constexpr size_t kWaveBytes = 16384, kRowBytes = 32768;
 constexpr int kTopList = 512;          // candidates of a row that LDS holds
 
-// The row to LDS, BATCH pieces of a lane in flight (pieces of 16 bytes; classes behind the last are -infinity); returns the lane's maximum.  `between` runs
-// while the first pieces are on their way.
+// The row to LDS, BATCH pieces of a lane in flight (pieces of 16 bytes; classes behind the last are -infinity); returns the
+// lane's maximum.  `between` runs while the first pieces are on their way.
 template <int THREADS, int BATCH, bool TINY, class T, class F>
 __device__ __forceinline__ float row_to_lds(const T* p, int V, uintx4* buf, F between) {
     constexpr int P = kPiece<T>;
@@ -448,7 +449,7 @@ __device__ __forceinline__ void write_one_by_one(const TopArgs<T>& a, int64_t ro
     }
 }
 
-// A row in LDS, W waves on it.  The bound: every wave bisects its own 64 maxima for the ceil(K / W)-th largest, the least
+// A row in LDS, W waves on it: bound by reading the logits (16384 rows of 6719 float32, 32 entries: 98 us, 4.5 TB/s).  The bound of the candidates: every wave bisects its own 64 maxima for the ceil(K / W)-th largest, the least
 // of those is reached by at least K values.
 template <class T, int W, int BATCH>
 __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
@@ -734,7 +735,8 @@ __device__ __forceinline__ void put_entry(void* row, int idx, float v) {
 }
 
 // Rows of up to 128 classes and 16 entries: 16 lanes per row, four rows a wave, in LDS of the group's own.  Such a row is 776
-// bytes and a few hundred float64 instructions, so the next row's loads (and the weight of the one after it, which says
+// bytes and a few hundred float64 instructions (131072 rows of 97 float32, 10 entries: 31 us, 3.7 TB/s, bound by the vector
+// ALU), so the next row's loads (and the weight of the one after it, which says
 // whether to load it) are on their way while one is worked on.
 template <class T, bool TINY>
 __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs<T> a) {
@@ -840,7 +842,8 @@ __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs<T> a) {
     }
 }
 
-// A row in LDS, W waves on it: read from memory once.  The first wave has the entries, and does the teacher's part while
+// A row in LDS, W waves on it: read from memory once, bound by that and by writing the gradient (16384 rows of 6719 bfloat16
+// 101 us, 4.4 TB/s).  The first wave has the entries, and does the teacher's part while
 // the row is on its way.  The entries' places hold -infinity during the sum, so that nothing has to be tested per class;
 // every wave turns its own pieces into gradients in place, puts the entries' gradients among them and stores whole pieces.
 template <class T, int W, int BATCH, bool TINY>
@@ -957,7 +960,8 @@ __global__ __launch_bounds__(W * 64) void distill_lds_kernel(DistillArgs<T> a) {
 }
 
 // Rows of any length, a workgroup of 8 waves each: one pass with a running maximum and sum per thread, and for the gradient
-// a second one over the row (which the caches still hold in part).
+// a second one over the row (which the caches still hold in part).  Bound by reading the row: 2048 rows of 131071 bfloat16 classes, the loss
+// alone, 112 us, 4.8 TB/s.
 template <class T>
 __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
     constexpr int P = kPiece<T>, THREADS = 512, WAVES = 8, AHEAD = 4;
@@ -1067,6 +1071,12 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
 
 constexpr int64_t kMaxGrid = 1 << 20;          // workgroups of a launch; each walks the rows from there
 
+// Rows of up to 128 classes and 16 entries: 16 lanes a row (97 classes, 10 entries, 1.4M rows 315 us; a wave a row 894).
+// Rows in LDS: one wave up to 6 KB (float32, 32 entries, 134M classes in all: 1100 classes 205 us against 223 of two waves,
+// 1500 182 against 173, 2000 193 against 147), two up to 16 KB (4000 classes 134 against 141 of four, 208 of one), four up to
+// 32 KB (6719 classes 119 against 164 of two).  More than 32 entries of a longer row need a second wave's maxima for a useful
+// bound (2000 classes, 64 entries: 194 against 1032).  Beyond, and where a compute unit would hold few rows: eight waves on a
+// row that is read twice (8000 float32 classes: 176 against 129 in LDS).
 template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
@@ -1077,7 +1087,7 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
         hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
     else if (a.V <= kShort && a.K <= 16)
         hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
-    else if (row_lds <= 8192 && (a.K <= 32 || a.V <= kTopList)) {      // one wave: K of 64 maxima have to be a useful bound
+    else if (row_lds <= 6144 && (a.K <= 32 || a.V <= kTopList)) {
         if (row_lds <= 2048)
             hipLaunchKernelGGL((top_lds_kernel<T, 1, 2>), dim3(grid), dim3(64), row_lds, s, a);
         else if (row_lds <= 4096)
@@ -1094,6 +1104,10 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
     return OCRHIP_OK;
 }
 
+// Rows of up to 128 classes and 16 entries: 16 lanes a row (97 classes, 10 entries, 1.4M rows 344 us; a wave a row 1723).  Rows
+// in LDS: one wave up to 16 KB (float32, 32 entries, 134M classes in all: 2000 classes 197 us against 251 of two waves, 418 of
+// four; 4000 208 against 188 and 248; bfloat16 4000 classes 114 against 152), four up to 32 KB (6719 classes 198 against 263
+// of one, 203 of two).  Beyond: eight waves on a row that is read twice (8000 float32 classes: 288 against 186 in LDS).
 template <class T>
 int launch_distill(const DistillArgs<T>& a, hipStream_t s) {
     constexpr int P = kPiece<T>;
