@@ -1385,7 +1385,10 @@ int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t r
     return launch_quantize_fp8(d_x, x_dtype, rows, cols, ld_x, block_rows, transpose != 0, d_q, ld_q, d_scale, ld_scale, (hipStream_t)stream);
 }
 
-size_t ocrhip_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) { return M > 0 && N > 0 && K > 0 ? gemm_fp8_workspace(M, N, K) : 0; }
+// sizes that a product takes (the others' workspaces are 0, and the product is refused)
+static bool product_sizes(int64_t M, int64_t N, int64_t K) { return M > 0 && N > 0 && K > 0 && M < (1ll << 31) && N < (1ll << 31) && K <= kMaxDepth; }
+
+size_t ocrhip_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) { return product_sizes(M, N, K) ? gemm_fp8_workspace(M, N, K) : 0; }
 
 int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uint8_t* d_a_scale, int64_t ld_a_scale, const uint8_t* d_b,
                     int64_t ld_b, const uint8_t* d_b_scale, int64_t ld_b_scale, int b_block_rows, int64_t M, int64_t N, int64_t K,
@@ -1402,7 +1405,7 @@ int ocrhip_gemm_fp8(ocrhip_handle h, const uint8_t* d_a, int64_t ld_a, const uin
 
 // workspace of linear_fp8: the quantised rows, their scales, then the product's own
 size_t ocrhip_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || linear_fp8_fits_rows(M, K)) return 0;
+    if (!product_sizes(M, N, K) || linear_fp8_fits_rows(M, K)) return 0;
     return (size_t)(M * round_up(K, 128) + (K + 127) / 128 * round_up(M, 16)) + gemm_fp8_workspace(M, N, K);
 }
 

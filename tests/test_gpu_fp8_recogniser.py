@@ -74,6 +74,37 @@ def test_recogniser_with_8_bit_dense_layers(ctx, n, wpad, vocab):
     np.testing.assert_array_equal(run(BF16)[0], plain[0])
 
 
+# blocks of k that the columns do not fill (64, 192), per-step recurrence
+@pytest.mark.parametrize('hidden', [64, 128, 192, 512])
+def test_other_lstm_widths(ctx, hidden):
+    from ocr_amd._lib import BF16
+    params = nets.init_crnn_params(vocab_size=211, hidden=hidden, seed=3)
+    ctx.crnn_load_weights(params)
+    x = torch.from_numpy(np.random.default_rng(hidden).uniform(-1, 1, (6, 64, 100, 1)).astype(np.float32)).cuda()
+    plain = ctx.crnn_forward(x, compute_dtype=BF16)['logits'].cpu().numpy()
+    ctx.set_option('fp8_dense', 1)
+    try:
+        logits = ctx.crnn_forward(x, compute_dtype=BF16)['logits'].cpu().numpy()
+        ctx.check_errors()
+    finally:
+        ctx.set_option('fp8_dense', 0)
+    check_class_layer(params, np.asarray(ctx.crnn_activation('seq1'), np.float64).reshape(-1, hidden), logits.reshape(-1, 211))
+    assert 0 < rel(logits, plain) <= BAR
+
+
+def test_resnet_recogniser_does_not_know_the_option(ctx):
+    from ocr_amd._lib import BF16
+    ctx.crnn_load_weights(nets.init_crnn_params(vocab_size=97, hidden=256, seed=3, backbone='resnet'))
+    x = torch.from_numpy(np.random.default_rng(1).uniform(-1, 1, (2, 64, 64, 1)).astype(np.float32)).cuda()
+    plain = ctx.crnn_forward(x, compute_dtype=BF16)['logits']
+    ctx.set_option('fp8_dense', 1)
+    try:
+        got = ctx.crnn_forward(x, compute_dtype=BF16)['logits']
+    finally:
+        ctx.set_option('fp8_dense', 0)
+    assert torch.equal(got, plain)
+
+
 def test_packed_batch_with_8_bit_dense_layers(ctx):
     """Several widths in one call; then a smaller one: the buffers of the larger one hold other values behind its rows."""
     from ocr_amd._lib import BF16

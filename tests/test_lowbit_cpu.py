@@ -201,7 +201,7 @@ def test_a_workspace_that_is_too_small_is_a_capacity_error():
 def test_workspaces_of_empty_and_negative_sizes_are_nothing():
     from ocr_amd import _lib
     lib = _lib.load()
-    for m, n, k in ((0, 5, 5), (5, 0, 5), (5, 5, 0), (-1, 5, 5)):
+    for m, n, k in ((0, 5, 5), (5, 0, 5), (5, 5, 0), (-1, 5, 5), (1 << 62, 5, 5), (70, 1 << 62, 5), (70, 5, 1 << 62), (1 << 31, 5, 5)):
         assert lib.ocrhip_gemm_fp8_workspace(m, n, k) == 0 and lib.ocrhip_linear_fp8_workspace(m, n, k) == 0
 
 
