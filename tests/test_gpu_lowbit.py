@@ -316,6 +316,9 @@ def check_top(ctx, x, k, t):
     val, idx, lse = lowbit.top_logits(x64, k, t)
     np.testing.assert_array_equal(got_i.cpu().numpy().reshape(-1, k), idx)
     np.testing.assert_array_equal(got_v.cpu().numpy().reshape(-1, k).astype(np.float64), val)
+    # the result is a float32: what lies half a step beyond its largest, 2^128 (1 - 2^-25), rounds to infinity (a masked row
+    # of the type's lowest value at a temperature below 1: -3.4e38 / 0.25 = -1.36e39)
+    lse = np.where(np.abs(lse) >= 2.0 ** 128 * (1 - 2.0 ** -25), np.copysign(np.inf, lse), lse)
     got_l, fin = got_l.cpu().numpy().reshape(-1).astype(np.float64), np.isfinite(lse)
     np.testing.assert_array_equal(np.isnan(got_l), np.isnan(lse))
     np.testing.assert_array_equal(got_l[~fin & ~np.isnan(lse)], lse[~fin & ~np.isnan(lse)])
@@ -366,6 +369,42 @@ def test_top_logits_with_nan_and_infinity(ctx, v):
     np.testing.assert_array_equal(got_v.cpu().numpy().astype(np.float64), val)
     l = got_l.cpu()
     assert torch.isnan(l[0]) and l[1] == float('inf') and torch.isnan(l[2]) and torch.isnan(l[3])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('v,k', [(1, 1), (3, 3), (4, 1), (7, 7), (8, 8), (9, 5), (16, 16), (17, 16), (40, 16), (97, 1), (97, 16), (127, 10), (128, 16)])
+def test_top_logits_of_short_rows(ctx, v, k, dtype):
+    """Up to 128 classes and 16 entries: one class far above the rest, equal values within a lane's classes and across lanes,
+    masked classes, rows without a finite logit, infinities, zeros of both signs, NaN; and more rows than one pass of the
+    grid holds."""
+    g = torch.Generator().manual_seed(v * 100 + k)
+    x = torch.randn(24, v, generator=g)
+    x[0] = 0.0
+    x[1] = torch.randint(0, 2, (v,), generator=g).float()
+    x[2] = torch.arange(v).float()
+    x[3] = -torch.arange(v).float()
+    x[4] = -float('inf')
+    x[5] = -float('inf')
+    x[5, v // 2] = 1.0
+    x[6, v - 1] = float('inf')
+    x[7] = torch.finfo(dtype).min
+    x[8, ::2] = torch.finfo(dtype).min
+    x[9] = torch.where(torch.arange(v) % 2 == 0, 0.0, -0.0)
+    x[10] = 3e38
+    x[11] = torch.randint(-2, 3, (v,), generator=g).float() * 1e-40
+    x[12, : v // 2 + 1] = 5.0
+    x[13, v // 2:] = 5.0
+    x[14, v // 3] = float('nan')
+    x[15] = float('nan')
+    x = x.to(dtype)
+    for t in (1.0, 0.25):
+        check_top(ctx, x.cuda(), k, t)
+    many = x.cuda().repeat(1500, 1)[:35001]
+    val, idx, lse = ctx.top_logits(many, k)
+    want = ctx.top_logits(x.cuda(), k)
+    for got, w in zip((val, idx, lse), want):
+        w = w.repeat(1500, 1)[:35001] if w.dim() == 2 else w.repeat(1500)[:35001]
+        assert torch.equal(got.nan_to_num(1e9) if got.is_floating_point() else got, w.nan_to_num(1e9) if w.is_floating_point() else w)
 
 
 def test_top_logits_strides_and_offsets(ctx):
