@@ -265,8 +265,9 @@ __device__ __forceinline__ void lds_phase() {
 // Bound by reading the logits once.  Rows of up to 128 classes and 16 entries: 16 lanes per row (top16_kernel).  Longer rows:
 // the K-th largest of the lanes' own maxima is a lower bound of the K-th largest of all (K lanes hold a value that large),
 // and hardly more than K values reach it: it is found by bisection of its leading bits, the values that reach it are put on
-// a list in LDS and each finds its rank by counting the larger ones.  A row whose list overflows (hundreds of equal values)
-// takes its maxima one by one.
+// a list in LDS and each finds its rank by counting the larger ones.  A row with too many candidates (hundreds of equal
+// values, as under a mask) takes the few above the K-th largest and the first of those equal to it, or failing that its
+// maxima one by one.
 template <class T>
 struct TopArgs {
     const T* x;
@@ -396,10 +397,11 @@ __device__ __forceinline__ float row_to_lds(const T* p, int V, uintx4* buf, F be
     return m;
 }
 
-// the largest bound of 20 leading bits that K of the wave's keys reach (0: fewer than K lanes have one)
-__device__ __forceinline__ unsigned bisect(const unsigned* keys, int n, int K) {
-    unsigned bound = 0;
-    for (int bit = 31; bit >= 12; --bit) {
+// the largest bound that K of the wave's keys reach (0: fewer than K lanes have one), its bits from FROM down to TO; those in
+// front of them are given
+template <int FROM, int TO>
+__device__ __forceinline__ unsigned bisect(const unsigned* keys, int n, int K, unsigned bound = 0) {
+    for (int bit = FROM; bit >= TO; --bit) {
         const unsigned next = bound | 1u << bit;
         int reach = 0;
         for (int w = 0; w < n; ++w) reach += __popcll(__ballot(keys[w] >= next));
@@ -421,6 +423,43 @@ __device__ __forceinline__ void write_ranked(const TopArgs<T>& a, int64_t row, c
             a.index[row * a.K + rank] = (int)(0xFFFFFFFFu - (unsigned)own);
         }
     }
+}
+
+// The same for a row that has more candidates than the list holds, with a key that at least K values reach.  Mostly the K-th
+// largest value is that key and many others are equal to it (classes masked with one low value, a row without a finite
+// logit): the fewer than K values above it go to the list, then the first equal ones in the order of the classes.  False
+// where K values or more lie above it.
+template <int WAVES, class T>
+__device__ __forceinline__ bool write_equal(const TopArgs<T>& a, int64_t row, unsigned key, unsigned long long* list, int* count) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const T* p = a.x + row * a.ld;
+    __syncthreads();                                       // every thread has read the count that led here
+    if (tid == 0) *count = 0;
+    __syncthreads();
+    for (int at = tid; at < a.V; at += WAVES * 64) {
+        const unsigned own = order_key(load_f32(p + at));
+        if (own > key) {
+            const int slot = atomicAdd(count, 1);
+            if (slot < a.K) list[slot] = (unsigned long long)own << 32 | (0xFFFFFFFFu - (unsigned)at);
+        }
+    }
+    __syncthreads();
+    const int above = *count;
+    if (above >= a.K) return false;
+    if (tid < 64) {
+        int have = above;
+        for (int base = 0; base < a.V && have < a.K; base += 64) {
+            const int at = base + lane;
+            const bool equal = at < a.V && order_key(load_f32(p + min(at, a.V - 1))) == key;
+            const unsigned long long all = __ballot(equal);
+            const int slot = have + __popcll(all & ((1ull << lane) - 1));
+            if (equal && slot < a.K) list[slot] = (unsigned long long)key << 32 | (0xFFFFFFFFu - (unsigned)at);
+            have += __popcll(all);
+        }
+    }
+    __syncthreads();
+    write_ranked(a, row, list, a.K, tid, WAVES * 64);
+    return true;
 }
 
 // The same without a list: the maxima one by one, a pass over the row each.
@@ -465,7 +504,8 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
         if (tid == 0) count = 0;
         const float mine = row_to_lds<THREADS, BATCH, false>(a.x + row * a.ld, a.V, buf, [] {});
         const unsigned key = tid < pieces ? order_key(mine) : 0u;
-        unsigned least = bisect(&key, 1, (a.K + W - 1) / W);
+        const unsigned own_least = bisect<31, 12>(&key, 1, (a.K + W - 1) / W);
+        unsigned least = own_least;
         float high = group_max<64>(mine);                  // NaN apart
         if (W > 1) {
             if (lane == 0) {
@@ -504,14 +544,23 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
         if (lane == 0) wave_sum[wave] = sum;
         __syncthreads();
         const int n = count;
-        if (n <= kTopList)
-            write_ranked(a, row, list, n, tid, THREADS);
-        else
-            write_one_by_one<W>(a, row, wave_best);
         if (a.lse && tid == THREADS - 1) {
             double total = 0.0;
             for (int i = 0; i < W; ++i) total += (double)wave_sum[i];
             a.lse[row] = (float)((double)base * a.inv_t + log_sum(total));
+        }
+        if (n <= kTopList) {
+            write_ranked(a, row, list, n, tid, THREADS);
+        } else {
+            unsigned exact = bisect<11, 0>(&key, 1, (a.K + W - 1) / W, own_least);
+            if (W > 1) {
+                if (lane == 0) wave_bits[wave] = exact;
+                __syncthreads();
+                exact = wave_bits[0];
+#pragma unroll
+                for (int i = 1; i < W; ++i) exact = min(exact, wave_bits[i]);
+            }
+            if (!write_equal<W>(a, row, exact, list, &count)) write_one_by_one<W>(a, row, wave_best);
         }
         __syncthreads();
     }
@@ -526,7 +575,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
     __shared__ unsigned maxima[THREADS];
     __shared__ float wave_sum[WAVES];
     __shared__ unsigned long long wave_best[WAVES];
-    __shared__ unsigned shared_bound;
+    __shared__ unsigned shared_bound, shared_exact;
     __shared__ float shared_high;
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -565,7 +614,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
                 m[w] = maxima[w * 64 + lane];
                 top = max(top, m[w]);
             }
-            const unsigned bits = bisect(m, WAVES, a.K);
+            const unsigned bits = bisect<31, 12>(m, WAVES, a.K);
             top = group_max<64>(top);
             if (lane == 0) {
                 shared_bound = bits;
@@ -595,7 +644,15 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
         if (n <= kTopList) {
             write_ranked(a, row, list, n, tid, THREADS);
         } else {
-            write_one_by_one<WAVES>(a, row, wave_best);
+            if (wave == 0) {
+                unsigned m[WAVES];
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) m[w] = maxima[w * 64 + lane];
+                const unsigned exact = bisect<11, 0>(m, WAVES, a.K, shared_bound);
+                if (lane == 0) shared_exact = exact;
+            }
+            __syncthreads();
+            if (!write_equal<WAVES>(a, row, shared_exact, list, &count)) write_one_by_one<WAVES>(a, row, wave_best);
         }
         if (a.lse && tid == 0) {
             double total = 0.0;
@@ -1074,8 +1131,9 @@ constexpr int64_t kMaxGrid = 1 << 20;          // workgroups of a launch; each w
 // Rows of up to 128 classes and 16 entries: 16 lanes a row (97 classes, 10 entries, 1.4M rows 315 us; a wave a row 894).
 // Rows in LDS: one wave up to 6 KB (float32, 32 entries, 134M classes in all: 1100 classes 205 us against 223 of two waves,
 // 1500 182 against 173, 2000 193 against 147), two up to 16 KB (4000 classes 134 against 141 of four, 208 of one), four up to
-// 32 KB (6719 classes 119 against 164 of two).  More than 32 entries of a longer row need a second wave's maxima for a useful
-// bound (2000 classes, 64 entries: 194 against 1032).  Beyond, and where a compute unit would hold few rows: eight waves on a
+// 32 KB (6719 classes 119 against 164 of two).  More than 32 entries need a second wave's maxima for a useful bound, where the
+// row has pieces for that many lanes (64 entries, 67M classes in all: 768 float32 classes 258 against 541, but 600 bfloat16
+// classes, 75 pieces, 723 with one wave and 3033 with two).  Beyond, and where a compute unit would hold few rows: eight waves on a
 // row that is read twice (8000 float32 classes: 176 against 129 in LDS).
 template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
@@ -1087,7 +1145,7 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
         hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
     else if (a.V <= kShort && a.K <= 16)
         hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
-    else if (row_lds <= 6144 && (a.K <= 32 || a.V <= kTopList)) {
+    else if (row_lds <= 6144 && (a.K <= 32 || row_lds / 16 < (size_t)(64 + a.K / 2))) {
         if (row_lds <= 2048)
             hipLaunchKernelGGL((top_lds_kernel<T, 1, 2>), dim3(grid), dim3(64), row_lds, s, a);
         else if (row_lds <= 4096)

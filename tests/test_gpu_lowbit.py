@@ -407,6 +407,34 @@ def test_top_logits_of_short_rows(ctx, v, k, dtype):
         assert torch.equal(got.nan_to_num(1e9) if got.is_floating_point() else got, w.nan_to_num(1e9) if w.is_floating_point() else w)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('v,k', [(300, 20), (520, 64), (700, 64), (769, 64), (1500, 32), (3000, 64), (6719, 32), (9000, 64), (20000, 64)])
+def test_top_logits_of_masked_rows(ctx, v, k, dtype):
+    """Many classes at one low value, in rows of every length: fewer classes left than asked for, none, about as many, in one
+    place and spread; two levels of equal values; equal values above and below the K-th; NaN among them."""
+    g = torch.Generator().manual_seed(v + k)
+    low = torch.finfo(dtype).min
+    rows = []
+    for left in (0, 1, k - 1, k, k + 1, 3 * k, v // 2, v - 1):
+        for fill in (-float('inf'), low, 0.0):
+            for spread in (False, True):
+                r = torch.full((v,), fill)
+                at = torch.randperm(v, generator=g)[:left] if spread else torch.arange(v - left, v)
+                r[at] = torch.randn(len(at), generator=g)
+                rows.append(r)
+    levels = torch.zeros(6, v)
+    levels[0, ::2] = 1.0
+    levels[1, 3::7] = 1.0
+    levels[2, :k // 2] = 2.0
+    levels[2, v // 2:v // 2 + k] = 1.0
+    levels[3] = torch.randint(0, 3, (v,), generator=g).float()
+    levels[4, v // 2], levels[4, 1] = float('nan'), float('inf')
+    levels[5] = -float('inf')
+    levels[5, v - 1] = float('nan')
+    x = torch.cat([torch.stack(rows), levels]).to(dtype)
+    check_top(ctx, x.cuda(), k, 1.0)
+
+
 def test_top_logits_strides_and_offsets(ctx):
     big = logits(60, 300, 4).cuda()
     for dt in (torch.float32, torch.bfloat16):
