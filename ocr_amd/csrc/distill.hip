@@ -262,7 +262,7 @@ __device__ __forceinline__ void lds_phase() {
 
 // ---- top logits
 //
-// Bound by reading the logits once.  Rows of up to 128 classes and 16 entries: 16 lanes per row (top16_kernel).  Longer rows:
+// Bound by reading the logits once.  Rows of up to 128 classes: 16 lanes per row (top16_kernel).  Longer rows:
 // the K-th largest of the lanes' own maxima is a lower bound of the K-th largest of all (K lanes hold a value that large),
 // and hardly more than K values reach it: it is found by bisection of its leading bits, the values that reach it are put on
 // a list in LDS and each finds its rank by counting the larger ones.  A row with too many candidates (hundreds of equal
@@ -294,8 +294,9 @@ template <class T, bool TINY>
 __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
     constexpr int P = kPiece<T>, L = kShort / 16, N = L / P;
     __shared__ double lists[L][256];                       // from the third on; two entries below all behind the last
-    __shared__ double found[16][16];                       // per row
+    extern __shared__ double found_lds[];                  // K per row
     const int tid = threadIdx.x, part = tid & 15, sub = tid >> 4;
+    double* found = found_lds + sub * a.K;
     const float c = a.inv_t * kLog2e;
     const int64_t step = (int64_t)gridDim.x * 16;
     uintx4 next[N];
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
         for (int k = 0; k < a.K; ++k) {                    // K <= V: some head is a class
             const unsigned top = group_max<16>(hi), which = group_max<16>(hi == top ? lo : 0u);
             if (hi == top && lo == which) {
-                found[sub][k] = __hiloint2double((int)hi, (int)lo);
+                found[k] = __hiloint2double((int)hi, (int)lo);
                 hi = (unsigned)__double2hiint(second);
                 lo = (unsigned)__double2loint(second);
                 second = *behind;
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
         }
         lds_phase();
         if (a.lse) {
-            const float high = key_value(entry_key((unsigned)__double2hiint(found[sub][0]), (unsigned)__double2loint(found[sub][0])));
+            const float high = key_value(entry_key((unsigned)__double2hiint(found[0]), (unsigned)__double2loint(found[0])));
             const float base = fabsf(high) == INFINITY || high != high ? 0.0f : high;
             float sum = 0.0f;
 #pragma unroll
@@ -356,11 +357,12 @@ __global__ __launch_bounds__(256) void top16_kernel(TopArgs<T> a) {
             sum = group_sum<16>(sum);
             if (part == 0 && row < a.rows) a.lse[row] = (float)((double)base * a.inv_t + log_sum((double)sum));
         }
-        if (part < a.K && row < a.rows) {
-            const unsigned h = (unsigned)__double2hiint(found[sub][part]), l = (unsigned)__double2loint(found[sub][part]);
-            a.values[row * a.K + part] = key_value(entry_key(h, l));
-            a.index[row * a.K + part] = (int)entry_class(l);
-        }
+        if (row < a.rows)
+            for (int k = part; k < a.K; k += 16) {
+                const unsigned h = (unsigned)__double2hiint(found[k]), l = (unsigned)__double2loint(found[k]);
+                a.values[row * a.K + k] = key_value(entry_key(h, l));
+                a.index[row * a.K + k] = (int)entry_class(l);
+            }
         lds_phase();
     }
 }
@@ -793,8 +795,8 @@ __device__ __forceinline__ void put_entry(void* row, int idx, float v) {
 
 // Rows of up to 128 classes and 16 entries: 16 lanes per row, four rows a wave, in LDS of the group's own.  Such a row is 776
 // bytes and a few hundred float64 instructions (131072 rows of 97 float32, 10 entries: 31 us, 3.7 TB/s, bound by the vector
-// ALU), so the next row's loads (and the weight of the one after it, which says
-// whether to load it) are on their way while one is worked on.
+// ALU), so the next row's loads (and the weight of the one after it, which says whether to load it) are on their way while
+// one is worked on.
 template <class T, bool TINY>
 __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs<T> a) {
     constexpr int G = 16, ROWS = 256 / G, P = kPiece<T>, N = kShort / G / P;
@@ -1128,7 +1130,8 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
 
 constexpr int64_t kMaxGrid = 1 << 20;          // workgroups of a launch; each walks the rows from there
 
-// Rows of up to 128 classes and 16 entries: 16 lanes a row (97 classes, 10 entries, 1.4M rows 315 us; a wave a row 894).
+// Rows of up to 128 classes: 16 lanes a row (97 float32 classes, 10 entries, 1.4M rows 315 us, a wave a row 894; 0.7M rows and
+// 64 entries 446 against 821).
 // Rows in LDS: one wave up to 6 KB (float32, 32 entries, 134M classes in all: 1100 classes 205 us against 223 of two waves,
 // 1500 182 against 173, 2000 193 against 147), two up to 16 KB (4000 classes 134 against 141 of four, 208 of one), four up to
 // 32 KB (6719 classes 119 against 164 of two).  More than 32 entries need a second wave's maxima for a useful bound, where the
@@ -1139,12 +1142,12 @@ template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
     constexpr int P = kPiece<T>;
-    const size_t row_lds = (size_t)(a.V + P - 1) / P * 16;
+    const size_t row_lds = (size_t)(a.V + P - 1) / P * 16, found_lds = (size_t)a.K * 16 * sizeof(double);
     const unsigned groups = (unsigned)std::min<int64_t>((a.rows + 15) / 16, 2048);          // 8 per compute unit, which walk the rows
     if (a.V < P)                       // K <= V
-        hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
-    else if (a.V <= kShort && a.K <= 16)
-        hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), found_lds, s, a);
+    else if (a.V <= kShort)
+        hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), found_lds, s, a);
     else if (row_lds <= 6144 && (a.K <= 32 || row_lds / 16 < (size_t)(64 + a.K / 2))) {
         if (row_lds <= 2048)
             hipLaunchKernelGGL((top_lds_kernel<T, 1, 2>), dim3(grid), dim3(64), row_lds, s, a);

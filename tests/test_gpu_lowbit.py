@@ -372,9 +372,10 @@ def test_top_logits_with_nan_and_infinity(ctx, v):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize('v,k', [(1, 1), (3, 3), (4, 1), (7, 7), (8, 8), (9, 5), (16, 16), (17, 16), (40, 16), (97, 1), (97, 16), (127, 10), (128, 16)])
+@pytest.mark.parametrize('v,k', [(1, 1), (3, 3), (4, 1), (7, 7), (8, 8), (9, 5), (16, 16), (17, 16), (40, 16), (97, 1), (97, 16), (127, 10), (128, 16),
+                                 (17, 17), (40, 33), (65, 64), (97, 17), (97, 64), (128, 64), (129, 64), (129, 10)])
 def test_top_logits_of_short_rows(ctx, v, k, dtype):
-    """Up to 128 classes and 16 entries: one class far above the rest, equal values within a lane's classes and across lanes,
+    """Up to 128 classes, and one more: one class far above the rest, equal values within a lane's classes and across lanes,
     masked classes, rows without a finite logit, infinities, zeros of both signs, NaN; and more rows than one pass of the
     grid holds."""
     g = torch.Generator().manual_seed(v * 100 + k)
