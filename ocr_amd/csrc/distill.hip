@@ -490,9 +490,9 @@ __device__ __forceinline__ void write_one_by_one(const TopArgs<T>& a, int64_t ro
     }
 }
 
-// A row in LDS, W waves on it: bound by reading the logits (16384 rows of 6719 float32, 32 entries: 98 us, 4.5 TB/s).  The bound of the candidates: every wave bisects its own 64 maxima for the ceil(K / W)-th largest, the least
+// A row in LDS, W waves on it (FEW: as many maxima a lane as a piece has classes, one wave): bound by reading the logits (16384 rows of 6719 float32, 32 entries: 98 us, 4.5 TB/s).  The bound of the candidates: every wave bisects its own 64 maxima for the ceil(K / W)-th largest, the least
 // of those is reached by at least K values.
-template <class T, int W, int BATCH>
+template <class T, int W, int BATCH, bool FEW = false>
 __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
     constexpr int P = kPiece<T>, THREADS = W * 64;
     extern __shared__ uintx4 buf[];                        // the row
@@ -506,7 +506,22 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
         if (tid == 0) count = 0;
         const float mine = row_to_lds<THREADS, BATCH, false>(a.x + row * a.ld, a.V, buf, [] {});
         const unsigned key = tid < pieces ? order_key(mine) : 0u;
-        const unsigned own_least = bisect<31, 12>(&key, 1, (a.K + W - 1) / W);
+        unsigned fine[P] = {};
+        if (FEW) {
+            float part[P];
+#pragma unroll
+            for (int e = 0; e < P; ++e) part[e] = -INFINITY;
+            lds_phase();
+            for (int q = tid; q < pieces; q += THREADS) {
+                float v[P];
+                unpack_piece(buf[q], v);
+#pragma unroll
+                for (int e = 0; e < P; ++e) part[e] = fmaxf(part[e], v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < P; ++e) fine[e] = tid * P + e < a.V ? order_key(part[e]) : 0u;
+        }
+        const unsigned own_least = FEW ? bisect<31, 12>(fine, P, a.K) : bisect<31, 12>(&key, 1, (a.K + W - 1) / W);
         unsigned least = own_least;
         float high = group_max<64>(mine);                  // NaN apart
         if (W > 1) {
@@ -554,7 +569,7 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
         if (n <= kTopList) {
             write_ranked(a, row, list, n, tid, THREADS);
         } else {
-            unsigned exact = bisect<11, 0>(&key, 1, (a.K + W - 1) / W, own_least);
+            unsigned exact = FEW ? bisect<11, 0>(fine, P, a.K, own_least) : bisect<11, 0>(&key, 1, (a.K + W - 1) / W, own_least);
             if (W > 1) {
                 if (lane == 0) wave_bits[wave] = exact;
                 __syncthreads();
@@ -1134,10 +1149,11 @@ constexpr int64_t kMaxGrid = 1 << 20;          // workgroups of a launch; each w
 // 64 entries 446 against 821).
 // Rows in LDS: one wave up to 6 KB (float32, 32 entries, 134M classes in all: 1100 classes 205 us against 223 of two waves,
 // 1500 182 against 173, 2000 193 against 147), two up to 16 KB (4000 classes 134 against 141 of four, 208 of one), four up to
-// 32 KB (6719 classes 119 against 164 of two).  More than 32 entries need a second wave's maxima for a useful bound, where the
-// row has pieces for that many lanes (64 entries, 67M classes in all: 768 float32 classes 258 against 541, but 600 bfloat16
-// classes, 75 pieces, 723 with one wave and 3033 with two).  Beyond, and where a compute unit would hold few rows: eight waves on a
-// row that is read twice (8000 float32 classes: 176 against 129 in LDS).
+// 32 KB (6719 classes 119 against 164 of two).  More than 32 entries need a second wave's maxima for a useful bound, where
+// the row has pieces for that many lanes (67M classes in all: 768 float32 classes, 64 entries 265 against 541); where it has
+// hardly more pieces than entries, a lane's maxima are taken class by class (FEW: 500 bfloat16 classes, 64 entries 207 against
+// 2145, 150 and 32 567 against 1059; with a few pieces more it costs: 500 and 32 180 against 122).  Beyond 32 KB, where a
+// compute unit would hold few rows: eight waves on a row that is read twice (8000 float32 classes: 176 against 129 in LDS).
 template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
@@ -1148,7 +1164,9 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
         hipLaunchKernelGGL((top16_kernel<T, true>), dim3(groups), dim3(256), found_lds, s, a);
     else if (a.V <= kShort)
         hipLaunchKernelGGL((top16_kernel<T, false>), dim3(groups), dim3(256), found_lds, s, a);
-    else if (row_lds <= 6144 && (a.K <= 32 || row_lds / 16 < (size_t)(64 + a.K / 2))) {
+    else if (row_lds < (size_t)(a.K > 32 ? 2 * a.K : a.K) * 16)          // less than 2 KB: K <= 64
+        hipLaunchKernelGGL((top_lds_kernel<T, 1, 2, true>), dim3(grid), dim3(64), row_lds, s, a);
+    else if (row_lds <= 6144 && (a.K <= 32 || row_lds < 2048)) {
         if (row_lds <= 2048)
             hipLaunchKernelGGL((top_lds_kernel<T, 1, 2>), dim3(grid), dim3(64), row_lds, s, a);
         else if (row_lds <= 4096)

@@ -409,7 +409,7 @@ def test_top_logits_of_short_rows(ctx, v, k, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize('v,k', [(300, 20), (520, 64), (700, 64), (769, 64), (1500, 32), (3000, 64), (6719, 32), (9000, 64), (20000, 64)])
+@pytest.mark.parametrize('v,k', [(130, 20), (150, 32), (260, 64), (300, 20), (500, 64), (520, 64), (700, 64), (769, 64), (1500, 32), (3000, 64), (6719, 32), (9000, 64), (20000, 64)])
 def test_top_logits_of_masked_rows(ctx, v, k, dtype):
     """Many classes at one low value, in rows of every length: fewer classes left than asked for, none, about as many, in one
     place and spread; two levels of equal values; equal values above and below the K-th; NaN among them."""
