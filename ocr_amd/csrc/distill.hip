@@ -35,7 +35,7 @@ __device__ __forceinline__ unsigned order_key(float x) {
 }
 __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
-// ---- reductions over groups of 16 or 64 lanes, on the vector ALU: quad, half row and row exchanges, then the swaps of
+// ---- reductions over groups of 16, 32 or 64 lanes, on the vector ALU: quad, half row and row exchanges, then the swaps of
 // rows and halves; every lane gets the same bits
 template <int CTRL>
 __device__ __forceinline__ unsigned lanes(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
@@ -75,10 +75,13 @@ __device__ __forceinline__ T reduce(T v, OP op) {
     v = op(v, lanes<0x4E>(v));               // lane ^ 2
     v = op(v, lanes<0x141>(v));              // the other quad of the half row
     v = op(v, lanes<0x140>(v));              // the other half row
-    if (G == 64) {
+    if (G >= 32) {
         T a, b;
         swapped<false>(v, a, b);
         v = op(a, b);
+    }
+    if (G == 64) {
+        T a, b;
         swapped<true>(v, a, b);
         v = op(a, b);
     }
@@ -98,7 +101,7 @@ __device__ __forceinline__ unsigned group_min(unsigned v) { return reduce<G>(v, 
 template <int G>
 __device__ __forceinline__ unsigned long long group_ballot(bool b) {
     const unsigned long long w = __ballot(b);
-    return G == 64 ? w : w >> (threadIdx.x & 48) & 0xFFFFull;
+    return G == 64 ? w : G == 32 ? w >> (threadIdx.x & 32) & 0xFFFFFFFFull : w >> (threadIdx.x & 48) & 0xFFFFull;
 }
 
 // ---- a row in pieces of 16 bytes, at any alignment of its elements
@@ -682,7 +685,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
 
 // ---- distillation
 
-// A group of G lanes (16 or 64, K <= G), lane k = entry k; float64 throughout.
+// A group of G lanes (16, 32 or 64, K <= G), lane k = entry k; float64 throughout.
 //
 // With d_k = (s_k - m) / tau, S = sum of exp((s - m) / tau) over all classes and S_r over those outside the entries, so that
 // log q_k = d_k - log S and log q_rest = log S_r - log S:
@@ -808,13 +811,13 @@ __device__ __forceinline__ void put_entry(void* row, int idx, float v) {
     store_f32(reinterpret_cast<T*>(reinterpret_cast<slot_t*>(row) + idx), v);
 }
 
-// Rows of up to 128 classes and 16 entries: 16 lanes per row, four rows a wave, in LDS of the group's own.  Such a row is 776
+// Rows of up to 128 classes: as many lanes per row as it has entries, at least 16, in LDS of the group's own.  Such a row is 776
 // bytes and a few hundred float64 instructions (131072 rows of 97 float32, 10 entries: 31 us, 3.7 TB/s, bound by the vector
 // ALU), so the next row's loads (and the weight of the one after it, which says whether to load it) are on their way while
 // one is worked on.
-template <class T, bool TINY>
+template <class T, bool TINY, int G>
 __global__ __launch_bounds__(256) void distill_short_kernel(DistillArgs<T> a) {
-    constexpr int G = 16, ROWS = 256 / G, P = kPiece<T>, N = kShort / G / P;
+    constexpr int ROWS = 256 / G, P = kPiece<T>, N = kShort / P > G ? kShort / P / G : 1;
     __shared__ uintx4 rows_lds[ROWS][N * G];
     const int part = threadIdx.x & (G - 1), sub = threadIdx.x / G, pieces = (a.V + P - 1) / P;
     uintx4* buf = rows_lds[sub];
@@ -1183,21 +1186,29 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
     return OCRHIP_OK;
 }
 
-// Rows of up to 128 classes and 16 entries: 16 lanes a row (97 classes, 10 entries, 1.4M rows 344 us; a wave a row 1723).  Rows
-// in LDS: one wave up to 16 KB (float32, 32 entries, 134M classes in all: 2000 classes 197 us against 251 of two waves, 418 of
-// four; 4000 208 against 188 and 248; bfloat16 4000 classes 114 against 152), four up to 32 KB (6719 classes 198 against 263
-// of one, 203 of two).  Beyond: eight waves on a row that is read twice (8000 float32 classes: 288 against 186 in LDS).
+// Rows of up to 128 classes: 16, 32 or 64 lanes a row, as many as entries (97 float32 classes, 1.4M rows, 10 entries: 344 us
+// against 1723 of a wave a row; 0.7M rows: 32 entries 292 against 672, 64 entries 559 against 677, where the row is also a
+// wave's but the next one's loads are on their way).  Rows in LDS: one wave up to 16 KB (float32, 32 entries, 134M classes in
+// all: 2000 classes 197 us against 251 of two waves, 418 of four; 4000 208 against 188 and 248; bfloat16 4000 classes 114
+// against 152), four up to 32 KB (6719 classes 198 against 263 of one, 203 of two).  Beyond: eight waves on a row that is read
+// twice (8000 float32 classes: 288 against 186 in LDS).
 template <class T>
 int launch_distill(const DistillArgs<T>& a, hipStream_t s) {
     constexpr int P = kPiece<T>;
     const size_t bits = (size_t)(a.V + 31) / 32 * 4, row_lds = (size_t)(a.V + P - 1) / P * 16;
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
-    const unsigned groups = (unsigned)std::min<int64_t>((a.rows + 15) / 16, 2048);          // 8 per compute unit, which walk the rows
+    const int lanes = a.K <= 16 ? 16 : a.K <= 32 ? 32 : 64;
+    const unsigned groups = (unsigned)std::min<int64_t>((a.rows + 256 / lanes - 1) / (256 / lanes), 2048);   // 8 per compute unit, which walk the rows
     if (a.K <= 16 && a.V < P)
-        hipLaunchKernelGGL((distill_short_kernel<T, true>), dim3(groups), dim3(256), 0, s, a);
-    else if (a.K <= 16 && a.V <= kShort)
-        hipLaunchKernelGGL((distill_short_kernel<T, false>), dim3(groups), dim3(256), 0, s, a);
-    else if (a.V < P)
+        hipLaunchKernelGGL((distill_short_kernel<T, true, 16>), dim3(groups), dim3(256), 0, s, a);
+    else if (a.V >= P && a.V <= kShort) {
+        if (lanes == 16)
+            hipLaunchKernelGGL((distill_short_kernel<T, false, 16>), dim3(groups), dim3(256), 0, s, a);
+        else if (lanes == 32)
+            hipLaunchKernelGGL((distill_short_kernel<T, false, 32>), dim3(groups), dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((distill_short_kernel<T, false, 64>), dim3(groups), dim3(256), 0, s, a);
+    } else if (a.V < P)
         hipLaunchKernelGGL((distill_lds_kernel<T, 1, 1, true>), dim3(grid), dim3(64), row_lds, s, a);
     else if (row_lds <= 2048)
         hipLaunchKernelGGL((distill_lds_kernel<T, 1, 2, false>), dim3(grid), dim3(64), row_lds, s, a);
