@@ -6,18 +6,17 @@
 //              the division is exact, so the only rounding is that to four significant bits.
 //   product:   C[m,n] = sum over blocks j of 2^(ea[m,j] + eb[n,j]) * sum over k in j of A[m,k] * B[n,k]  (+ bias[n])
 //
-// The scales are powers of two because the matrix instruction takes those itself (one exponent byte per row and 32 values
-// of k): the products of all blocks then add up in ONE float32 accumulator, without a multiply-add of every accumulator by
-// a float scale after each block.  A float scale would use the range of e4m3 better by less than a factor of 2, which a
+// The scales are powers of two because a value times its scale is then a bfloat16 number, and the conversion instruction takes
+// the scale itself: the products of all blocks add up in ONE float32 accumulator, without a multiply-add of every accumulator
+// by a float scale after each block.  A float scale would use the range of e4m3 better by less than a factor of 2, which a
 // floating type does not need: the relative rounding error is 2^-4 at any magnitude.
 //
-// Two forms of the product, chosen by the type of the result:
-//   bfloat16 result: v_mfma_scale_f32_16x16x128_f8f6f4 on the bytes.  The 8-bit matrix instructions add the products of a
-//     group of neighbouring values of k (at most 16) aligned to the largest of them and keep 13 bits below it (measured: a
-//     product 2^-14 of its neighbour's is lost, one 16 places further is not; group sums and the accumulator are float32).
-//     That is 1e-4 of the result at most for ordinary data, a fortieth of the rounding to bfloat16 that follows.
-//   float32 result: the bytes times their scale are converted to bfloat16 on the way from LDS (exact: 4 significant bits)
-//     and multiplied by v_mfma_f32_16x16x32_bf16, which keeps float32 throughout, at half the rate.
+// Sums are float32: the bytes times their scale are converted to bfloat16 on the way from LDS (exact: 4 significant bits) and
+// multiplied by v_mfma_f32_16x16x32_bf16.  The 8-bit matrix instructions, at twice its rate, would not do: they add the
+// products of a group of neighbouring values of k (at most 16) aligned to the largest of them and keep 13 bits below it
+// (measured, with and without scales: a product 2^-14 of its neighbour's is lost, one 16 places further is not).  448 * 448 -
+// 448 * 448 + 4 gave 0, and 3.8 % of a large product's bfloat16 results were other roundings than those of float32 sums.  The
+// price: 8192^3 into bfloat16 takes 875 us instead of 440, 2048^3 23 instead of 15, 79872 x 256 x 512 25 as before.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -364,20 +363,15 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k)
                     a[i][e] = (int)pack4_e4m3(no_infinity(v[4 * e] * inv), no_infinity(v[4 * e + 1] * inv), no_infinity(v[4 * e + 2] * inv), no_infinity(v[4 * e + 3] * inv));
             }
         }
-        if constexpr (OUT_F32) {
-            const float fb = scale_float(sb);
-            bf16x8 bv[4];
+        const float fb = scale_float(sb);
+        bf16x8 bv[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) bv[t] = to_bf16(b[2 * t], b[2 * t + 1], fb);
+        for (int t = 0; t < 4; ++t) bv[t] = to_bf16(b[2 * t], b[2 * t + 1], fb);
 #pragma unroll
-            for (int i = 0; i < IM; ++i) {
-                const float fa = scale_float(sa[i]);
+        for (int i = 0; i < IM; ++i) {
+            const float fa = scale_float(sa[i]);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[t], to_bf16(a[i][2 * t], a[i][2 * t + 1], fa), acc[i], 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < IM; ++i) acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a[i], acc[i], 0, 0, 0, sb, 0, sa[i]);
+            for (int t = 0; t < 4; ++t) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[t], to_bf16(a[i][2 * t], a[i][2 * t + 1], fa), acc[i], 0, 0, 0);
         }
     }
     // B is the row operand: lane r holds C[i * 16 + r][n0 + 4 kg + e]
@@ -417,10 +411,10 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k)
 // beyond the descriptor: zeros.
 // B is the matrix instruction's row operand, A its column operand: a lane then holds 4 neighbouring columns of one row.
 //
-// Measured: bfloat16 8192^3 441 us (2.5 PFLOP/s of the 8-bit instruction's 5; a large library product of one scale per
-// tensor reaches 2.9).  float32, bound by the conversions and matrix instructions beside the operands' loads: 6719 x 256 x
-// 16384 73 us (0.78 PFLOP/s with the join of 4 pieces).  16384 x 6719 x 256: 108 us with rows of whole lines (6720 columns
-// apart: 4.1 TB/s, bound by writing), 141 us with rows that start anywhere in one, whose ends two tiles write.
+// Measured: bound by the conversions and matrix instructions beside the operands' loads, 8192^3 into bfloat16 875 us (1.26
+// PFLOP/s; a large bfloat16 library product reaches 1.37), 6719 x 256 x 16384 into float32 73 us (0.78 PFLOP/s with the join of
+// 4 pieces).  16384 x 6719 x 256 into float32: 108 us with rows of whole lines (6720 columns apart: 4.1 TB/s, bound by
+// writing), 141 us with rows that start anywhere in one, whose ends two tiles write.
 struct TileArgs {
     GemmArgs g;
     int tiles_m, tiles_n, splits, kb_split;       // kb_split: blocks of k per split
@@ -586,46 +580,26 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
         const unsigned char* psa = base + (BM + BN) * kBlk + a_row;
         const unsigned char* psb = base + (BM + BN) * kBlk + 256 + b_row;
         const int sw = place(r);                        // rows 16 apart have the same permutation
-        if constexpr (OUT_F32) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {               // 16 of the lane's 32 bytes: two instructions of 32 values of k
-                const int at = ((2 * kg + h) ^ sw) * 16;
-                bf16x8 bv[IN][2];
-#pragma unroll
-                for (int j = 0; j < IN; ++j) {
-                    const intx4 q = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at);
-                    const float f = scale_float(BROWS == 1 ? (int)psb[j * 16] : sb);
-                    bv[j][0] = to_bf16(q[0], q[1], f);
-                    bv[j][1] = to_bf16(q[2], q[3], f);
-                }
-#pragma unroll
-                for (int i = 0; i < IM; ++i) {
-                    const intx4 q = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at);
-                    const float f = scale_float((int)psa[i * 16]);
-                    const bf16x8 a0 = to_bf16(q[0], q[1], f), a1 = to_bf16(q[2], q[3], f);
-#pragma unroll
-                    for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j][0], a0, acc[i][j], 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j][1], a1, acc[i][j], 0, 0, 0);
-                }
-            }
-        } else {
-            const int at0 = ((2 * kg) ^ sw) * 16, at1 = ((2 * kg + 1) ^ sw) * 16;
-            intx8 bv[IN];
-            int sbv[IN];
+        for (int h = 0; h < 2; ++h) {                   // 16 of the lane's 32 bytes: two instructions of 32 values of k
+            const int at = ((2 * kg + h) ^ sw) * 16;
+            bf16x8 bv[IN][2];
 #pragma unroll
             for (int j = 0; j < IN; ++j) {
-                const intx4 lo4 = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at0), hi4 = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at1);
-                bv[j] = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
-                sbv[j] = BROWS == 1 ? (int)psb[j * 16] : sb;
+                const intx4 q = *reinterpret_cast<const intx4*>(pb + j * 16 * kBlk + at);
+                const float f = scale_float(BROWS == 1 ? (int)psb[j * 16] : sb);
+                bv[j][0] = to_bf16(q[0], q[1], f);
+                bv[j][1] = to_bf16(q[2], q[3], f);
             }
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
-                const intx4 lo4 = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at0), hi4 = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at1);
-                const intx8 av = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
-                const int sa = psa[i * 16];
+                const intx4 q = *reinterpret_cast<const intx4*>(pa + i * 16 * kBlk + at);
+                const float f = scale_float((int)psa[i * 16]);
+                const bf16x8 a0 = to_bf16(q[0], q[1], f), a1 = to_bf16(q[2], q[3], f);
 #pragma unroll
-                for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv[j], av, acc[i][j], 0, 0, 0, sbv[j], 0, sa);
+                for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j][0], a0, acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j][1], a1, acc[i][j], 0, 0, 0);
             }
         }
     }
@@ -764,10 +738,11 @@ struct TilePlan {
 
 // Which tiles a product of M > kMaxRows rows takes, and into how many pieces of k it is split.
 //
-// Tiles of 256 x 256 (bfloat16 results; one workgroup per compute unit) read their operands half as often: from 192 tiles on
-// they win or are level (4096^3 67 us against 77 of 128 x 128, 131072 x 1024 x 256 67 against 77, 4096 x 3200 x 512 16 against
-// 15), below that they leave compute units idle (3000 x 3000 x 1024: 47 against 20).  float32 results need twice the
-// registers for the converted operands: 128 x 128 throughout.
+// Tiles of 256 x 256 (bfloat16 results; one workgroup per compute unit) read their operands half as often.  They win where
+// they fill their rounds of the 256 compute units to nine tenths (8192^3 875 us against 976 of 128 x 128, 4096^3 108 against
+// 115, 131072 x 1024 x 256 85 against 92) and lose where the last round leaves compute units idle (5000 x 5000 x 640, 400 tiles,
+// 44 against 40; 79872 x 256 x 512, 312 tiles, 36 against 25; 4096 x 3200 x 512, 208 tiles, 22 against 20).  float32 results
+// take 128 x 128 throughout.
 //
 // Pieces of k: a workgroup takes 1.05 us per block of k as long as it has its compute unit to itself and 1.6 us when two
 // share one; joining the pieces costs a launch, 2.5 us, and 0.27 us per MB of partial sums (written and read).  What comes
@@ -778,7 +753,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
     TilePlan p;
     const int64_t nkb = (K + kBlk - 1) / kBlk;
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    const bool large = !out_f32 && big >= 192;
+    const bool large = !out_f32 && 10 * big >= 9 * 256 * ((big + 255) / 256);
     p.bm = large ? 256 : 128;
     p.bn = large ? 256 : 128;
     p.tiles_m = (M + p.bm - 1) / p.bm;

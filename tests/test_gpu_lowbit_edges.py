@@ -1,0 +1,49 @@
+"""8-bit products and distillation on the GPU, at the edges of what their documentation settles: sums that cancel, values at
+the ends of the range, rows without a finite logit, masses other than 1, operands inside wider buffers."""
+import ctypes
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip('torch')
+
+from oracle import lowbit  # noqa: E402
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope='module')
+def ctx():
+    from ocr_amd.engine import HipContext
+    c = HipContext(0)
+    yield c
+    c.close()
+
+
+# --------------------------------------------------------------------------------------- product
+# few rows; tiles of 128; k in pieces; tiles of 256 (510 of them on 256 compute units, three blocks of k)
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('block_rows', [1, 128])
+@pytest.mark.parametrize('mnk', [(1, 97, 16), (40, 70, 384), (64, 33, 1024), (200, 130, 384), (300, 97, 1280), (4100, 7600, 384)])
+def test_products_that_cancel_leave_the_small_ones(ctx, mnk, block_rows, out_dtype):
+    """Every group of 16 neighbours in k holds 448 * 448, its negative and one product i j, |i| <= 7, |j| <= 2, at places of
+    their own.  All products are integers and every partial sum, in any order, is below K / 16 (448^2 + 14) < 2^24 for K up to
+    1280: a float32 holds it, so the sums are exact and the result is the exact integer, rounded once."""
+    m, n, k = mnk
+    g = torch.Generator().manual_seed(m + n + k)
+    groups = k // 16
+    at = torch.stack([torch.randperm(16, generator=g)[:3] for _ in range(groups)]) + 16 * torch.arange(groups)[:, None]
+    a, b = torch.zeros(m, k), torch.zeros(n, k)
+    a[:, at[:, 0]], a[:, at[:, 1]], b[:, at[:, 0]], b[:, at[:, 1]] = 448.0, 448.0, 448.0, -448.0
+    small_a = torch.randint(-7, 8, (m, groups), generator=g).float()
+    small_b = torch.randint(-2, 3, (n, groups), generator=g).float()
+    a[:, at[:, 2]], b[:, at[:, 2]] = small_a, small_b
+    want = (small_a.cuda() @ small_b.cuda().t().contiguous()).to(out_dtype)      # integers: exact
+    aq, bq = ctx.quantize_fp8(a.cuda()), ctx.quantize_fp8(b.cuda(), block_rows=block_rows)
+    assert torch.equal(aq.q[:, :k].float().cpu(), a) and torch.equal(bq.q[:, :k].float().cpu(), b)
+    assert torch.equal(ctx.gemm_fp8(aq, bq, out_dtype=out_dtype), want)
+    if m <= 300:
+        assert torch.equal(ctx.linear_fp8(a.cuda(), bq, out_dtype=out_dtype), want)
+        assert torch.equal(ctx.linear_fp8(a.bfloat16().cuda(), bq, out_dtype=out_dtype), want)
