@@ -48,7 +48,7 @@ SOURCES = {
     'metrics.hip': ['-ffp-contract=off'],
     'rnms.hip': ['-ffp-contract=off'],
 }
-HEADERS = ['common.h', os.path.join('..', '..', 'include', 'ocrhip.h')]
+HEADERS = ['common.h', 'scale_window.h', os.path.join('..', '..', 'include', 'ocrhip.h')]
 
 
 def _mtime(p):

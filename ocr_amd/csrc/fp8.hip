@@ -22,6 +22,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "scale_window.h"
 
 namespace ocrhip {
 
@@ -527,11 +528,11 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
             copy16(c < NA ? ra : rb, base + c * 1024, src[i], (kb - in.kb0) * kBlk);
         }
         if (wave == 0) {
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.as + (int64_t)kb * g.ldas + in.m0), 0, (unsigned)min((int64_t)BM, g.ldas - in.m0), 0x00020000);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.as + (int64_t)kb * g.ldas + in.m0), 0, (unsigned)scale_window(BM, g.M, in.m0), 0x00020000);
             copy4(rs, base + (BM + BN) * kBlk, lane * 4);
         }
         if (BROWS == 1 && wave == WAVES - 1) {
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.bs + (int64_t)kb * g.ldbs + in.n0), 0, (unsigned)min((int64_t)BN, g.ldbs - in.n0), 0x00020000);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(g.bs + (int64_t)kb * g.ldbs + in.n0), 0, (unsigned)scale_window(BN, g.N, in.n0), 0x00020000);
             copy4(rs, base + (BM + BN) * kBlk + 256, lane * 4);
         }
     };

@@ -47,3 +47,21 @@ def test_products_that_cancel_leave_the_small_ones(ctx, mnk, block_rows, out_dty
     if m <= 300:
         assert torch.equal(ctx.linear_fp8(a.cuda(), bq, out_dtype=out_dtype), want)
         assert torch.equal(ctx.linear_fp8(a.bfloat16().cuda(), bq, out_dtype=out_dtype), want)
+
+
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('block_rows', [1, 128])
+@pytest.mark.parametrize('mnk', [(5, 40, 300), (65, 129, 300), (130, 67, 1000), (300, 97, 2048)])
+def test_operands_are_the_last_columns_of_wider_buffers(ctx, mnk, block_rows, out_dtype):
+    """Bytes and scales of both operands end where their buffers end; what lies in front are other columns (NaN)."""
+    m, n, k = mnk
+    g = torch.Generator().manual_seed(k)
+    a = ctx.quantize_fp8(torch.randn(m, k, generator=g).cuda())
+    w = ctx.quantize_fp8(torch.randn(n, k, generator=g).cuda(), block_rows=block_rows)
+
+    def last_columns(t, wider):
+        big = torch.full((t.shape[0], t.shape[1] + wider), 255, dtype=torch.uint8, device='cuda')
+        big[:, wider:] = t.view(torch.uint8)
+        return big[:, wider:]
+    wide = [x._replace(q=last_columns(x.q, 256), scale=last_columns(x.scale, 944)) for x in (a, w)]
+    assert torch.equal(ctx.gemm_fp8(*wide, out_dtype=out_dtype), ctx.gemm_fp8(a, w, out_dtype=out_dtype))
