@@ -426,7 +426,8 @@ int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t 
  *       temperature - lse), everything outside the entries is one more class with p_rest = max(0, 1 - sum p_k) and q_rest
  *       = the sum of q there (none when the entries name all V classes);  loss as above plus p_rest log(p_rest / q_rest),
  *       grad_v = weight * temperature * q_v * (1 - p_rest / q_rest) outside the entries
- * An entry whose class lies outside [0, V) is none, one whose logit is -infinity has p_k = 0; several entries of one
+ * An entry whose class lies outside [0, V) is none, one whose logit is -infinity has p_k = 0 (whatever the log normaliser: a
+ * teacher's row without a finite logit, whose lse is -infinity as well, has p_rest = 1); several entries of one
  * class add up.  Without d_top_lse a row whose entries carry no probability (none, or all -infinity) has loss 0 and
  * gradient 0.  A row with weight 0 has both 0 and is not read.  A class with p > 0 and q = 0 makes the loss +infinity.
  * A NaN or +infinity among the logits or the entries' values makes the row's loss and gradient NaN.

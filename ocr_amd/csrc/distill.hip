@@ -703,7 +703,7 @@ __device__ __forceinline__ Teacher teacher_of(bool there, float z, bool has_lse,
     Teacher o;
     o.any = true;
     if (has_lse) {
-        o.log_p = there ? fma((double)z, inv_t, -(double)lse) : -INFINITY;
+        o.log_p = there && z != -INFINITY ? fma((double)z, inv_t, -(double)lse) : -INFINITY;       // lse may be -infinity too
         o.p = exp64(o.log_p);
         o.mass = group_sum<G>(o.p);
         o.rest = o.mass >= 1.0 ? 0.0 : 1.0 - o.mass;

@@ -1,17 +1,12 @@
 """8-bit products and distillation on the GPU, at the edges of what their documentation settles: sums that cancel, values at
 the ends of the range, rows without a finite logit, masses other than 1, operands inside wider buffers."""
-import ctypes
-
-import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from oracle import lowbit  # noqa: E402
-
-U = 2.0 ** -24
+from test_gpu_lowbit import check_distill, logits, teacher_of  # noqa: E402
 
 
 @pytest.fixture(scope='module')
@@ -65,3 +60,30 @@ def test_operands_are_the_last_columns_of_wider_buffers(ctx, mnk, block_rows, ou
         return big[:, wider:]
     wide = [x._replace(q=last_columns(x.q, 256), scale=last_columns(x.scale, 944)) for x in (a, w)]
     assert torch.equal(ctx.gemm_fp8(*wide, out_dtype=out_dtype), ctx.gemm_fp8(a, w, out_dtype=out_dtype))
+
+
+# ---------------------------------------------------------------------------------- distillation
+# one row length for each form: 16, 32 and 64 lanes a row, a row in LDS on one wave and on four, a row read twice
+FORMS = [(97, 6), (97, 30), (97, 50), (3, 3), (3, 20), (1000, 6), (6719, 6), (40000, 6)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('v,k', FORMS)
+@pytest.mark.filterwarnings('ignore:invalid value encountered in subtract')      # the tolerance's own p_rest of those rows
+def test_a_teacher_row_without_a_finite_logit(ctx, v, k, dtype):
+    """What ocrhip_top_logits returns for it (entries and log normaliser -infinity): entries without probability, so with the
+    normaliser everything lies outside them, and without it the row counts nothing."""
+    t = 2.0
+    x = logits(4, v, v, dtype).cuda()
+    teacher = logits(4, v, v + 1).cuda()
+    teacher[1:3] = -float('inf')
+    n = min(k, v)
+    z, i, lse = ctx.top_logits(teacher, n, temperature=t)
+    assert (z[1:3] == -float('inf')).all() and (lse[1:3] == -float('inf')).all()
+    if n < k:
+        z = torch.cat([z, torch.zeros(4, k - n, device='cuda')], 1)
+        i = torch.cat([i, torch.full((4, k - n), -1, dtype=torch.int32, device='cuda')], 1)
+    for l in (lse, None):
+        out = check_distill(ctx, x, z, i, l, t, None)
+        assert torch.isfinite(out['loss']).all() and torch.isfinite(out['grad'].float()).all()
+        assert l is not None or not (out['loss'][1:3].any() or out['grad'][1:3].any())
