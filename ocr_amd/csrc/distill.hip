@@ -751,7 +751,7 @@ __device__ __forceinline__ RowResult row_result(const Teacher& t, int K, bool th
         const bool rest = t.rest != 0.0 && __popcll(group_ballot<G>(first)) != V;
         loss += (t.mass + (rest ? t.rest : 0.0)) * log64(total);
         if (rest && m_r == -INFINITY)
-            loss = INFINITY;
+            loss += INFINITY;                              // a NaN of the entries stays one
         else if (rest) {
             const double ratio = t.rest * rcp64(sum_r);
             loss += t.rest * (log64(ratio) - d_r);

@@ -87,3 +87,19 @@ def test_a_teacher_row_without_a_finite_logit(ctx, v, k, dtype):
         out = check_distill(ctx, x, z, i, l, t, None)
         assert torch.isfinite(out['loss']).all() and torch.isfinite(out['grad'].float()).all()
         assert l is not None or not (out['loss'][1:3].any() or out['grad'][1:3].any())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('v,k', [f for f in FORMS if f[1] < f[0]])
+def test_a_nan_next_to_a_rest_without_mass(ctx, v, k, dtype):
+    """Nothing finite outside the entries and p_rest > 0: an infinite loss, but NaN with a NaN or +infinity among the student's
+    logits or the teacher's entries."""
+    x = torch.full((6, v), -float('inf'))
+    z, i = torch.zeros(6, k), torch.arange(k, dtype=torch.int32).repeat(6, 1)
+    x[:, :k] = torch.randn(6, k, generator=torch.Generator().manual_seed(v + k))
+    lse = torch.full((6,), float(torch.log(torch.tensor(float(k)))) + 1.0)
+    x[1, k - 1], z[2, 0], x[3, 0], z[4, k // 2] = float('nan'), float('nan'), float('inf'), float('inf')
+    x[5, v - 1] = float('nan')
+    out = ctx.distill_loss(x.to(dtype).cuda(), z.cuda(), i.cuda(), top_lse=lse.cuda(), want_grad=True)
+    assert out['loss'][0] == float('inf') and torch.isnan(out['loss'][1:]).all()
+    assert not torch.isnan(out['grad'][0]).any() and torch.isnan(out['grad'][1:]).all()
