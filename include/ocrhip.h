@@ -414,7 +414,7 @@ int ocrhip_linear_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t ld_
  * ranks above every number, as in a descending sort), and the row's log normaliser at a temperature.
  *   d_logits: device float32 or bfloat16 (dtype), row r at d_logits + r * ld elements, V classes, 1 <= V <= 262144
  *   d_values: device (rows, K) float32;  d_index: device (rows, K) int32;  1 <= K <= 64, K <= V
- *   d_lse   : device (rows) float32 = log sum_v exp(logit_v / temperature), or NULL;  temperature > 0, finite */
+ *   d_lse   : device (rows) float32 = log sum_v exp(logit_v / temperature), or NULL;  temperature finite, >= 4.3e-39 */
 int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t rows, int V, int64_t ld, int K,
                       float temperature, float* d_values, int* d_index, float* d_lse, ocrhip_stream stream);
 
@@ -433,7 +433,7 @@ int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t 
  * A NaN or +infinity among the logits or the entries' values makes the row's loss and gradient NaN.
  *   d_logits    : device float32 or bfloat16 (dtype), row r at d_logits + r * ld elements, 1 <= V <= 262144
  *   d_top_values: device (rows, K) float32, d_top_index: device (rows, K) int32, in any order;  1 <= K <= 64
- *   d_row_weight: device (rows) float32 or NULL (1);  d_loss: device (rows) float32 or NULL
+ *   d_row_weight: device (rows) float32 or NULL (1);  d_loss: device (rows) float32 or NULL;  temperature as above
  *   d_grad      : of d_logits' type, row r at d_grad + r * ld_grad elements, or NULL; must not overlap d_logits */
 int ocrhip_distill_loss(ocrhip_handle h, const void* d_logits, int dtype, int64_t rows, int V, int64_t ld,
                         const float* d_top_values, const int* d_top_index, int K, const float* d_top_lse,

@@ -1362,7 +1362,10 @@ int check_apart(const char* who, const void* c, int64_t M, int64_t c_ld, int64_t
 int check_rows(const char* who, const void* x, int dtype, int64_t rows, int V, int64_t ld, int K, float temperature) {
     OCR_REQUIRE(V >= 1 && V <= 262144, "%s: %d classes (1 .. 262144)", who, V);
     OCR_REQUIRE(K >= 1 && K <= 64, "%s: %d entries per row (1 .. 64)", who, K);
-    OCR_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(1.0f / temperature), "%s: temperature must be positive and finite (got %g)", who, (double)temperature);
+    // the kernels multiply by log2(e) / temperature, which has to be a float32 number too
+    constexpr float kLog2e = 1.44269504088896340736f;
+    OCR_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(kLog2e / temperature) && std::isfinite(1.0f / temperature * kLog2e),
+                "%s: temperature must be finite and at least 4.3e-39 (got %g)", who, (double)temperature);
     return check_values(who, "logits", x, dtype, rows, V, ld);
 }
 }  // namespace

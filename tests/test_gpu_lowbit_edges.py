@@ -103,3 +103,20 @@ def test_a_nan_next_to_a_rest_without_mass(ctx, v, k, dtype):
     out = ctx.distill_loss(x.to(dtype).cuda(), z.cuda(), i.cuda(), top_lse=lse.cuda(), want_grad=True)
     assert out['loss'][0] == float('inf') and torch.isnan(out['loss'][1:]).all()
     assert not torch.isnan(out['grad'][0]).any() and torch.isnan(out['grad'][1:]).all()
+
+
+@pytest.mark.parametrize('v,k', FORMS)
+def test_extreme_temperatures(ctx, v, k):
+    """At 4.3e-39 only the largest logit is left, at 3e38 all are alike: log sum exp(x / t) = max / t and log V, to half a step; the
+    gradient t (q - p) has no NaN."""
+    k = min(k, v)
+    x = torch.zeros(2, v)
+    x[0, v // 2], x[1, v - 1] = 1.0, 0.5
+    for t in (4.3e-39, 3e38):
+        for dtype in (torch.float32, torch.bfloat16):
+            val, idx, lse = ctx.top_logits(x.to(dtype).cuda(), k, temperature=t)
+            assert idx[:, 0].tolist() == [v // 2, v - 1] and val[:, 0].tolist() == [1.0, 0.5]
+            want = torch.tensor([1.0, 0.5]).double() / torch.tensor(t).double() if t < 1 else torch.full((2,), v).double().log()
+            assert ((lse.cpu().double() - want).abs() <= 2.0 ** -22 * want).all()       # exp and sum 2^-23 of 1 + log V each, the store
+            out = ctx.distill_loss(x.to(dtype).cuda(), val, idx, top_lse=lse, temperature=t, want_grad=True)
+            assert not torch.isnan(out['loss']).any() and not torch.isnan(out['grad'].float()).any()
