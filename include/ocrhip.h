@@ -425,7 +425,8 @@ int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t 
  *   d_top_lse (the teacher's log normaliser at this temperature, as ocrhip_top_logits returns it): p_k = exp(logit_k /
  *       temperature - lse), everything outside the entries is one more class with p_rest = max(0, 1 - sum p_k) and q_rest
  *       = the sum of q there (none when the entries name all V classes);  loss as above plus p_rest log(p_rest / q_rest),
- *       grad_v = weight * temperature * q_v * (1 - p_rest / q_rest) outside the entries
+ *       its derivative grad_v = weight * temperature * (P q_v - p_v), and weight * temperature * q_v * (P - p_rest / q_rest)
+ *       outside the entries, P = sum p_k + p_rest (1, unless sum p_k exceeds it or the entries name all V classes)
  * An entry whose class lies outside [0, V) is none, one whose logit is -infinity has p_k = 0 (whatever the log normaliser: a
  * teacher's row without a finite logit, whose lse is -infinity as well, has p_rest = 1); several entries of one
  * class add up.  Without d_top_lse a row whose entries carry no probability (none, or all -infinity) has loss 0 and

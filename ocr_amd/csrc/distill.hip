@@ -7,7 +7,8 @@
 //   p_k = exp(z_k / tau - lse) and one more class p_rest = 1 - sum p_k for everything outside the entries
 //   q   = softmax(s / tau);  q_rest = sum of q outside the entries
 //   loss = w tau^2 (sum_k p_k log(p_k / q_(i_k)) [+ p_rest log(p_rest / q_rest)])
-//   d loss / d s_v = w tau (q_v - p_v) for the entries, w tau q_v (1 [- p_rest / q_rest]) outside them
+//   d loss / d s_v = w tau (P q_v - p_v) for the entries, w tau q_v (P [- p_rest / q_rest]) outside them, P = sum_k p_k
+//   [+ p_rest], which is 1 but where the entries' mass exceeds it or they name every class
 //
 // Where teacher and student nearly agree the loss is far smaller than the terms it is the sum of.  The sums over the
 // classes outside the entries are float32: an error there changes the loss only in proportion to q_rest - p_rest.  What
@@ -746,10 +747,13 @@ __device__ __forceinline__ RowResult row_result(const Teacher& t, int K, bool th
     if (m_r != m && m_r != -INFINITY) shift = exp64(d_r);
     const double total = group_sum<G>(e_k) + sum_r * shift, inv_total = rcp64(total);
     double loss = group_sum<G>(t.p == 0.0 ? 0.0 : t.p * (t.log_p - d_k));
-    double coef = shift * inv_total;
+    double of_q = inv_total, coef = shift * inv_total;
     if (has_lse) {
         const bool rest = t.rest != 0.0 && __popcll(group_ballot<G>(first)) != V;
-        loss += (t.mass + (rest ? t.rest : 0.0)) * log64(total);
+        const double all = t.mass + (rest ? t.rest : 0.0);
+        loss += all * log64(total);
+        of_q *= all;
+        coef *= all;
         if (rest && m_r == -INFINITY)
             loss += INFINITY;                              // a NaN of the entries stays one
         else if (rest) {
@@ -772,7 +776,7 @@ __device__ __forceinline__ RowResult row_result(const Teacher& t, int K, bool th
     out.first = first;
     out.loss = t.any ? loss : 0.0;
     out.coef = !t.any ? 0.0 : loss != loss ? loss : coef;
-    out.grad_k = !t.any ? 0.0 : loss != loss ? loss : e_k * inv_total - sum_same;
+    out.grad_k = !t.any ? 0.0 : loss != loss ? loss : e_k * of_q - sum_same;
     return out;
 }
 

@@ -106,7 +106,10 @@ def distill_row(s, z, idx, lse, t, w):
             target[i] += p
         grad = q - target
         if lse is not None:
-            rest = max(0.0, 1.0 - np.exp(log_p).sum()) if not inside.all() else 0.0
+            mass = np.exp(log_p).sum()
+            rest = max(0.0, 1.0 - mass) if not inside.all() else 0.0
+            q = (mass + rest) * q                     # the loss carries (mass + rest) times the log of the student's sum
+            grad = q - target
             if not inside.all():
                 out = np.where(inside, -np.inf, log_q)
                 top = out.max()

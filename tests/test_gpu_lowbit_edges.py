@@ -1,12 +1,14 @@
 """8-bit products and distillation on the GPU, at the edges of what their documentation settles: sums that cancel, values at
 the ends of the range, rows without a finite logit, masses other than 1, operands inside wider buffers."""
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip('torch')
 
-from test_gpu_lowbit import check_distill, logits, teacher_of  # noqa: E402
+from oracle import lowbit  # noqa: E402
+from test_gpu_lowbit import U, check_distill, logits, sum_error, teacher_of  # noqa: E402
 
 
 @pytest.fixture(scope='module')
@@ -120,3 +122,47 @@ def test_extreme_temperatures(ctx, v, k):
             assert ((lse.cpu().double() - want).abs() <= 2.0 ** -22 * want).all()       # exp and sum 2^-23 of 1 + log V each, the store
             out = ctx.distill_loss(x.to(dtype).cuda(), val, idx, top_lse=lse, temperature=t, want_grad=True)
             assert not torch.isnan(out['loss']).any() and not torch.isnan(out['grad'].float()).any()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('v,k', FORMS + [(33, 33), (64, 64)])
+def test_gradient_where_the_mass_is_not_1(ctx, v, k, dtype):
+    """A log normaliser too large and too small (p of more than 1 in all, no rest), and every class named: the gradient is the
+    derivative of the loss, against the formula and against differences.
+
+    Against the formula: q is off by q (eps + eps_v) relative to itself, times the mass P, as in check_distill.  Against
+    differences along d of 0 and +-1, h = 2^-6 (s + h d exact): h^2 / 6 times a third derivative of at most 2 P, the two losses off
+    by 2u of theirs and P times the error of the logarithm each, the gradient's own error along d."""
+    t, h = 1.0, 2.0 ** -6
+    n = min(k, v)
+    x = (logits(6, v, v).cuda() * 8).round().div(8).to(dtype)          # few bits: s + h d is exact in float32
+    z, i, lse = teacher_of(ctx, x, n, t, 7)
+    lse = lse + torch.tensor([0.0, 0.5, -0.5, -1.5, -3.0, 2.0], device='cuda')
+    if n < k:
+        z = torch.cat([z, torch.zeros(6, k - n, device='cuda')], 1)
+        i = torch.cat([i, torch.full((6, k - n), -1, dtype=torch.int32, device='cuda')], 1)
+    out = ctx.distill_loss(x, z, i, top_lse=lse, temperature=t, want_grad=True)
+    s64, z64, i64, l64 = x.double().cpu().numpy(), z.double().cpu().numpy(), i.cpu().numpy(), lse.cpu().numpy()
+    loss, grad = lowbit.distill(s64, z64, i64, l64, t, None)
+    mass = np.where(i64 >= 0, np.exp(z64 - l64[:, None].astype(np.float64)), 0.0).sum(1)
+    full = np.maximum(mass, 1.0) if n < v else mass
+    rest = np.maximum(0.0, 1.0 - mass) if n < v else 0.0 * mass
+    e = np.exp(s64 - s64.max(1, keepdims=True))
+    q = e / e.sum(1, keepdims=True)
+    inside = np.zeros((6, v + 1), dtype=bool)
+    np.put_along_axis(inside, np.where(i64 >= 0, i64, v).astype(np.int64), True, 1)
+    q_rest = np.where(inside[:, :v], 0.0, q).sum(1)
+    ratio = rest / np.where(q_rest > 0, q_rest, 1.0)
+    eps = sum_error(v)
+    assert (np.abs(out['loss'].double().cpu().numpy() - loss) <= full * eps * 2 + 2 * U * np.abs(loss)).all()
+    own = 4 * U * (s64.max(1, keepdims=True) - s64) + 2.0 ** -22
+    half = 2.0 ** -8 * 1.01 if dtype == torch.bfloat16 else 0.0
+    tol = q * (full + ratio)[:, None] * (2 * eps + own + 4 * U) + (half + 2 * U) * np.abs(grad) + 1e-37
+    assert (np.abs(out['grad'].double().cpu().numpy() - grad) <= tol).all()
+    if dtype == torch.float32:
+        d = (torch.randint(0, 3, x.shape, generator=torch.Generator().manual_seed(9)) - 1).float().cuda()
+        up = ctx.distill_loss(x + h * d, z, i, top_lse=lse, temperature=t)['loss'].double().cpu().numpy()
+        down = ctx.distill_loss(x - h * d, z, i, top_lse=lse, temperature=t)['loss'].double().cpu().numpy()
+        slope = (out['grad'].double() * d).sum(1).cpu().numpy()
+        tol = h * h / 6 * 2 * full + (2 * U * (np.abs(up) + np.abs(down)) + 4 * full * eps) / (2 * h) + 4 * full * eps
+        assert (np.abs((up - down) / (2 * h) - slope) <= tol).all()

@@ -1,7 +1,9 @@
 """8-bit products and distillation, CPU side, at the edges of what their documentation settles: what the C entries accept and
 refuse there, and the plain float64 forms (oracle/lowbit.py)."""
+import numpy as np
 import pytest
 
+from oracle import lowbit
 from test_lowbit_cpu import _call
 
 
@@ -12,3 +14,25 @@ def test_temperatures(name, t, good):
     """log2(e) / temperature is a float32 number from 4.3e-39 on; below it 0 times infinity would be NaN."""
     rc, msg = _call(name, t=t)
     assert rc == -1 and (msg == 'null handle' if good else 'temperature' in msg and msg.startswith(name)), msg
+
+
+@pytest.mark.parametrize('shift', [0.7, 0.0, -0.9, -3.0])
+@pytest.mark.parametrize('every', [False, True])
+def test_plain_gradient_is_the_derivative_whatever_the_mass(shift, every):
+    """The entries' probabilities sum to less than 1, to 1 or to more (a log normaliser of another temperature), and with every
+    class named there is no rest whatever they sum to."""
+    rng = np.random.default_rng(5)
+    V, t, w = 13, 1.7, 0.6
+    s, teacher = rng.normal(0, 2, V), rng.normal(0, 2, V)
+    idx = rng.permutation(V) if every else np.array([3, 7, 1, -1, 12])
+    z = teacher[idx]
+    lse = float(np.log(np.exp(teacher / t).sum())) + shift
+    _, grad = lowbit.distill_row(s, z, idx, lse, t, w)
+    h = 1e-5
+    for v in range(V):
+        up, down = s.copy(), s.copy()
+        up[v] += h
+        down[v] -= h
+        d = (lowbit.distill_row(up, z, idx, lse, t, w)[0] - lowbit.distill_row(down, z, idx, lse, t, w)[0]) / (2 * h)
+        # truncation h^2 times a third derivative ~ 1e-10, cancellation eps / h ~ 1e-11, times the mass
+        assert abs(d - grad[v]) < 1e-8 * max(1.0, np.exp(-shift))
