@@ -429,7 +429,7 @@ int ocrhip_top_logits(ocrhip_handle h, const void* d_logits, int dtype, int64_t 
  *       outside the entries, P = sum p_k + p_rest (1, unless sum p_k exceeds it or the entries name all V classes)
  * An entry whose class lies outside [0, V) is none, one whose logit is -infinity has p_k = 0 (whatever the log normaliser: a
  * teacher's row without a finite logit, whose lse is -infinity as well, has p_rest = 1); several entries of one
- * class add up.  Without d_top_lse a row whose entries carry no probability (none, or all -infinity) has loss 0 and
+ * class add up to one p.  Without d_top_lse a row whose entries carry no probability (none, or all -infinity) has loss 0 and
  * gradient 0.  A row with weight 0 has both 0 and is not read.  A class with p > 0 and q = 0 makes the loss +infinity.
  * A NaN or +infinity among the logits or the entries' values makes the row's loss and gradient NaN.
  *   d_logits    : device float32 or bfloat16 (dtype), row r at d_logits + r * ld elements, 1 <= V <= 262144

@@ -746,7 +746,18 @@ __device__ __forceinline__ RowResult row_result(const Teacher& t, int K, bool th
     double shift = m_r == -INFINITY ? 0.0 : 1.0;
     if (m_r != m && m_r != -INFINITY) shift = exp64(d_r);
     const double total = group_sum<G>(e_k) + sum_r * shift, inv_total = rcp64(total);
-    double loss = group_sum<G>(t.p == 0.0 ? 0.0 : t.p * (t.log_p - d_k));
+    double sum_same = t.p, p_k = t.p, log_p = t.log_p;
+    if (doubled) {                                             // entries of one class add up, in its first lane
+        sum_same = 0.0;
+        for (int j = 0; j < K; ++j) {
+            const int other = __shfl(there ? idx : -1, j, G);
+            const double pj = __shfl(t.p, j, G);
+            if (there && other == idx) sum_same += pj;
+        }
+        p_k = first ? sum_same : 0.0;
+        if (first && sum_same != t.p) log_p = log64(sum_same) - (has_lse ? 0.0 : log64(t.rest));
+    }
+    double loss = group_sum<G>(p_k == 0.0 ? 0.0 : p_k * (log_p - d_k));
     double of_q = inv_total, coef = shift * inv_total;
     if (has_lse) {
         const bool rest = t.rest != 0.0 && __popcll(group_ballot<G>(first)) != V;
@@ -763,15 +774,6 @@ __device__ __forceinline__ RowResult row_result(const Teacher& t, int K, bool th
         }
     } else {
         loss += log64(total * t.rest);
-    }
-    double sum_same = t.p;
-    if (doubled) {
-        sum_same = 0.0;
-        for (int j = 0; j < K; ++j) {
-            const int other = __shfl(there ? idx : -1, j, G);
-            const double pj = __shfl(t.p, j, G);
-            if (there && other == idx) sum_same += pj;
-        }
     }
     out.first = first;
     out.loss = t.any ? loss : 0.0;

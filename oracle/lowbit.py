@@ -100,10 +100,11 @@ def distill_row(s, z, idx, lse, t, w):
         inside = np.zeros(V, dtype=bool)
         inside[[int(i) for i in idx if 0 <= i < V]] = True
         for (i, _), lp in zip(there, log_p):
-            p = np.exp(lp)
-            if p != 0:
-                loss += p * (lp - log_q[i])
-            target[i] += p
+            target[i] += np.exp(lp)
+        for i in dict.fromkeys(i for i, _ in there):           # entries of one class add up before the logarithm
+            own = [lp for (j, _), lp in zip(there, log_p) if j == i]
+            if target[i] != 0:
+                loss += target[i] * ((own[0] if len(own) == 1 else np.log(target[i])) - log_q[i])
         grad = q - target
         if lse is not None:
             mass = np.exp(log_p).sum()

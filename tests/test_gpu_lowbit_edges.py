@@ -166,3 +166,30 @@ def test_gradient_where_the_mass_is_not_1(ctx, v, k, dtype):
         slope = (out['grad'].double() * d).sum(1).cpu().numpy()
         tol = h * h / 6 * 2 * full + (2 * U * (np.abs(up) + np.abs(down)) + 4 * full * eps) / (2 * h) + 4 * full * eps
         assert (np.abs((up - down) / (2 * h) - slope) <= tol).all()
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('v,k', [f for f in FORMS if f[1] > 3])
+def test_entries_of_one_class_add_up(ctx, v, k, dtype, rest):
+    """Classes named several times - next to each other, far apart, by entries without probability, by every entry - count with
+    their whole probability; a student that agrees with the teacher's classes has the loss of its rest alone."""
+    x = logits(6, v, v, dtype).cuda()
+    z, i, lse = teacher_of(ctx, x, min(k, v), 1.0, 3)
+    if v < k:
+        z = torch.cat([z, z[:, :1].expand(6, k - v)], 1).contiguous()
+        i = torch.cat([i, i[:, :1].expand(6, k - v)], 1).contiguous()
+    i[1, 1] = i[1, 0]
+    i[2, k - 1] = i[2, 0]
+    i[3] = i[3, 0].item()
+    i[4, 1], z[4, 0] = i[4, 0], -float('inf')
+    i[5, 1], i[5, 3] = i[5, 0], i[5, 2]
+    top = x.float().gather(1, i[:, :1].long())[5, 0]
+    x[5] = -30.0
+    z[5] = -40.0                                               # row 5: all mass on one class, half of it in each of two entries
+    z[5, :2], x[5, i[5, 0].long()] = top - 0.6931472, top.to(dtype)
+    lse = torch.logsumexp(z, 1) + 0.1                          # p of less than 1 whatever the entries name
+    out = check_distill(ctx, x, z, i, lse if rest else None, 1.0, None)
+    if not rest:
+        # p = q = 1 but for what 29 times exp(-70) and log 2's rounding leave; each of the two alone would give -log 2
+        assert abs(float(out['loss'][5])) < 1e-6

@@ -36,3 +36,19 @@ def test_plain_gradient_is_the_derivative_whatever_the_mass(shift, every):
         d = (lowbit.distill_row(up, z, idx, lse, t, w)[0] - lowbit.distill_row(down, z, idx, lse, t, w)[0]) / (2 * h)
         # truncation h^2 times a third derivative ~ 1e-10, cancellation eps / h ~ 1e-11, times the mass
         assert abs(d - grad[v]) < 1e-8 * max(1.0, np.exp(-shift))
+
+
+@pytest.mark.parametrize('with_lse', [False, True])
+def test_plain_loss_of_a_class_named_twice_is_that_of_its_whole_probability(with_lse):
+    """A class's probability split over several entries (z - log 2 twice, z - log 3 three times) is the class named once; a
+    student that agrees entirely has no loss."""
+    rng = np.random.default_rng(6)
+    teacher = rng.normal(0, 2, 9)
+    lse = float(np.log(np.exp(teacher).sum())) if with_lse else None
+    once = np.arange(9)
+    split = np.concatenate([[4, 2, 4, 2, 2], [0, 1, 3, 5, 6, 7, 8]])
+    z = teacher[split] - np.array([np.log(2), np.log(3), np.log(2), np.log(3), np.log(3)] + [0.0] * 7)
+    for s in (rng.normal(0, 2, 9), teacher):
+        a, b = lowbit.distill_row(s, teacher, once, lse, 1.0, 1.0), lowbit.distill_row(s, z, split, lse, 1.0, 1.0)
+        assert abs(a[0] - b[0]) < 1e-14 * 16 and np.abs(a[1] - b[1]).max() < 1e-15 * 16
+    assert abs(b[0]) < 1e-14
