@@ -1380,9 +1380,9 @@ int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t r
     OCR_REQUIRE(transpose == 0 || transpose == 1, "quantize_fp8: transpose is 0 or 1");
     const int64_t R = transpose ? cols : rows, C = transpose ? rows : cols;
     OCR_TRY(check_blocks("quantize_fp8", "the output", d_q, ld_q, d_scale, ld_scale, block_rows, R, C, false));
-    const int64_t cb = (C + 127) / 128, x_row = cols * esize(x_dtype), x_ld = ld_x * esize(x_dtype);
-    OCR_REQUIRE(!overlap(d_x, rows, x_ld, x_row, d_q, R, ld_q, ld_q) && !overlap(d_x, rows, x_ld, x_row, d_scale, cb, ld_scale, ld_scale) &&
-                    !overlap(d_q, R, ld_q, ld_q, d_scale, cb, ld_scale, ld_scale),
+    const int64_t cb = (C + 127) / 128, rb = (R + block_rows - 1) / block_rows, x_row = cols * esize(x_dtype), x_ld = ld_x * esize(x_dtype);
+    OCR_REQUIRE(!overlap(d_x, rows, x_ld, x_row, d_q, R, ld_q, cb * 128) && !overlap(d_x, rows, x_ld, x_row, d_scale, cb, ld_scale, rb) &&
+                    !overlap(d_q, R, ld_q, cb * 128, d_scale, cb, ld_scale, rb),
                 "quantize_fp8: x, the bytes and the scales must not overlap");
     OCR_OPERATOR(h);
     return launch_quantize_fp8(d_x, x_dtype, rows, cols, ld_x, block_rows, transpose != 0, d_q, ld_q, d_scale, ld_scale, (hipStream_t)stream);

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from oracle import lowbit
-from test_lowbit_cpu import _call
+from test_lowbit_cpu import P, _call
 
 
 @pytest.mark.parametrize('name', ['top_logits', 'distill_loss'])
@@ -52,3 +52,22 @@ def test_plain_loss_of_a_class_named_twice_is_that_of_its_whole_probability(with
         a, b = lowbit.distill_row(s, teacher, once, lse, 1.0, 1.0), lowbit.distill_row(s, z, split, lse, 1.0, 1.0)
         assert abs(a[0] - b[0]) < 1e-14 * 16 and np.abs(a[1] - b[1]).max() < 1e-15 * 16
     assert abs(b[0]) < 1e-14
+
+
+@pytest.mark.parametrize('over,good', [
+    (dict(cols=32, ld_x=128, q=P + 128, ld_q=512), True),                     # x and the bytes in columns of one buffer of 512-byte rows
+    (dict(cols=32, ld_x=128, q=P + 112, ld_q=512), False),
+    (dict(cols=32, ld_x=128, q=P + 384, ld_q=512), True),
+    (dict(cols=32, ld_x=128, q=P + 400, ld_q=512), False),
+    (dict(cols=130, ld_x=132, q=64 * P, ld_q=512, x=64 * P + 9 * 512 + 256), True),      # x right behind the last row's bytes
+    (dict(cols=130, ld_x=132, q=64 * P, ld_q=512, x=64 * P + 9 * 512 + 252), False),
+    (dict(q=64 * P, ld_q=512, scale=64 * P + 256, ld_scale=512), True),       # bytes and scales in columns of one buffer
+    (dict(q=64 * P, ld_q=512, scale=64 * P + 240, ld_scale=512), False),
+    (dict(q=64 * P, ld_q=512, scale=64 * P + 496, ld_scale=512), True),
+    (dict(x=128 * P + 1024 + 12, scale=128 * P, ld_scale=1024), True),        # x right behind the last scale (10 of a row of 1024)
+    (dict(x=128 * P + 1024 + 8, scale=128 * P, ld_scale=1024), False),
+])
+def test_quantised_columns_of_a_wider_buffer_are_no_overlap(over, good):
+    """Only the columns rounded up to 128 and the scales of existing blocks are written."""
+    rc, msg = _call('quantize_fp8', **over)
+    assert rc == -1 and (msg == 'null handle' if good else 'overlap' in msg), msg
