@@ -46,6 +46,42 @@ def test_products_that_cancel_leave_the_small_ones(ctx, mnk, block_rows, out_dty
         assert torch.equal(ctx.linear_fp8(a.bfloat16().cuda(), bq, out_dtype=out_dtype), want)
 
 
+def values_64(m):
+    """Fp8Matrix -> its values in float64, on the GPU."""
+    e = m.scale[:, :-(-m.rows // m.block_rows)].double().t() - 127
+    row, col = torch.arange(m.rows, device='cuda') // m.block_rows, torch.arange(m.cols, device='cuda') // 128
+    return m.q[:, :m.cols].double() * torch.exp2(e[row][:, col])
+
+
+# Several blocks of k in workgroups that walk several tiles, the next tile's first block on its way while this one's last is
+# multiplied and its results leave: 510 tiles of 256 on 256 compute units (bfloat16), 600 and 1256 tiles of 128 on 512 workgroups.
+# Two blocks, three, five with a ragged last one; ragged last tiles in both directions.
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('block_rows', [1, 128])
+@pytest.mark.parametrize('bias', [False, True])
+@pytest.mark.parametrize('mnk', [(4100, 7600, 256), (4100, 7600, 384), (4100, 7600, 600), (3000, 3100, 256), (3000, 3100, 600), (20001, 999, 384)])
+def test_products_of_many_tiles_and_blocks(ctx, mnk, bias, block_rows, out_dtype):
+    """Every element against float64 on the GPU: float32 sums of K terms in any order, (K + 2) 2u sum |a b|, and for a bfloat16
+    result half a step of that."""
+    m, n, k = mnk
+    g = torch.Generator().manual_seed(m + k)
+    x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-4, 5, (m, 1), generator=g).float())
+    w = torch.randn(n, k, generator=g) * torch.exp2(torch.randint(-4, 5, (1, k), generator=g).float())
+    a, b = ctx.quantize_fp8(x.cuda()), ctx.quantize_fp8(w.cuda(), block_rows=block_rows)
+    v = torch.randn(n, generator=g).cuda() if bias else None
+    got = ctx.gemm_fp8(a, b, bias=v, out_dtype=out_dtype)
+    a64, b64 = values_64(a), values_64(b).t().contiguous()
+    want, mass = a64 @ b64, a64.abs() @ b64.abs()
+    if bias:
+        want, mass = want + v.double(), mass + v.double().abs()
+    tol = (k + 2) * 2 * U * mass
+    if out_dtype == torch.bfloat16:
+        tol = tol * 1.01 + 2.0 ** -8 * want.abs()
+    assert bool(((got.double() - want).abs() <= tol).all())
+    for _ in range(3):
+        assert torch.equal(ctx.gemm_fp8(a, b, bias=v, out_dtype=out_dtype), got)
+
+
 @pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('block_rows', [1, 128])
 @pytest.mark.parametrize('mnk', [(5, 40, 300), (65, 129, 300), (130, 67, 1000), (300, 97, 2048)])
