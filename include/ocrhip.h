@@ -391,7 +391,8 @@ int ocrhip_quantize_fp8(ocrhip_handle h, const void* d_x, int x_dtype, int64_t r
 /* ocrhip_gemm_fp8: C (M, N) = A (M, K) . B (N, K)^T + bias, C float32 or bfloat16.  A has a scale per row and 128 values
  * of k (block_rows 1), B per row or per 128 rows (b_block_rows 1 or 128).  A NaN in a row of A or B makes that row or
  * column of C NaN.  The sums of one call always run in the same order; they are float32, a bfloat16 result is rounded once.
- * Operand values (bytes times scale) below 2^-126 in magnitude count as 0 and from 2^128 on as infinite.
+ * Operand values (bytes times scale) count as the bfloat16 number nearest to them, which they are from 2^-130 up to 2^128:
+ * below, multiples of 2^-133; from 2^128 on, infinite.
  *   d_bias: device float32 (N) or NULL;  d_c: row m at d_c + m * ld_c elements, ld_c >= N;  M >= 0, N >= 0, 1 <= K <= 4194304 (so ld_a, ld_b)
  *   d_ws  : device scratch of ocrhip_gemm_fp8_workspace(M, N, K) bytes, 16-byte aligned (NULL when that is 0); what it
  *           holds before and after the call does not matter, calls that overlap need one each */

@@ -287,7 +287,8 @@ struct GemmArgs {
 // scale byte -> the float whose exponent field it is (what the conversion below reads)
 __device__ __forceinline__ float scale_float(int byte) { return byte ? __int_as_float(byte << 23) : __int_as_float(0x00400000); }
 
-// 8 e4m3 values of one row times the block's scale as bfloat16: 4 significant bits, so the conversion is exact
+// 8 e4m3 values of one row times the block's scale as bfloat16: 4 significant bits, so the conversion is exact (from 2^-130 up to
+// 2^128; it rounds to the multiples of 2^-133 that bfloat16 has below, and the products take those)
 __device__ __forceinline__ bf16x8 to_bf16(int lo, int hi, float scale) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, true);
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, true);

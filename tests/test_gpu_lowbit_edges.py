@@ -83,6 +83,37 @@ def test_products_of_many_tiles_and_blocks(ctx, mnk, bias, block_rows, out_dtype
 
 
 @pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('m', [5, 200])
+def test_operand_values_at_the_ends_of_the_range(ctx, m, out_dtype):
+    """Bytes times scale count as the bfloat16 number nearest to them, on either side: multiples of 2^-133 below 2^-126, infinite
+    from 2^128 on, and exact between.  One value per row, the other operand a power of two."""
+    from ocr_amd.engine import Fp8Matrix
+    # byte and exponent of the scale: around 2^-126 and 2^-133 (ties, and bits that are lost), 2^-127 as a scale, around 2^128
+    cases = [(0x08, -120), (0x04, -120), (0x0F, -120), (0x01, -117), (0x01, -124), (0x01, -125), (0x03, -125), (0x09, -127), (0x07, -127), (0x05, -126), (0x38, -126),
+             (0x37, -126), (0x40, -127), (0x3D, -127), (0x7E, -127), (0x38, 127), (0x3F, 127), (0x40, 127), (0x7E, 119), (0x7E, 120), (0x78, 120), (0xB8, -126),
+             (0x8F, -126), (0xC0, 127)]
+    table = lowbit.e4m3_table()
+    q = torch.zeros((m, 128), dtype=torch.uint8)
+    scale = torch.full((1, -(-m // 16) * 16), 127, dtype=torch.uint8)
+    for r in range(m):
+        byte, e = cases[r % len(cases)]
+        q[r, r % 128], scale[0, r] = byte, e + 127
+    one = torch.zeros((3, 128), dtype=torch.uint8)
+    one[:] = 0x38                                                     # 1
+    # powers of two that bring every value to the middle of the range: 2^120 for the small ones, 2^-120 for the large
+    other = Fp8Matrix(one.cuda().view(torch.float8_e4m3fn), torch.tensor([[247, 7, 127] + [127] * 13], dtype=torch.uint8).cuda(), 3, 128, 1)
+    small = Fp8Matrix(q.cuda().view(torch.float8_e4m3fn), scale.cuda(), m, 128, 1)
+    got = ctx.gemm_fp8(small, other, out_dtype=out_dtype).double().cpu()
+    flipped = ctx.gemm_fp8(other, small, out_dtype=out_dtype).double().cpu()
+    for r in range(m):
+        byte, e = cases[r % len(cases)]
+        n = 0 if e < 0 else 1
+        value = torch.tensor(table[byte] * 2.0 ** e, dtype=torch.float64).float().bfloat16()           # (exact in float32)
+        want = float(value) * 2.0 ** (120 if n == 0 else -120)
+        assert got[r, n] == want and flipped[n, r] == want, (r, got[r, n], want)
+
+
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('block_rows', [1, 128])
 @pytest.mark.parametrize('mnk', [(5, 40, 300), (65, 129, 300), (130, 67, 1000), (300, 97, 2048)])
 def test_operands_are_the_last_columns_of_wider_buffers(ctx, mnk, block_rows, out_dtype):
