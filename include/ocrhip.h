@@ -126,8 +126,8 @@ int ocrhip_destroy(ocrhip_handle h);
  *   through a buffer of the handle.  Same tokens and scores bit for bit.
  *   "fp8_dense": 0 (default) | 1: the bfloat16-tensor recogniser (compute_dtype OCRHIP_BF16, bf16_tensors = 1, VGG
  *   extractor) computes its dense layers - the LSTM input projections, the linear layers, Dense(vocab) - as
- *   ocrhip_linear_fp8 does: input rows quantised with a scale per 128 values, weights (quantised by
- *   ocrhip_crnn_load_weights) with a scale per 128 x 128.  Every operand is then off by up to 2^-4 of itself: logits within
+ *   ocrhip_linear_fp8 does: input rows quantised with a scale per 128 values, weights with a scale per 128 x 128 (by the call
+ *   that switches it on, which allocates and waits for the device, and by ocrhip_crnn_load_weights while it is on).  Every operand is then off by up to 2^-4 of itself: logits within
  *   0.2 of the bfloat16 recogniser's in norm (measured: 0.06).  Other forward calls do not read it. */
 int ocrhip_set_option(ocrhip_handle h, const char* name, int value);
 

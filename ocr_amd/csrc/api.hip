@@ -646,25 +646,35 @@ static std::vector<ResLayer> resnet_layers() {
 static int64_t fp8_ld(int64_t cols) { return (cols + 127) / 128 * 128; }
 static int64_t fp8_ld_scale(int64_t row_blocks) { return (row_blocks + 15) / 16 * 16; }
 
-// the 8-bit form of a dense layer's weights (cout, cin)
-static int prepare_dense_fp8(ConvLayer& L, const float* w, int cout, int cin) {
-    const int64_t ld = fp8_ld(cin), ld_scale = fp8_ld_scale((cout + 127) / 128);
-    OCR_TRY(L.w_fp8.reserve((size_t)cout * ld));
+// the 8-bit form of a dense layer's weights
+static int prepare_dense_fp8(ConvLayer& L) {
+    const int64_t ld = fp8_ld(L.cin), ld_scale = fp8_ld_scale((L.cout + 127) / 128);
+    std::vector<float> w;
+    OCR_TRY(read_dense_weights(L, w));
+    OCR_TRY(L.w_fp8.reserve((size_t)L.cout * ld));
     OCR_TRY(L.s_fp8.reserve((size_t)(ld / 128) * ld_scale));
     DevBuf src;
-    int rc = src.reserve((size_t)cout * cin * sizeof(float));
-    if (rc == OCRHIP_OK && hipMemcpy(src.ptr, w, (size_t)cout * cin * sizeof(float), hipMemcpyHostToDevice) != hipSuccess) {
-        set_error("crnn_load_weights: copying a layer's weights failed");
+    int rc = src.reserve(w.size() * sizeof(float));
+    if (rc == OCRHIP_OK && hipMemcpy(src.ptr, w.data(), w.size() * sizeof(float), hipMemcpyHostToDevice) != hipSuccess) {
+        set_error("fp8_dense: copying a layer's weights failed");
         rc = OCRHIP_EHIP;
     }
-    if (rc == OCRHIP_OK) rc = launch_quantize_fp8(src.ptr, OCRHIP_F32, cout, cin, cin, 128, false, L.w_fp8.as<uint8_t>(), ld, L.s_fp8.as<uint8_t>(), ld_scale, nullptr);
+    if (rc == OCRHIP_OK) rc = launch_quantize_fp8(src.ptr, OCRHIP_F32, L.cout, L.cin, L.cin, 128, false, L.w_fp8.as<uint8_t>(), ld, L.s_fp8.as<uint8_t>(), ld_scale, nullptr);
     // forward calls may run on streams that do not wait for the default one
     if (rc == OCRHIP_OK && hipStreamSynchronize(nullptr) != hipSuccess) {
-        set_error("crnn_load_weights: quantising a layer's weights failed");
+        set_error("fp8_dense: quantising a layer's weights failed");
         rc = OCRHIP_EHIP;
     }
     src.release();
     return rc;
+}
+
+// option fp8_dense: all of them, from the float32 weights on the device; the ResNet recogniser does not know the option
+static int crnn_prepare_fp8(CrnnNet& net) {
+    if (net.backbone || net.fp8_ready) return OCRHIP_OK;
+    for (ConvLayer* L : {&net.wih[0][0], &net.wih[0][1], &net.wih[1][0], &net.wih[1][1], &net.linear[0], &net.linear[1], &net.pred}) OCR_TRY(prepare_dense_fp8(*L));
+    net.fp8_ready = true;
+    return OCRHIP_OK;
 }
 
 int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n) {
@@ -672,7 +682,7 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
     OCR_REQUIRE(w && n > 0, "crnn_load_weights: no tensors");
     Weights W{w, n};
     CrnnNet& net = h->crnn;
-    net.loaded = false;
+    net.loaded = net.fp8_ready = false;
     std::vector<float> wf, bf;
     net.backbone = W.find("FeatureExtraction.ConvNet.conv0_1.weight") ? 1 : 0;
     net.feat_c = net.backbone ? 512 : 256;
@@ -728,7 +738,6 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
                     std::copy(wih + (size_t)(gq * Hd + u) * in_c, wih + (size_t)(gq * Hd + u + 1) * in_c, wperm.begin() + (size_t)(u * 4 + gq) * in_c);
                 }
             OCR_TRY(prepare_conv_mfma(net.wih[l][d], wperm.data(), bsum.data(), 4 * Hd, in_c, 1));
-            OCR_TRY(prepare_dense_fp8(net.wih[l][d], wperm.data(), 4 * Hd, in_c));
             OCR_TRY(net.whh[l][d].reserve((size_t)4 * Hd * Hd * sizeof(float)));
             OCR_HIP_CHECK(hipMemcpy(net.whh[l][d].ptr, whh, (size_t)4 * Hd * Hd * sizeof(float), hipMemcpyHostToDevice));
         }
@@ -736,7 +745,6 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
         OCR_TRY(get(W, pre + ".linear.weight", {Hd, 2 * Hd}, &lw));
         OCR_TRY(get(W, pre + ".linear.bias", {Hd}, &lb));
         OCR_TRY(prepare_conv_mfma(net.linear[l], lw, lb, Hd, 2 * Hd, 1));
-        OCR_TRY(prepare_dense_fp8(net.linear[l], lw, Hd, 2 * Hd));
     }
     {
         const ocrhip_tensor_desc* t = W.find("Prediction.weight");
@@ -746,10 +754,10 @@ int ocrhip_crnn_load_weights(ocrhip_handle h, const ocrhip_tensor_desc* w, int n
         const float* pb = nullptr;
         OCR_TRY(get(W, "Prediction.bias", {V}, &pb));
         OCR_TRY(prepare_conv_mfma(net.pred, t->data, pb, V, Hd, 1));
-        OCR_TRY(prepare_dense_fp8(net.pred, t->data, V, Hd));
         net.vocab = V;
         net.vocab_pad = net.pred.cout_pad;
     }
+    if (h->fp8_dense) OCR_TRY(crnn_prepare_fp8(net));
     net.loaded = true;
     return OCRHIP_OK;
 }
@@ -992,6 +1000,7 @@ static int crnn_sequence16(CrnnNet& net, const uint16_t* feats16, int n, int64_t
     OCR_TRY(net.lin.reserve((size_t)2 * R * Hd * sizeof(float)));
     OCR_TRY(net.seq16.reserve((size_t)R * 2 * Hd * sizeof(uint16_t)));
     if (fp8) {
+        OCR_REQUIRE(net.fp8_ready, "crnn: the dense layers have no 8-bit weights");
         const int64_t widest = fp8_ld(std::max(2 * Hd, net.feat_c));
         OCR_TRY(net.in8.reserve((size_t)R * widest));
         OCR_TRY(net.in8_scale.reserve((size_t)(widest / 128) * fp8_ld_scale(R)));
@@ -1541,6 +1550,7 @@ int ocrhip_set_option(ocrhip_handle h, const char* name, int value) {
     }
     if (std::strcmp(name, "fp8_dense") == 0) {
         OCR_REQUIRE(value == 0 || value == 1, "set_option: fp8_dense is 0 or 1");
+        if (value && h->crnn.loaded) OCR_TRY(crnn_prepare_fp8(h->crnn));
         h->fp8_dense = value;
         return OCRHIP_OK;
     }

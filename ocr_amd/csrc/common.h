@@ -166,6 +166,7 @@ struct CrnnNet {
     hipEvent_t aux_fork = nullptr, aux_join[kAux] = {nullptr, nullptr, nullptr};
     DevBuf feats, xw, hbuf, cbuf, seq, lin, logits, meta, lstm_counters;
     DevBuf seq16;            // bfloat16-tensor path: output rows of a BiLSTM layer (R, 2H)
+    bool fp8_ready = false;  // the dense layers' w_fp8 / s_fp8 hold the loaded weights (once fp8_dense is switched on)
     DevBuf in8, in8_scale, ws8;  // option fp8_dense: a dense layer's quantised input rows and their scales; the product's workspace
     DevBuf pmax, pidx;       // greedy decoding without logits: per row and block of 128 classes the maximum and its class
     static constexpr int kErrSlots = 16;
@@ -218,6 +219,7 @@ namespace ocrhip {
 //   up_src != nullptr: the first up_c input channels are the x2 align-corners bilinear upsampling of
 //   up_src (B,H/2,W/2,up_c) and the remaining cin - up_c channels come from x (B,H,W,cin-up_c).
 int prepare_conv_mfma(ConvLayer& L, const float* w_oihw, const float* bias, int cout, int cin, int ks);
+int read_dense_weights(const ConvLayer& L, std::vector<float>& w_oi);
 //   residual != nullptr (unpooled ks 3 / 2 only): a tensor shaped like y, added before the ReLU.
 int launch_conv_mfma(const ConvLayer& L, const float* x, float* y, int B, int H, int W, int pool, bool relu,
                      const float* up_src, int up_c, hipStream_t s, const float* residual = nullptr);

@@ -404,6 +404,22 @@ int prepare_conv_mfma(ConvLayer& L, const float* w_oihw, const float* bias, int 
     return OCRHIP_OK;
 }
 
+// The float32 weights of a layer of 1 x 1 taps, (cout, cin), back from their slabs.
+int read_dense_weights(const ConvLayer& L, std::vector<float>& w_oi) {
+    OCR_REQUIRE(!L.direct && L.ks == 1 && L.w_f32.ptr, "conv_mfma: no dense layer");
+    constexpr int CK = 32;
+    const int BN = L.cout_pad % 64 == 0 ? 64 : 32, nK = L.cin / CK;
+    std::vector<float> w((size_t)L.cout_pad * L.cin);
+    OCR_HIP_CHECK(hipMemcpy(w.data(), L.w_f32.ptr, w.size() * sizeof(float), hipMemcpyDeviceToHost));
+    w_oi.resize((size_t)L.cout * L.cin);
+    for (int o = 0; o < L.cout; ++o)
+        for (int c = 0; c < L.cin; ++c) {
+            const size_t slab = (size_t)(o / BN) * nK + c / CK;
+            w_oi[(size_t)o * L.cin + c] = w[(((slab * (CK / 8) + c % CK / 8) * 2 + c % 8 / 4) * BN + o % BN) * 4 + c % 4];
+        }
+    return OCRHIP_OK;
+}
+
 int launch_conv_mfma(const ConvLayer& L, const float* x, float* y, int B, int H, int W, int pool, bool relu,
                      const float* up_src, int up_c, hipStream_t s, const float* residual) {
     OCR_REQUIRE(!L.direct && L.w_f32.ptr, "conv_mfma: layer not prepared");
