@@ -93,11 +93,7 @@ __device__ __forceinline__ T group_sum(T v) { return reduce<G>(v, [](T a, T b) {
 template <int G>
 __device__ __forceinline__ float group_max(float v) { return reduce<G>(v, [](float a, float b) { return fmaxf(a, b); }); }
 template <int G>
-__device__ __forceinline__ double group_max(double v) { return reduce<G>(v, [](double a, double b) { return fmax(a, b); }); }
-template <int G>
 __device__ __forceinline__ unsigned group_max(unsigned v) { return reduce<G>(v, [](unsigned a, unsigned b) { return a > b ? a : b; }); }
-template <int G>
-__device__ __forceinline__ unsigned group_min(unsigned v) { return reduce<G>(v, [](unsigned a, unsigned b) { return a < b ? a : b; }); }
 // the ballot of the lane's group
 template <int G>
 __device__ __forceinline__ unsigned long long group_ballot(bool b) {
@@ -212,11 +208,12 @@ __device__ __forceinline__ double rcp64(double x) {
     return fma(fma(-x, r, 1.0), r, r);
 }
 // exp(x): x = n ln 2 + r, |r| <= ln 2 / 2, the series of exp to r^12 / 12! (the next term is 2e-16 of the value); 0 from
-// -infinity to -800, NaN stays NaN (and +infinity becomes one).
+// -infinity to -800, NaN stays NaN (and +infinity becomes one).  ln 2 is its first 40 bits behind the point, which n times are
+// exact, and the rest.
 __device__ __forceinline__ double exp64(double x) {
     x = x < -800.0 ? -800.0 : x;
     const double n = rint(x * 1.4426950408889634074);
-    const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.693147180369123816490, x));
+    const double r = fma(n, 1.7239444525614835e-13, fma(n, -0.6931471805601177, x));
     double p = 1.0 / 479001600.0;
     p = fma(p, r, 1.0 / 39916800.0);
     p = fma(p, r, 1.0 / 3628800.0);

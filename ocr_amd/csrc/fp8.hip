@@ -78,7 +78,6 @@ __device__ __forceinline__ float no_infinity(float v) { return fabsf(v) == INFIN
 // at any element.
 typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int intx4_any __attribute__((ext_vector_type(4), aligned(2)));
-typedef __bf16 bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef __bf16 bf16x8_any __attribute__((ext_vector_type(8), aligned(2)));
 
 // NV (a multiple of 8) values x[k0 ..] of a row of K, zeros beyond
@@ -303,18 +302,14 @@ __device__ __forceinline__ void store_c(void* c, int64_t at, float v) {
         reinterpret_cast<__bf16*>(c)[at] = (__bf16)v;
 }
 // 4 neighbouring columns of a row, of which `left` exist
-template <bool OUT_F32>
-__device__ __forceinline__ void store_c4(void* c, int64_t at, floatx4 v, int left) {
+__device__ __forceinline__ void store_f32x4_edge(float* p, floatx4 v, int left) {
     if (left >= 4) {
-        if (OUT_F32)
-            *reinterpret_cast<floatx4_any*>(reinterpret_cast<float*>(c) + at) = v;
-        else
-            *reinterpret_cast<bf16x4_any*>(reinterpret_cast<__bf16*>(c) + at) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        *reinterpret_cast<floatx4_any*>(p) = v;
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (e < left) store_c<OUT_F32>(c, at + e, v[e]);
+        if (e < left) p[e] = v[e];
 }
 
 // ---- few rows of A (M <= 64): bound by reading B once; up to a few MB of it by the latency of a launch and its loads (1 x 6719
@@ -639,7 +634,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
                     else if (full)
                         store_f32x4<false>(at, v);
                     else if (m_first + i * 16 + t * STEP < g.M)
-                        store_c4<true>(at, 0, v, g.N - n);
+                        store_f32x4_edge(at, v, g.N - n);
                 }
                 __builtin_amdgcn_wave_barrier();
             }
