@@ -45,11 +45,11 @@ typedef float floatx2 __attribute__((ext_vector_type(2)));
 
 // Arithmetic on two floats, one scalar instruction each: the packed float32 instructions that would do both at once have
 // given wrong results on MI355X now and then, and the library is built without them.
-__device__ __forceinline__ floatx2 pk_fma(floatx2 a, floatx2 b, floatx2 c) {
+__device__ __forceinline__ floatx2 fma2(floatx2 a, floatx2 b, floatx2 c) {
     return floatx2{__builtin_fmaf(a.x, b.x, c.x), __builtin_fmaf(a.y, b.y, c.y)};
 }
-__device__ __forceinline__ floatx2 pk_add(floatx2 a, floatx2 b) { return a + b; }
-__device__ __forceinline__ floatx2 pk_sub(floatx2 a, floatx2 b) { return a - b; }
+__device__ __forceinline__ floatx2 add2(floatx2 a, floatx2 b) { return a + b; }
+__device__ __forceinline__ floatx2 sub2(floatx2 a, floatx2 b) { return a - b; }
 
 constexpr int kCK = 8;            // input channels per chunk
 constexpr int kRS = 12;           // floats per raw pixel in LDS (8 + pad: conflict-free 16-byte reads)
@@ -182,8 +182,8 @@ __global__ __launch_bounds__(128 * CHB, CHB == 2 ? 2 : 1) void conv_wino_f32_ker
     };
     auto tr_row = [&](int c) {
         if (c < TC) {
-            tt[c][0] = pk_fma(t_sgn, tq[c].xy, tp[c].xy);
-            tt[c][1] = pk_fma(t_sgn, tq[c].zw, tp[c].zw);
+            tt[c][0] = fma2(t_sgn, tq[c].xy, tp[c].xy);
+            tt[c][1] = fma2(t_sgn, tq[c].zw, tp[c].zw);
         }
     };
     auto put2 = [&](float* u, floatx2 lo, floatx2 hi) {       // two 8-byte stores: no need for 4 consecutive registers
@@ -194,18 +194,18 @@ __global__ __launch_bounds__(128 * CHB, CHB == 2 ? 2 : 1) void conv_wino_f32_ker
         float* u = &lds[ubase + t_dst];
         if (CHB == 2) {
             if (half == 0) {
-                put2(u, pk_sub(tt[0][0], tt[2][0]), pk_sub(tt[0][1], tt[2][1]));
-                put2(u + kUC, pk_add(tt[1][0], tt[2][0]), pk_add(tt[1][1], tt[2][1]));
+                put2(u, sub2(tt[0][0], tt[2][0]), sub2(tt[0][1], tt[2][1]));
+                put2(u + kUC, add2(tt[1][0], tt[2][0]), add2(tt[1][1], tt[2][1]));
             } else {
-                put2(u + 2 * kUC, pk_sub(tt[2][0], tt[1][0]), pk_sub(tt[2][1], tt[1][1]));
-                put2(u + 3 * kUC, pk_sub(tt[1][0], tt[TC - 1][0]), pk_sub(tt[1][1], tt[TC - 1][1]));
+                put2(u + 2 * kUC, sub2(tt[2][0], tt[1][0]), sub2(tt[2][1], tt[1][1]));
+                put2(u + 3 * kUC, sub2(tt[1][0], tt[TC - 1][0]), sub2(tt[1][1], tt[TC - 1][1]));
             }
         } else {
             if (half == 0) {
-                put2(u + t_jd, pk_sub(tt[0][0], tt[2][0]), pk_sub(tt[0][1], tt[2][1]));
+                put2(u + t_jd, sub2(tt[0][0], tt[2][0]), sub2(tt[0][1], tt[2][1]));
             } else {
-                put2(u + t_je, pk_fma(t_s2, tt[2][0], pk_fma(t_s0, tt[0][0], tt[1][0])),
-                     pk_fma(t_s2, tt[2][1], pk_fma(t_s0, tt[0][1], tt[1][1])));
+                put2(u + t_je, fma2(t_s2, tt[2][0], fma2(t_s0, tt[0][0], tt[1][0])),
+                     fma2(t_s2, tt[2][1], fma2(t_s0, tt[0][1], tt[1][1])));
             }
         }
     };

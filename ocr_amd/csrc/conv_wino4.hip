@@ -532,8 +532,7 @@ __global__ __launch_bounds__(MODE == 3 ? 256 : 512, MODE == 3 ? 2 : 1) void conv
         constexpr int PW = (POOL == 1) ? 2 : 4, PH = (POOL == 0) ? 4 : 2;      // outputs a block keeps after pooling
         constexpr int kTW = 8 * PW, kTH = (NBLK / 8) * PH;                     // the tile after pooling
         constexpr int OS = NCH + 4;                                            // floats per staged pixel
-        // two of a lane's four blocks at a time (registers v and v + 1 of every accumulator: neighbours in a block row),
-        // so that the additions are packed ones
+        // two of a lane's four blocks at a time (registers v and v + 1 of every accumulator: neighbours in a block row)
         auto at4 = [](floatx2 m0, floatx2 m1, floatx2 m2, floatx2 m3, floatx2 m4, floatx2 m5, floatx2 (&o)[4]) {
             const floatx2 s1 = m1 + m2, d1 = m1 - m2, s2 = m3 + m4, d2 = m3 - m4;
             o[0] = (m0 + s1) + s2;
