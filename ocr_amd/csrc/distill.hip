@@ -10,8 +10,10 @@
 //   d loss / d s_v = w tau (P q_v - p_v) for the entries, w tau q_v (P [- p_rest / q_rest]) outside them, P = sum_k p_k
 //   [+ p_rest], which is 1 but where the entries' mass exceeds it or they name every class
 //
-// Where teacher and student nearly agree the loss is far smaller than the terms it is the sum of.  The sums over the
-// classes outside the entries are float32: an error there changes the loss only in proportion to q_rest - p_rest.  What
+// Where teacher and student nearly agree the loss is far smaller than the terms it is the sum of.  The exponentials of the
+// classes outside the entries are float32: an error there changes the loss only in proportion to q_rest - p_rest.  They are
+// added in float32 within a lane's pieces of a load (8 classes, 32 in rows that are streamed), beyond in float64, which the loads
+// hide; rows of up to 128 classes, which the vector ALU bounds, take float32 throughout (8 classes a lane, then a tree).  What
 // enters to first order (the entries' probabilities, the logarithms, the sum of the terms: K numbers per row) is float64.
 #include <algorithm>
 #include <type_traits>
@@ -930,21 +932,23 @@ template <class T, int W, int BATCH, bool TINY>
 __global__ __launch_bounds__(W * 64) void distill_lds_kernel(DistillArgs<T> a) {
     constexpr int P = kPiece<T>, THREADS = W * 64;
     extern __shared__ uintx4 buf[];
-    __shared__ float wave_top[W], wave_part[W], entry_grad[64];
+    __shared__ double wave_sum[W];
+    __shared__ float wave_top[W], entry_grad[64];
     __shared__ int entry_class[64];
     __shared__ float shared_coef;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
     const double inv_t = 1.0 / a.t;
     const float c = kLog2e / a.t;
-    auto over_waves = [&](float* part, float v, bool sum) {            // sum or maximum of the waves' values, in their order
+    auto over_waves = [&](auto* part, auto v, auto op) {                 // of the waves' values, in their order
         if (W == 1) return v;
         if (lane == 0) part[wave] = v;
         __syncthreads();
-        float o = part[0];
+        auto o = part[0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) o = sum ? o + part[i] : fmaxf(o, part[i]);
+        for (int i = 1; i < W; ++i) o = op(o, part[i]);
         return o;
     };
+    auto larger = [](float a, float b) { return fmaxf(a, b); };
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         T* g = a.grad ? a.grad + row * a.ld_grad : nullptr;
         const float w = a.weight ? a.weight[row] : 1.0f;
@@ -967,25 +971,26 @@ __global__ __launch_bounds__(W * 64) void distill_lds_kernel(DistillArgs<T> a) {
         const float own_top = row_to_lds<THREADS, BATCH, TINY>(a.x + row * a.ld, a.V, buf, [&] {
             if (wave == 0) t = teacher_of<64>(there, z, a.lse != nullptr, lse, inv_t);
         });
-        float m_r = over_waves(wave_top, group_max<64>(own_top), false);
+        float m_r = over_waves(wave_top, group_max<64>(own_top), larger);
         if (W == 1) lds_phase();
         float s_k = -INFINITY;
         bool again = false;
         if (wave == 0) s_k = take_entry<T>(buf, there, idx, lane, again);
         if (W > 1) __syncthreads();
         auto sum_of = [&](float base) {
-            float sum = 0.0f;
+            double sum = 0.0;
             for (int q = tid; q < pieces; q += THREADS) {
-                float v[P];
+                float v[P], part = 0.0f;
                 unpack_piece(buf[q], v);
 #pragma unroll
-                for (int e = 0; e < P; ++e) sum += __builtin_amdgcn_exp2f((v[e] - base) * c);
+                for (int e = 0; e < P; ++e) part += __builtin_amdgcn_exp2f((v[e] - base) * c);
+                sum += (double)part;
             }
-            return over_waves(wave_part, group_sum<64>(sum), true);
+            return over_waves(wave_sum, group_sum<64>(sum), [](double a, double b) { return a + b; });
         };
         float base = m_r == -INFINITY ? 0.0f : m_r;
-        float sum_r = sum_of(base);
-        if (sum_r < 1e-20f) {               // far below the entries: from their own maximum
+        double sum_r = sum_of(base);
+        if (sum_r < 1e-20) {               // far below the entries: from their own maximum
             m_r = -INFINITY;
             for (int q = tid; q < pieces; q += THREADS) {
                 float v[P];
@@ -993,13 +998,13 @@ __global__ __launch_bounds__(W * 64) void distill_lds_kernel(DistillArgs<T> a) {
 #pragma unroll
                 for (int e = 0; e < P; ++e) m_r = fmaxf(m_r, v[e]);
             }
-            m_r = over_waves(wave_top, group_max<64>(m_r), false);
+            m_r = over_waves(wave_top, group_max<64>(m_r), larger);
             base = m_r == -INFINITY ? 0.0f : m_r;
             sum_r = sum_of(base);
         }
         if (wave == 0) {
             // a NaN outside the entries: the maximum does not see it, the sum does
-            const RowResult r = row_result<64>(t, a.K, there, again, idx, s_k, a.lse != nullptr, inv_t, sum_r != sum_r ? NAN : m_r, (double)sum_r, a.V);
+            const RowResult r = row_result<64>(t, a.K, there, again, idx, s_k, a.lse != nullptr, inv_t, sum_r != sum_r ? NAN : m_r, sum_r, a.V);
             const double scale = (double)w * a.t;
             if (lane == 0) {
                 if (a.loss) a.loss[row] = (float)(r.loss * scale * a.t);
@@ -1046,7 +1051,8 @@ template <class T>
 __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
     constexpr int P = kPiece<T>, THREADS = 512, WAVES = 8, AHEAD = 4;
     extern __shared__ unsigned member[];                  // a bit per class
-    __shared__ float wave_max[WAVES], wave_part[WAVES];
+    __shared__ float wave_max[WAVES];
+    __shared__ double wave_part[WAVES];
     __shared__ float shared_coef;
     const int words = (a.V + 31) / 32, pieces = (a.V + P - 1) / P;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1077,7 +1083,8 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
             again = atomicOr(&member[idx >> 5], 1u << (idx & 31)) >> (idx & 31) & 1;
         }
         __syncthreads();
-        float m_own = -INFINITY, s_own = 0.0f;
+        float m_own = -INFINITY;
+        double s_own = 0.0;
         for (int q = tid; q < pieces; q += THREADS * AHEAD) {
             uintx4 raw[AHEAD];
             float v[AHEAD][P];
@@ -1097,11 +1104,13 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
                 }
             }
             const float base = m == -INFINITY ? 0.0f : m;
-            s_own = m_own == -INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((m_own - base) * c);
+            s_own = m_own == -INFINITY ? s_own : s_own * (double)__builtin_amdgcn_exp2f((m_own - base) * c);
+            float part_own = 0.0f;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-                for (int e = 0; e < P; ++e) s_own += __builtin_amdgcn_exp2f((v[i][e] - base) * c);
+                for (int e = 0; e < P; ++e) part_own += __builtin_amdgcn_exp2f((v[i][e] - base) * c);
+            s_own += (double)part_own;
             m_own = m;
         }
         float m_r = group_max<64>(m_own);
@@ -1111,12 +1120,12 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) m_r = fmaxf(m_r, wave_max[i]);
         const float base = m_r == -INFINITY ? 0.0f : m_r;
-        const float part = group_sum<64>(m_own == -INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((m_own - base) * c));
+        const double part = group_sum<64>(m_own == -INFINITY ? s_own : s_own * (double)__builtin_amdgcn_exp2f((m_own - base) * c));
         if (lane == 0) wave_part[wave] = part;
         __syncthreads();
         if (wave == 0) {
             double sum_r = 0.0;
-            for (int i = 0; i < WAVES; ++i) sum_r += (double)wave_part[i];
+            for (int i = 0; i < WAVES; ++i) sum_r += wave_part[i];
             const double scale = (double)w * a.t;
             const double inv_t = 1.0 / a.t;
             const Teacher t = teacher_of<64>(there, z, a.lse != nullptr, a.lse ? a.lse[row] : 0.0f, inv_t);

@@ -260,3 +260,21 @@ def test_entries_of_one_class_add_up(ctx, v, k, dtype, rest):
     if not rest:
         # p = q = 1 but for what 29 times exp(-70) and log 2's rounding leave; each of the two alone would give -log 2
         assert abs(float(out['loss'][5])) < 1e-6
+
+
+@pytest.mark.parametrize('v', [4000, 8000, 20001, 262144])
+def test_small_probabilities_beside_a_large_one_are_not_lost(ctx, v):
+    """One class at 0 and all others at -16.75, 2^-24.2 of it each: added to 1 one by one in float32 they are all lost.  The
+    largest class's gradient is 1 / S, S = 1 + (V - 1) e^-16.75: S may lose the up to 31 that share a float32 sum with the 1
+    (2^-24.1 each), its other terms are off by 2^-22 and 4u * 16.75 of themselves, and the gradient by 4u for its roundings."""
+    x = torch.full((3, v), -16.75)
+    i = torch.tensor([[v - 1], [1], [v // 2]], dtype=torch.int32)
+    for r, at in enumerate((0, v - 1, v // 3)):
+        x[r, at] = 0.0
+    out = ctx.distill_loss(x.cuda(), torch.zeros(3, 1).cuda(), i.cuda(), want_grad=True)
+    small = np.exp(-16.75)
+    s = 1.0 + (v - 1) * small
+    tol = 31 * small + (s - 1) * (2.0 ** -22 + 4 * U * 16.75) + 4 * U
+    tol = tol if v > 8192 else tol - 24 * small                  # rows in LDS: 4 classes share one
+    for r, at in enumerate((0, v - 1, v // 3)):
+        assert abs(float(out['grad'][r, at]) - 1.0 / s) <= tol, (r, float(out['grad'][r, at]) - 1.0 / s, tol)
