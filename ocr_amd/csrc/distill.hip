@@ -501,7 +501,8 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
     extern __shared__ uintx4 buf[];                        // the row
     __shared__ unsigned long long list[kTopList], wave_best[W];
     __shared__ unsigned wave_bits[W];
-    __shared__ float wave_top[W], wave_sum[W];
+    __shared__ float wave_top[W];
+    __shared__ double wave_sum[W];
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = (a.V + P - 1) / P;
     const float c = a.inv_t * kLog2e;
@@ -542,16 +543,17 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
         lds_phase();
         const float bound = least ? key_value(least) : -INFINITY;
         const float base = fabsf(high) == INFINITY ? 0.0f : high;
-        float sum = 0.0f;
+        double sum = 0.0;
         for (int q = tid; q < pieces; q += THREADS) {      // its own pieces
-            float v[P];
+            float v[P], part = 0.0f;
             unpack_piece(buf[q], v);
             bool any = false;
 #pragma unroll
             for (int e = 0; e < P; ++e) {
                 any |= !(v[e] < bound);                    // a NaN as well
-                sum += __builtin_amdgcn_exp2f((v[e] - base) * c);
+                part += __builtin_amdgcn_exp2f((v[e] - base) * c);
             }
+            sum += (double)part;
             if (any)
 #pragma unroll
                 for (int e = 0; e < P; ++e)
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
         const int n = count;
         if (a.lse && tid == THREADS - 1) {
             double total = 0.0;
-            for (int i = 0; i < W; ++i) total += (double)wave_sum[i];
+            for (int i = 0; i < W; ++i) total += wave_sum[i];
             a.lse[row] = (float)((double)base * a.inv_t + log_sum(total));
         }
         if (n <= kTopList) {
@@ -593,7 +595,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
     constexpr int P = kPiece<T>, WAVES = 8, THREADS = 512, AHEAD = 4;
     __shared__ unsigned long long list[kTopList];
     __shared__ unsigned maxima[THREADS];
-    __shared__ float wave_sum[WAVES];
+    __shared__ double wave_sum[WAVES];
     __shared__ unsigned long long wave_best[WAVES];
     __shared__ unsigned shared_bound, shared_exact;
     __shared__ float shared_high;
@@ -603,7 +605,8 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
     const float c = a.inv_t * kLog2e;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* p = a.x + row * a.ld;
-        float m_own = -INFINITY, s_own = 0.0f;             // running maximum and sum of the thread
+        float m_own = -INFINITY;                           // running maximum and sum of the thread
+        double s_own = 0.0;
         if (tid == 0) count = 0;
         for (int q = tid; q < pieces; q += THREADS * AHEAD) {
             uintx4 raw[AHEAD];
@@ -618,11 +621,13 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
 #pragma unroll
                 for (int e = 0; e < P; ++e) m = fmaxf(m, w[i][e]);
             const float base = fabsf(m) == INFINITY ? 0.0f : m;
-            s_own = fabsf(m_own) == INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((m_own - base) * c);
+            s_own = fabsf(m_own) == INFINITY ? s_own : s_own * (double)__builtin_amdgcn_exp2f((m_own - base) * c);
+            float part = 0.0f;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-                for (int e = 0; e < P; ++e) s_own += __builtin_amdgcn_exp2f((w[i][e] - base) * c);
+                for (int e = 0; e < P; ++e) part += __builtin_amdgcn_exp2f((w[i][e] - base) * c);
+            s_own += (double)part;
             m_own = m;
         }
         maxima[tid] = tid < pieces ? order_key(m_own) : 0u;
@@ -657,7 +662,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
                     }
             }
         const float own_base = fabsf(m_own) == INFINITY ? 0.0f : m_own;
-        const float sum = group_sum<64>(m_own == -INFINITY ? s_own : s_own * __builtin_amdgcn_exp2f((own_base - base) * c));
+        const double sum = group_sum<64>(m_own == -INFINITY ? s_own : s_own * (double)__builtin_amdgcn_exp2f((own_base - base) * c));
         if (lane == 0) wave_sum[wave] = sum;
         __syncthreads();
         const int n = count;
@@ -676,7 +681,7 @@ __global__ __launch_bounds__(512) void top_stream_kernel(TopArgs<T> a) {
         }
         if (a.lse && tid == 0) {
             double total = 0.0;
-            for (int w = 0; w < WAVES; ++w) total += (double)wave_sum[w];
+            for (int w = 0; w < WAVES; ++w) total += wave_sum[w];
             a.lse[row] = (float)((double)base * a.inv_t + log_sum(total));
         }
         __syncthreads();

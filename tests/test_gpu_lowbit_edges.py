@@ -278,3 +278,17 @@ def test_small_probabilities_beside_a_large_one_are_not_lost(ctx, v):
     tol = tol if v > 8192 else tol - 24 * small                  # rows in LDS: 4 classes share one
     for r, at in enumerate((0, v - 1, v // 3)):
         assert abs(float(out['grad'][r, at]) - 1.0 / s) <= tol, (r, float(out['grad'][r, at]) - 1.0 / s, tol)
+
+
+@pytest.mark.parametrize('v,k', [(4000, 8), (8000, 8), (500, 64), (20001, 8), (262144, 64)])
+def test_log_normaliser_of_small_probabilities_beside_a_large_one(ctx, v, k):
+    """The same rows: log S, S = 1 + (V - 1) e^-16.75, off by what S is off by relative to itself and half a step of the store."""
+    x = torch.full((3, v), -16.75)
+    for r, at in enumerate((0, v - 1, v // 3)):
+        x[r, at] = 0.0
+    small = np.exp(-16.75)
+    s = 1.0 + (v - 1) * small
+    tol = (31 if v > 8192 else 7) * small + (s - 1) * (2.0 ** -22 + 4 * U * 16.75) + U * np.log(s)
+    for dtype in (torch.float32, torch.bfloat16):                 # -16.75 has six bits
+        lse = ctx.top_logits(x.to(dtype).cuda(), k)[2].double().cpu().numpy()
+        assert (np.abs(lse - np.log(s)) <= tol).all(), (lse - np.log(s), tol)
