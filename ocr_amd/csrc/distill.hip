@@ -283,7 +283,7 @@ struct TopArgs {
 };
 
 // Every lane sorts its 8 classes, the lists go to LDS, and the K largest of the row are K times the largest head of 16 lists;
-// the winner writes its class down and moves on.  Bound by the vector ALU (1.4M rows of 97 float32, 10 entries: 315 us, 1.8
+// the winner writes its class down and moves on.  Bound by the vector ALU (1.4M rows of 97 float32, 10 entries: 328 us, 1.7
 // TB/s): the next row's loads are on their way, and a logit's key with its class (7 bits; among equals the lower class counts
 // as the larger) is held as the bits of a float64 between 1 and 2, which order like the numbers: two instructions sort a
 // pair.
@@ -493,8 +493,9 @@ __device__ __forceinline__ void write_one_by_one(const TopArgs<T>& a, int64_t ro
     }
 }
 
-// A row in LDS, W waves on it (FEW: as many maxima a lane as a piece has classes, one wave): bound by reading the logits (16384 rows of 6719 float32, 32 entries: 98 us, 4.5 TB/s).  The bound of the candidates: every wave bisects its own 64 maxima for the ceil(K / W)-th largest, the least
-// of those is reached by at least K values.
+// A row in LDS, W waves on it (FEW: as many maxima a lane as a piece has classes, one wave): bound by reading the logits (16384
+// rows of 6719 float32, 32 entries: 98 us, 4.5 TB/s).  The bound of the candidates: every wave bisects its own 64 maxima for
+// the ceil(K / W)-th largest, the least of those is reached by at least K values.
 template <class T, int W, int BATCH, bool FEW = false>
 __global__ __launch_bounds__(W * 64) void top_lds_kernel(TopArgs<T> a) {
     constexpr int P = kPiece<T>, THREADS = W * 64;
@@ -1165,15 +1166,15 @@ __global__ __launch_bounds__(512) void distill_stream_kernel(DistillArgs<T> a) {
 
 constexpr int64_t kMaxGrid = 1 << 20;          // workgroups of a launch; each walks the rows from there
 
-// Rows of up to 128 classes: 16 lanes a row (97 float32 classes, 10 entries, 1.4M rows 315 us, a wave a row 894; 0.7M rows and
-// 64 entries 446 against 821).
-// Rows in LDS: one wave up to 6 KB (float32, 32 entries, 134M classes in all: 1100 classes 205 us against 223 of two waves,
-// 1500 182 against 173, 2000 193 against 147), two up to 16 KB (4000 classes 134 against 141 of four, 208 of one), four up to
-// 32 KB (6719 classes 119 against 164 of two).  More than 32 entries need a second wave's maxima for a useful bound, where
-// the row has pieces for that many lanes (67M classes in all: 768 float32 classes, 64 entries 265 against 541); where it has
-// hardly more pieces than entries, a lane's maxima are taken class by class (FEW: 500 bfloat16 classes, 64 entries 207 against
-// 2145, 150 and 32 567 against 1059; with a few pieces more it costs: 500 and 32 180 against 122).  Beyond 32 KB, where a
-// compute unit would hold few rows: eight waves on a row that is read twice (8000 float32 classes: 176 against 129 in LDS).
+// Rows of up to 128 classes: 16 lanes a row (97 float32 classes, 10 entries, 1.4M rows 328 us, a wave a row 793; 0.7M rows and
+// 64 entries 455 against 703).
+// Rows in LDS: one wave up to 6 KB (float32, 32 entries, 134M classes in all: 1100 classes 205 us against 287 of two waves,
+// 1500 181 against 216, 2000 188 against 170), two up to 16 KB (4000 classes 135 against 162 of four, 203 of one), four up to
+// 32 KB (6719 classes 120 against 165 of two).  More than 32 entries need a second wave's maxima for a useful bound, where
+// the row has pieces for that many lanes (67M classes in all: 768 float32 classes, 64 entries 270 against 564); where it has
+// hardly more pieces than entries, a lane's maxima are taken class by class (FEW: 500 bfloat16 classes, 64 entries 223 against
+// 2212, 150 and 32 584 against 1069; with a few pieces more it costs: 500 and 32 180 against 123).  Beyond 32 KB, where a
+// compute unit would hold few rows: eight waves on a row that is read twice (8000 float32 classes: 178 against 128 in LDS).
 template <class T>
 int launch_top(const TopArgs<T>& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min(a.rows, kMaxGrid);
@@ -1203,12 +1204,12 @@ int launch_top(const TopArgs<T>& a, hipStream_t s) {
     return OCRHIP_OK;
 }
 
-// Rows of up to 128 classes: 16, 32 or 64 lanes a row, as many as entries (97 float32 classes, 1.4M rows, 10 entries: 344 us
-// against 1723 of a wave a row; 0.7M rows: 32 entries 292 against 672, 64 entries 559 against 677, where the row is also a
+// Rows of up to 128 classes: 16, 32 or 64 lanes a row, as many as entries (97 float32 classes, 1.4M rows, 10 entries: 365 us
+// against 1290 of a wave a row; 0.7M rows: 32 entries 298 against 666, 64 entries 568 against 681, where the row is also a
 // wave's but the next one's loads are on their way).  Rows in LDS: one wave up to 16 KB (float32, 32 entries, 134M classes in
-// all: 2000 classes 197 us against 251 of two waves, 418 of four; 4000 208 against 188 and 248; bfloat16 4000 classes 114
-// against 152), four up to 32 KB (6719 classes 198 against 263 of one, 203 of two).  Beyond: eight waves on a row that is read
-// twice (8000 float32 classes: 288 against 186 in LDS).
+// all: 1000 classes 225 us against 404 of two waves, 2000 195 against 288; 4000 214 against 195; bfloat16 4000 classes 112
+// against 157), four up to 32 KB (6719 classes 199 against 261 of one, 208 of two).  Beyond: eight waves on a row that is read
+// twice (8000 float32 classes: 284 against 190 in LDS).
 template <class T>
 int launch_distill(const DistillArgs<T>& a, hipStream_t s) {
     constexpr int P = kPiece<T>;

@@ -280,7 +280,7 @@ struct GemmArgs {
     int64_t M;
     int N, K;
     bool stream;         // rows of C are whole 128-byte lines: stored past the caches (131072 x 1024 float32 147 -> 113 us; rows that
-                         // share lines meet in the L2 instead: 141 us for 16384 x 6719, 188 past it)
+                         // share lines meet in the L2 instead: 141 us for 16384 x 6719, 188 past it), and partial sums like it
 };
 
 // scale byte -> the float whose exponent field it is (what the conversion below reads)
@@ -450,7 +450,8 @@ __device__ __forceinline__ void store_bf16x8(__bf16* p, bf16x8 v) {
 }
 
 // A workgroup walks its share of the tiles as one sequence of blocks of k: the first block of the next tile is on its way
-// while the last of this one is multiplied and the results leave.
+// while the last of this one is multiplied and the results leave (with a bias, whose loads are issued behind that block's, the
+// results wait for it).
 template <int BM, int BN, int WGM, int WGN, bool OUT_F32, int BROWS>
 __global__ __launch_bounds__(WGM * WGN * 64) void gemm_tile_kernel(TileArgs a) {
     constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, IM = TM / 16, IN = TN / 16;
@@ -741,9 +742,9 @@ struct TilePlan {
 // 44 against 40; 79872 x 256 x 512, 312 tiles, 36 against 25; 4096 x 3200 x 512, 208 tiles, 22 against 20).  float32 results
 // take 128 x 128 throughout.
 //
-// Pieces of k: a workgroup takes 1.05 us per block of k as long as it has its compute unit to itself and 1.6 us when two
-// share one; joining the pieces costs a launch, 2.5 us, and 0.27 us per MB of partial sums (written and read).  What comes
-// out least is taken, up to two workgroups per compute unit, for the 513th would make a second round of them all.  Measured
+// Pieces of k (both result types run the same loop): a workgroup takes 1.05 us per block of k as long as it has its compute
+// unit to itself and 1.6 us when two share one; joining the pieces costs a launch, 2.5 us, and 0.27 us per MB of partial sums
+// (written and read).  What comes out least is taken, up to two workgroups per compute unit, for the 513th would make a second round of them all.  Measured
 // against one piece: 300 x 97 x 2048 10 us / 22, 256 x 256 x 131072 33 / 1087, 6719 x 256 x 16384 73 / 142; where one piece
 // stays, against two: 1900 x 1900 x 2048 26 / 32, 1000 x 1000 x 1024 14 / 16.
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, bool out_f32) {
