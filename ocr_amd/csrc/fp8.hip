@@ -16,7 +16,7 @@
 // products of a group of neighbouring values of k (at most 16) aligned to the largest of them and keep 13 bits below it
 // (measured, with and without scales: a product 2^-14 of its neighbour's is lost, one 16 places further is not).  448 * 448 -
 // 448 * 448 + 4 gave 0, and 3.8 % of a large product's bfloat16 results were other roundings than those of float32 sums.  The
-// price: 8192^3 into bfloat16 takes 875 us instead of 440, 2048^3 23 instead of 15, 79872 x 256 x 512 25 as before.
+// price: 8192^3 into bfloat16 takes 794 us instead of 440, 2048^3 23 instead of 15, 79872 x 256 x 512 25 as before.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -408,8 +408,8 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int waves_k)
 // beyond the descriptor: zeros.
 // B is the matrix instruction's row operand, A its column operand: a lane then holds 4 neighbouring columns of one row.
 //
-// Measured: bound by the conversions and matrix instructions beside the operands' loads, 8192^3 into bfloat16 875 us (1.26
-// PFLOP/s; a large bfloat16 library product reaches 1.37), 6719 x 256 x 16384 into float32 73 us (0.78 PFLOP/s with the join of
+// Measured: bound by the conversions and matrix instructions beside the operands' loads, 8192^3 into bfloat16 794 to 875 us (1.26
+// to 1.38 PFLOP/s; a large bfloat16 library product reaches 1.37), 6719 x 256 x 16384 into float32 73 us (0.78 PFLOP/s with the join of
 // 4 pieces).  16384 x 6719 x 256 into float32: 108 us with rows of whole lines (6720 columns apart: 4.1 TB/s, bound by
 // writing), 141 us with rows that start anywhere in one, whose ends two tiles write.
 struct TileArgs {
