@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <new>
 
 #include "common.h"
 
@@ -672,7 +673,12 @@ static int prepare_dense_fp8(ConvLayer& L) {
 // option fp8_dense: all of them, from the float32 weights on the device; the ResNet recogniser does not know the option
 static int crnn_prepare_fp8(CrnnNet& net) {
     if (net.backbone || net.fp8_ready) return OCRHIP_OK;
-    for (ConvLayer* L : {&net.wih[0][0], &net.wih[0][1], &net.wih[1][0], &net.wih[1][1], &net.linear[0], &net.linear[1], &net.pred}) OCR_TRY(prepare_dense_fp8(*L));
+    try {
+        for (ConvLayer* L : {&net.wih[0][0], &net.wih[0][1], &net.wih[1][0], &net.wih[1][1], &net.linear[0], &net.linear[1], &net.pred}) OCR_TRY(prepare_dense_fp8(*L));
+    } catch (const std::bad_alloc&) {                          // no exception leaves a C entry
+        set_error("fp8_dense: no host memory for a layer's weights");
+        return OCRHIP_ECAP;
+    }
     net.fp8_ready = true;
     return OCRHIP_OK;
 }
