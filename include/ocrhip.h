@@ -374,7 +374,7 @@ int ocrhip_ctc_beam_search(ocrhip_handle h, const float* d_logits, int B, int T,
  * Block-scaled 8-bit matrix of R rows and C columns: row r at d_q + r * ld_q, OCP e4m3 bytes (8 bits, no infinities),
  * the columns from C up to the next multiple of 128 zero; the scale of the block (row block i, column block j) is the
  * byte d_scale[j * ld_scale + i] = exponent + 127, column blocks being 128 columns and row blocks `block_rows` rows (1 or
- * 128): the element (r, c) stands for q[r][c] * 2^(d_scale[(c / 128) * ld_scale + r / block_rows] - 127).
+ * 128): the element (r, c) stands for q[r][c] * 2^(d_scale[(c / 128) * ld_scale + r / block_rows] - 127), 255 for NaN.
  *   ld_q: multiple of 128, >= C;  ld_scale: multiple of 16, >= the number of row blocks;  both pointers 16-byte aligned.
  *
  * ocrhip_quantize_fp8: x (rows, cols), or its transpose, as such a matrix.  The exponent of a block is the least e with

@@ -131,6 +131,37 @@ def test_operands_are_the_last_columns_of_wider_buffers(ctx, mnk, block_rows, ou
     assert torch.equal(ctx.gemm_fp8(*wide, out_dtype=out_dtype), ctx.gemm_fp8(a, w, out_dtype=out_dtype))
 
 
+@pytest.mark.parametrize('out_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('m', [5, 200])
+def test_a_scale_of_255_makes_its_block_nan(ctx, m, out_dtype):
+    """In the scales of either operand: that row or column of the product and nothing else, zeros in the block included."""
+    a, b = ctx.quantize_fp8(torch.randn(m, 300).cuda()), ctx.quantize_fp8(torch.zeros(40, 300).cuda())
+    a.scale[1, m // 2], b.scale[2, 7] = 255, 255
+    bad = torch.isnan(ctx.gemm_fp8(a, b, out_dtype=out_dtype))
+    assert bad[m // 2].all() and bad[:, 7].all() and int(bad.sum()) == 40 + m - 1
+
+
+@pytest.mark.parametrize('block_rows', [1, 128])
+@pytest.mark.parametrize('transpose', [False, True])
+def test_quantise_beyond_32_bits(ctx, transpose, block_rows):
+    """More than 2^31 elements in and bytes out: the first and last rows equal those of a matrix of their own."""
+    rows, cols = 65536 + 256, 33000
+    part = torch.randn(256, cols, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    want = ctx.quantize_fp8(part, block_rows=block_rows, transpose=transpose)
+    x = part.repeat(rows // 256, 1)
+    assert x.numel() > 2 ** 31
+    got = ctx.quantize_fp8(x, block_rows=block_rows, transpose=transpose)
+    del x
+    for first in (0, 256 * (rows // 512), rows - 256):
+        if transpose:
+            assert torch.equal(got.q.view(torch.uint8)[:, first:first + 256], want.q.view(torch.uint8))
+            assert torch.equal(got.scale[first // 128:first // 128 + 2, :-(-cols // block_rows)], want.scale[:, :-(-cols // block_rows)])
+        else:
+            blocks = 256 // block_rows
+            assert torch.equal(got.q.view(torch.uint8)[first:first + 256], want.q.view(torch.uint8))
+            assert torch.equal(got.scale[:, first // block_rows:first // block_rows + blocks], want.scale[:, :blocks])
+
+
 # ---------------------------------------------------------------------------------- distillation
 # one row length for each form: 16, 32 and 64 lanes a row, a row in LDS on one wave and on four, a row read twice
 FORMS = [(97, 6), (97, 30), (97, 50), (3, 3), (3, 20), (1000, 6), (6719, 6), (40000, 6)]
